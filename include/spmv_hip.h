@@ -43,6 +43,8 @@ struct mtx { int i; int j; double a; };
 typedef struct spmv_hip_matrix spmv_hip_matrix;
 
 enum { SPMV_HIP_F64 = 0, SPMV_HIP_F32 = 1 };
+/* further element types of the vectors that the 8-bit block functions take */
+enum { SPMV_HIP_BF16 = 2, SPMV_HIP_F16 = 3, SPMV_HIP_E4M3 = 4 };
 
 /* storage format + kernel of a handle */
 enum {
@@ -53,13 +55,14 @@ enum {
     SPMV_HIP_SELL       = 4,  /* SELL-C-sigma                        (mult_sell,      sell.c:35-42)  */
     SPMV_HIP_SELLP      = 5,  /* sliced ELL, natural row order       (mult_sellp,     sellp.c:304-342) */
     SPMV_HIP_ELL        = 6,  /* sliced ELL, natural row order       (mult_ell,       ell.c:28-45)   */
-    SPMV_HIP_SELL_DFC   = 7   /* SELL-C-sigma without padding: active lanes per column (csr_to_sellcs_dfc, sellcs_format.c:53-136) */
+    SPMV_HIP_SELL_DFC   = 7,  /* SELL-C-sigma without padding: active lanes per column (csr_to_sellcs_dfc, sellcs_format.c:53-136) */
+    SPMV_HIP_BLOCK8     = 8   /* 128 x 128 blocks of 8-bit values, one scale each (no reference counterpart) */
 };
 
 /* arrays that spmv_hip_download() can read back (layout parity tests) */
 enum {
-    SPMV_HIP_ARR_ROW_PTR    = 0,  /* int32  [rows+1]            CSR family                       */
-    SPMV_HIP_ARR_COL        = 1,  /* int32  [stored]            CSR col / sliced column_indices  */
+    SPMV_HIP_ARR_ROW_PTR    = 0,  /* int32  [rows+1]            CSR family; BLOCK8: block_ptr [ceil(rows/128)+1] */
+    SPMV_HIP_ARR_COL        = 1,  /* int32  [stored]            CSR col / sliced column_indices; BLOCK8: block_col [nblocks] */
     SPMV_HIP_ARR_VAL        = 2,  /* dtype  [stored]            CSR val / sliced values          */
     SPMV_HIP_ARR_SLICE_PTR  = 3,  /* int64  [nslices+1]         sliced formats (slice_pointers / block_ptr) */
     SPMV_HIP_ARR_ROW_ORDER  = 4,  /* int32  [rows]              SELL only (row_order)            */
@@ -350,6 +353,76 @@ int spmv_hip_dist_get_peer_access(const spmv_hip_dist *d, int *access);
 /* ngpus, bounds[0..ngpus], blocks[0..ngpus) -- any of them may be NULL */
 int spmv_hip_dist_get_info(const spmv_hip_dist *d, int *ngpus, int *bounds, spmv_hip_rowblock_info *blocks);
 int spmv_hip_dist_free(spmv_hip_dist *d);
+
+/* ---- matrices of 128 x 128 blocks in 8 bits --------------------------------------
+ * No reference counterpart (its values are double).  For matrices whose stored
+ * entries come in whole blocks and whose values tolerate 8 bits: the layers of a
+ * neural network, pruned block by block or full.
+ *
+ * Number format.  Values are e4m3 (OCP: 4 exponent bits, 3 mantissa bits, no
+ * infinities, largest finite 448).  A group of values shares one scale 2^(b-127),
+ * kept as the byte b, 1 <= b <= 254.  The scale of a group is the least power of
+ * two >= 2^-126 that brings its largest finite magnitude to at most 448 (1 for a
+ * group of zeros), and a value is x / scale rounded to nearest even: dividing by
+ * the scale is exact, so that rounding is the only one.  Infinities and NaN become
+ * NaN and do not count for the scale.  Groups are the matrix's blocks, and 128
+ * consecutive entries of a vector.
+ *
+ * The matrix: block k covers rows 128 I .. 128 I + 127 (I = its block row) and
+ * columns 128 block_col[k] .. + 127; positions beyond the matrix's edge hold zero,
+ * whatever set_values / load are given there.  Blocks of a block row may come in
+ * any order; two blocks at one place add up.
+ *
+ * Vectors: vector v starts at p + v * ld (ld in elements).  In 8 bits (SPMV_HIP_E4M3)
+ * ld8 is a multiple of 128 and >= columns rounded up to 128, the base is 16-byte
+ * aligned, the bytes past `columns` are zero (spmv_hip_quantize8_dev writes them),
+ * and scale[g * lds + v] is the scale byte of its entries 128 g .. 128 g + 127
+ * (lds >= n).  In F32, BF16 or F16 nothing is asked of the alignment beyond the
+ * element's own; 16-byte aligned bases and strides are faster.
+ *
+ * All calls are asynchronous on `stream`, allocate nothing and may be captured
+ * into a graph; they keep nothing in the handle, so that products on one handle
+ * may overlap.  n = 0 is allowed.  spmv_hip_mult, _mult_dev, _mult_mv, _mult_mv_dev
+ * and _bench take such a handle too (dtype F32): x is rounded to 8 bits on its way
+ * in.  "variant", "block_map" and "hot_columns" do not apply. */
+
+/* block_ptr[0 .. ceil(rows/128)], block_col[0 .. nblocks): host arrays, like row_ptr
+ * and col of a CSR matrix.  All values are zero until one of the next two calls. */
+spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, const int *block_ptr, const int *block_col);
+/* d_values[nblocks][128][128] (F32, BF16 or F16, row-major inside a block): rounds
+ * every block to 8 bits with its own scale. */
+int spmv_hip_block8_set_values_dev(spmv_hip_matrix *m, const void *d_values, int dtype, void *stream);
+/* 8-bit values and scale bytes as they are: d_values8[nblocks][128][128], d_scale[nblocks]. */
+int spmv_hip_block8_load_dev(spmv_hip_matrix *m, const uint8_t *d_values8, const uint8_t *d_scale, void *stream);
+/* The reverse of load. */
+int spmv_hip_block8_store_dev(const spmv_hip_matrix *m, uint8_t *d_values8, uint8_t *d_scale, void *stream);
+
+/* x (n vectors of F32, BF16 or F16) to 8 bits, and back.  The pair keeps an
+ * activation between a layer's forward and backward pass at a half (a quarter)
+ * of its size.  restore8 gives value * scale in `dtype`, the largest finite number
+ * of `dtype` (with its sign) where that overflows. */
+int spmv_hip_quantize8_dev(int n, int columns, const void *d_x, int dtype, int64_t ldx, uint8_t *d_x8, int64_t ldx8,
+                           uint8_t *d_scale, int64_t lds, void *stream);
+int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds,
+                          void *d_x, int dtype, int64_t ldx, void *stream);
+
+/* y_v = A x_v (mult_mv_csr, spmv.h:54, for this format).  x_dtype E4M3: x in 8 bits
+ * with its scales; otherwise x is F32, BF16 or F16, d_scale is NULL, x is rounded to
+ * 8 bits inside the product, and n is at most SPMV_HIP_BLOCK8_MAX_WIDE (quantize
+ * larger blocks of vectors first).  y in F32, BF16 or F16. */
+enum { SPMV_HIP_BLOCK8_MAX_WIDE = 64 };
+int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, int x_dtype, int64_t ldx,
+                             const uint8_t *d_scale, int64_t lds, void *d_y, int y_dtype, int64_t ldy, void *stream);
+/* dx_v = A^T dy_v: the gradient of the product's input.  dy and dx in F32, BF16 or
+ * F16; dy is used as it is, not rounded to 8 bits. */
+int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, void *d_dx,
+                               int dx_dtype, int64_t lddx, void *stream);
+/* The gradient of the stored blocks: d_dvalues[k][r][c] = sum over v of
+ * dy_v[128 I_k + r] * x_v[128 J_k + c], x as its 8-bit checkpoint; zero beyond the
+ * matrix's edge.  accumulate != 0 adds to what d_dvalues holds. */
+int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
+                                 const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dvalues,
+                                 int dtype, int accumulate, void *stream);
 
 /* free_X (csr.c:205-210, sellp.c:461-465; the reference leaks the others) */
 int spmv_hip_free(spmv_hip_matrix *m);

@@ -13,11 +13,12 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspmv_hip.so")
 
 F64, F32 = 0, 1
-CSR_SCALAR, CSR_VECTOR, CSR_MERGE, CSR_BAL, SELL, SELLP, ELL, SELL_DFC = range(8)
+BF16, F16, E4M3 = 2, 3, 4             # further element types of the vectors of an 8-bit block matrix
+CSR_SCALAR, CSR_VECTOR, CSR_MERGE, CSR_BAL, SELL, SELLP, ELL, SELL_DFC, BLOCK8 = range(9)
 ARR_ROW_PTR, ARR_COL, ARR_VAL, ARR_SLICE_PTR, ARR_ROW_ORDER, ARR_TILE_COORD, ARR_VOP_PTR, ARR_VOP_LEN = range(8)
 
 FORMAT_NAMES = {CSR_SCALAR: "csr_scalar", CSR_VECTOR: "csr_vector", CSR_MERGE: "csr_merge",
-                CSR_BAL: "csr_bal", SELL: "sell", SELLP: "sellp", ELL: "ell", SELL_DFC: "sell_dfc"}
+                CSR_BAL: "csr_bal", SELL: "sell", SELLP: "sellp", ELL: "ell", SELL_DFC: "sell_dfc", BLOCK8: "block8"}
 
 
 class Info(C.Structure):
@@ -62,6 +63,15 @@ SIGNATURES = {
     "spmv_hip_mult_dev": (_i, [_vp, _vp, _vp, _vp]),
     "spmv_hip_mult_mv": (_i, [_vp, _i, _vp, _vp]),
     "spmv_hip_mult_mv_dev": (_i, [_vp, _i, _vp, C.c_int64, _vp, C.c_int64, _vp]),
+    "spmv_hip_create_block8": (_vp, [_i, _i, _i, _vp, _vp]),
+    "spmv_hip_block8_set_values_dev": (_i, [_vp, _vp, _i, _vp]),
+    "spmv_hip_block8_load_dev": (_i, [_vp, _vp, _vp, _vp]),
+    "spmv_hip_block8_store_dev": (_i, [_vp, _vp, _vp, _vp]),
+    "spmv_hip_quantize8_dev": (_i, [_i, _i, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "spmv_hip_restore8_dev": (_i, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i, _i64, _vp]),
+    "spmv_hip_block8_mult_dev": (_i, [_vp, _i, _vp, _i, _i64, _vp, _i64, _vp, _i, _i64, _vp]),
+    "spmv_hip_block8_mult_t_dev": (_i, [_vp, _i, _vp, _i, _i64, _vp, _i, _i64, _vp]),
+    "spmv_hip_block8_gradient_dev": (_i, [_vp, _i, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i, _vp]),
     "spmv_hip_set_row_map": (_i, [_vp, _vp]),
     "spmv_hip_free": (_i, [_vp]),
     "spmv_hip_bench": (_i, [_vp, _i, C.c_double, _vp, C.POINTER(_i), C.POINTER(C.c_double)]),

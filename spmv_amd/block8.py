@@ -1,0 +1,253 @@
+"""Matrices of 128 x 128 blocks in 8 bits: a layer's product, both its gradients, and 8-bit checkpoints of activations.
+
+The host side of the `spmv_hip_block8_*` / `_quantize8_` / `_restore8_` calls of include/spmv_hip.h on torch tensors.
+Vectors are the rows of a tensor [..., columns]; every call runs on the device of its tensors, on torch's current stream
+there, and is checked here before the library sees an address.
+
+    A = Block8(rows, columns, block_ptr, block_col)   # which blocks are stored, as a CSR pattern of blocks
+    A.set_values(w)                                   # w [blocks, 128, 128], rounded to 8 bits block by block
+    y = A.linear(x)                                   # differentiable in x and w; keeps x in 8 bits until backward
+    y = A.product(x)                                  # the product alone
+
+Number format (include/spmv_hip.h has the definition): e4m3 values, one power-of-two scale per block of the matrix and per
+128 consecutive entries of a vector, kept as the byte b of 2^(b-127).  Gradients are those of the product with the
+rounded operands (the rounding itself counts as the identity).
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from .matrix import Matrix
+
+BLOCK = 128
+MAX_WIDE = 64                         # vectors a product rounds to 8 bits by itself (SPMV_HIP_BLOCK8_MAX_WIDE)
+_DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _wide(name: str, x: torch.Tensor, length: int | None = None) -> torch.Tensor:
+    """x as [n, length] rows that are contiguous inside (any distance apart); copies only what has no such view."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPE:
+        raise TypeError(f"{name} must be a float32, bfloat16 or float16 tensor")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be on a GPU; there is no CPU path")
+    if x.dim() < 1 or (length is not None and x.shape[-1] != length):
+        raise ValueError(f"{name} has shape {tuple(x.shape)}, expected (..., {length})")
+    if x.dim() != 2:
+        x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()                       # transposed or broadcast rows
+    return x
+
+
+def _ld(x: torch.Tensor) -> int:
+    return max(x.stride(0), x.shape[1])
+
+
+class Packed8:
+    """n vectors in 8 bits: `values` uint8 [n, columns rounded up to 128] (zero past `columns`), `scale` uint8
+    [groups, n], `dtype` of the vectors it was made from."""
+
+    __slots__ = ("values", "scale", "columns", "dtype", "shape")
+
+    def __init__(self, values: torch.Tensor, scale: torch.Tensor, columns: int, dtype: torch.dtype, shape=None):
+        groups = -(-columns // BLOCK)
+        if dtype not in _DTYPE:
+            raise TypeError("dtype must be float32, bfloat16 or float16")
+        if values.dtype != torch.uint8 or values.dim() != 2 or values.shape[1] != groups * BLOCK or not values.is_contiguous():
+            raise ValueError(f"values must be a contiguous uint8 tensor [n, {groups * BLOCK}]")
+        if scale.dtype != torch.uint8 or tuple(scale.shape) != (groups, values.shape[0]) or not scale.is_contiguous():
+            raise ValueError(f"scale must be a contiguous uint8 tensor [{groups}, {values.shape[0]}]")
+        if not values.is_cuda or scale.device != values.device:
+            raise ValueError("values and scale must be on one GPU")
+        self.values, self.scale, self.columns, self.dtype = values, scale, columns, dtype
+        self.shape = tuple(shape) if shape is not None else (values.shape[0], columns)
+
+    @property
+    def n(self) -> int:
+        return self.values.shape[0]
+
+    def restore(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The vectors their 8-bit form stands for, in the shape they came in."""
+        dtype = dtype or self.dtype
+        if dtype not in _DTYPE:
+            raise TypeError("dtype must be float32, bfloat16 or float16")
+        x = torch.empty(self.shape, dtype=dtype, device=self.values.device)
+        with torch.cuda.device(x.device):
+            L.check(L.lib().spmv_hip_restore8_dev(self.n, self.columns, self.values.data_ptr(), self.values.shape[1],
+                                                  self.scale.data_ptr(), self.n, x.data_ptr(), _DTYPE[dtype], self.columns,
+                                                  _stream(x.device)))
+        return x
+
+
+def quantize(x: torch.Tensor) -> Packed8:
+    """x [..., columns] to 8 bits."""
+    rows = _wide("x", x.detach() if isinstance(x, torch.Tensor) else x)
+    n, columns = rows.shape
+    groups = -(-columns // BLOCK)
+    values = torch.empty((n, groups * BLOCK), dtype=torch.uint8, device=rows.device)
+    scale = torch.empty((groups, n), dtype=torch.uint8, device=rows.device)
+    with torch.cuda.device(rows.device):
+        L.check(L.lib().spmv_hip_quantize8_dev(n, columns, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows), values.data_ptr(),
+                                               groups * BLOCK, scale.data_ptr(), n, _stream(rows.device)))
+    return Packed8(values, scale, columns, rows.dtype, x.shape)
+
+
+class Block8(Matrix):
+    """A handle of 8-bit blocks on the current device.  block_ptr [ceil(rows / 128) + 1] and block_col are host integers
+    like the row_ptr and col of a CSR matrix, in units of blocks."""
+
+    def __init__(self, rows: int, columns: int, block_ptr, block_col):
+        ptr = np.ascontiguousarray(block_ptr, np.int32)
+        col = np.ascontiguousarray(block_col, np.int32)
+        if ptr.shape != (-(-max(rows, 0) // BLOCK) + 1,) or col.ndim != 1:
+            raise ValueError(f"block_ptr has shape {ptr.shape} for {rows} rows, block_col {col.shape}")
+        super().__init__(L.lib().spmv_hip_create_block8(rows, columns, len(col), ptr.ctypes.data, col.ctypes.data))
+        self.rows, self.columns, self.nblocks = rows, columns, len(col)
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self.values = None               # the tensor set_values last took: the leaf that linear() differentiates
+        self._version = 0                # set_values / load calls so far
+
+    @classmethod
+    def full(cls, rows: int, columns: int) -> "Block8":
+        """Every block stored."""
+        brows, bcols = -(-rows // BLOCK), -(-columns // BLOCK)
+        return cls(rows, columns, np.arange(brows + 1) * bcols, np.tile(np.arange(bcols), brows))
+
+    def _here(self, name: str, t: torch.Tensor) -> None:
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, the matrix on {self.device}")
+
+    def _blocks(self, name: str, t: torch.Tensor, dtypes) -> None:
+        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+            raise TypeError(f"{name} must be a tensor of one of {sorted(str(d) for d in dtypes)}")
+        if tuple(t.shape) != (self.nblocks, BLOCK, BLOCK) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [{self.nblocks}, 128, 128], has shape {tuple(t.shape)}")
+        self._here(name, t)
+
+    def _out(self, out, shape, dtype, like: torch.Tensor):
+        if dtype not in _DTYPE:
+            raise TypeError("the result's type must be float32, bfloat16 or float16")
+        if out is None:
+            return torch.empty(shape, dtype=dtype, device=like.device)
+        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous {tuple(shape)} of {dtype}")
+        self._here("out", out)
+        return out
+
+    def set_values(self, values: torch.Tensor) -> None:
+        """Rounds values [blocks, 128, 128] into the matrix.  linear() returns the gradient of this tensor."""
+        self._blocks("values", values, _DTYPE)
+        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _stream(self.device)))
+        self.values = values
+        self._version += 1
+
+    def load(self, values8: torch.Tensor, scale: torch.Tensor) -> None:
+        """8-bit values [blocks, 128, 128] (uint8 or float8_e4m3fn) and scale bytes uint8 [blocks] as they are."""
+        self._blocks("values8", values8, (torch.uint8, torch.float8_e4m3fn))
+        if scale.dtype != torch.uint8 or tuple(scale.shape) != (self.nblocks,) or not scale.is_contiguous():
+            raise ValueError(f"scale must be a contiguous uint8 tensor [{self.nblocks}]")
+        self._here("scale", scale)
+        L.check(L.lib().spmv_hip_block8_load_dev(self._h, values8.data_ptr(), scale.data_ptr(), _stream(self.device)))
+        self.values = None
+        self._version += 1
+
+    def store(self):
+        """(values8 uint8 [blocks, 128, 128], scale uint8 [blocks]): what load takes."""
+        values8 = torch.empty((self.nblocks, BLOCK, BLOCK), dtype=torch.uint8, device=self.device)
+        scale = torch.empty(self.nblocks, dtype=torch.uint8, device=self.device)
+        L.check(L.lib().spmv_hip_block8_store_dev(self._h, values8.data_ptr(), scale.data_ptr(), _stream(self.device)))
+        return values8, scale
+
+    def product(self, x, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """y[..., rows] = A x for the vectors of x: a tensor [..., columns] (rounded to 8 bits on the way in) or a
+        Packed8.  `dtype` of y: that of x unless given."""
+        if not isinstance(x, Packed8):
+            rows = _wide("x", x.detach() if isinstance(x, torch.Tensor) else x, self.columns)
+            self._here("x", rows)
+            shape = (*x.shape[:-1], self.rows)
+            if rows.shape[0] <= MAX_WIDE:
+                y = self._out(out, shape, dtype or rows.dtype, rows)
+                L.check(L.lib().spmv_hip_block8_mult_dev(self._h, rows.shape[0], rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
+                                                         None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self.device)))
+                return y
+            dtype = dtype or rows.dtype
+            x = quantize(rows)
+        else:
+            if x.columns != self.columns:
+                raise ValueError(f"x has {x.columns} columns, the matrix {self.columns}")
+            self._here("x", x.values)
+            shape = (*x.shape[:-1], self.rows)
+        y = self._out(out, shape, dtype or x.dtype, x.values)
+        L.check(L.lib().spmv_hip_block8_mult_dev(self._h, x.n, x.values.data_ptr(), L.E4M3, x.values.shape[1], x.scale.data_ptr(),
+                                                 x.n, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self.device)))
+        return y
+
+    def product_t(self, dy: torch.Tensor, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """dx[..., columns] = A^T dy for dy [..., rows]; dy is not rounded."""
+        d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
+        self._here("dy", d)
+        dx = self._out(out, (*dy.shape[:-1], self.columns), dtype or d.dtype, d)
+        L.check(L.lib().spmv_hip_block8_mult_t_dev(self._h, d.shape[0], d.data_ptr(), _DTYPE[d.dtype], _ld(d), dx.data_ptr(),
+                                                   _DTYPE[dx.dtype], self.columns, _stream(self.device)))
+        return dx
+
+    def gradient(self, dy: torch.Tensor, x: Packed8, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                 accumulate: bool = False) -> torch.Tensor:
+        """The gradient of the stored blocks [blocks, 128, 128] from dy [..., rows] and the 8-bit x of the product."""
+        d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
+        self._here("dy", d)
+        if not isinstance(x, Packed8):
+            raise TypeError("x must be a Packed8 (quantize)")
+        if x.columns != self.columns or x.n != d.shape[0]:
+            raise ValueError(f"x holds {x.n} vectors of {x.columns}, dy {d.shape[0]} for a matrix of {self.columns} columns")
+        self._here("x", x.values)
+        if accumulate and out is None:
+            raise ValueError("accumulate adds to out, which is missing")
+        dv = self._out(out, (self.nblocks, BLOCK, BLOCK), out.dtype if out is not None else dtype, d)
+        L.check(L.lib().spmv_hip_block8_gradient_dev(self._h, d.shape[0], d.data_ptr(), _DTYPE[d.dtype], _ld(d), x.values.data_ptr(),
+                                                     x.values.shape[1], x.scale.data_ptr(), x.n, dv.data_ptr(), _DTYPE[dv.dtype],
+                                                     int(accumulate), _stream(self.device)))
+        return dv
+
+    def linear(self, x: torch.Tensor) -> torch.Tensor:
+        """y = A x, differentiable in x and in the tensor that set_values took.  Between the passes x is kept in 8 bits;
+        the backward pass refuses a matrix whose values were set again meanwhile."""
+        if not isinstance(x, torch.Tensor):
+            raise TypeError("x must be a tensor")
+        if torch.is_grad_enabled() and (x.requires_grad or self.values is not None and self.values.requires_grad):
+            return _Linear.apply(x, self.values, self)
+        return self.product(x)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, values, matrix):
+        _wide("x", x, matrix.columns)
+        matrix._here("x", x)
+        q = quantize(x)
+        ctx.save_for_backward(q.values, q.scale)
+        ctx.matrix, ctx.version, ctx.x_shape, ctx.x_dtype = matrix, matrix._version, x.shape, x.dtype
+        ctx.values_dtype = values.dtype if values is not None else None
+        return matrix.product(q)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        values8, scale = ctx.saved_tensors
+        matrix = ctx.matrix
+        if matrix._version != ctx.version:
+            raise RuntimeError("the values of the 8-bit matrix were set again between forward and backward")
+        dx = matrix.product_t(dy, ctx.x_dtype) if ctx.needs_input_grad[0] else None
+        dv = None
+        if ctx.needs_input_grad[1]:
+            dv = matrix.gradient(dy, Packed8(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), ctx.values_dtype)
+        return dx, dv, None

@@ -486,7 +486,8 @@ int spmv_hip_free(spmv_hip_matrix *m)
     release_csr(m);
     void *ptrs[] = {m->d_tile_coord, m->d_row_carry, m->d_val_carry, m->d_nzr_id, m->d_nzr_end, m->d_slice_ptr,
                     m->d_row_order, m->d_scol, m->d_sval, m->d_sorted_len, m->d_vop_ptr, m->d_vop_len,
-                    m->d_x, m->d_y, m->d_norm, m->d_hot_col, m->d_hot_old, m->d_hot_x, m->d_xcd_y, m->d_xcd_presence, m->d_xcd_base, m->d_sdiag, m->d_block_pat, m->d_tile_pat};
+                    m->d_x, m->d_y, m->d_norm, m->d_hot_col, m->d_hot_old, m->d_hot_x, m->d_xcd_y, m->d_xcd_presence, m->d_xcd_base, m->d_sdiag, m->d_block_pat, m->d_tile_pat,
+                    m->d_block_ptr, m->d_block_col, m->d_block_row, m->d_bt_ptr, m->d_bt_row, m->d_bt_id, m->d_val8, m->d_scale8};
     if (m->xcd_sub) spmv_hip_free(m->xcd_sub);
     for (void *p : ptrs)
         if (p) (void)hipFree(p);
@@ -643,6 +644,10 @@ int spmv_hip_set_option(spmv_hip_matrix *m, const char *name, int64_t value)
     if (!m || !name) { set_error("NULL argument"); return 1; }
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
+    if (m->format == SPMV_HIP_BLOCK8 && strcmp(name, "exact_order")) {
+        set_error("option '%s' does not apply to 8-bit blocks", name);
+        return 1;
+    }
     if (!strcmp(name, "variant")) { m->variant = (int)value; return 0; }
     if (!strcmp(name, "block_map")) {
         if (value < 0 || value > (1 << 20)) { set_error("block_map takes 0, 1 or a run length up to 2^20"); return 1; }
@@ -940,8 +945,10 @@ int spmv_hip_download(const spmv_hip_matrix *m, int which, void *host, size_t by
     if (!m || !host) { set_error("NULL argument"); return 1; }
     const void *src = nullptr;
     size_t need = 0;
-    const bool sliced = m->d_slice_ptr != nullptr;
-    switch (which) {
+    const bool sliced = m->d_slice_ptr != nullptr, block8 = m->format == SPMV_HIP_BLOCK8;
+    switch (block8 ? which + 100 : which) {
+    case 100 + SPMV_HIP_ARR_ROW_PTR: src = m->d_block_ptr; need = sizeof(int) * ((size_t)m->brows + 1); break;
+    case 100 + SPMV_HIP_ARR_COL: src = m->d_block_col; need = sizeof(int) * (size_t)m->nblocks; break;
     case SPMV_HIP_ARR_ROW_PTR: src = m->d_row_ptr; need = sizeof(int) * ((size_t)m->rows + 1); break;
     case SPMV_HIP_ARR_COL: src = sliced ? m->d_scol : m->d_col; need = sizeof(int) * (size_t)m->stored; break;
     case SPMV_HIP_ARR_VAL: src = sliced ? m->d_sval : m->d_val; need = dtype_size(m->dtype) * (size_t)m->stored; break;
@@ -950,7 +957,10 @@ int spmv_hip_download(const spmv_hip_matrix *m, int which, void *host, size_t by
     case SPMV_HIP_ARR_TILE_COORD: src = m->d_tile_coord; need = sizeof(int) * 2 * ((size_t)m->ntiles + 1); break;
     case SPMV_HIP_ARR_VOP_PTR: src = m->d_vop_ptr; need = sizeof(int64_t) * ((size_t)m->nslices + 1); break;
     case SPMV_HIP_ARR_VOP_LEN: src = m->d_vop_len; need = (size_t)m->vops; break;
-    default: set_error("unknown array id %d", which); return 1;
+    default:
+        if (block8) set_error("array %d is not part of format %d", which, m->format);
+        else set_error("unknown array id %d", which);
+        return 1;
     }
     if (!src) { set_error("array %d is not part of format %d", which, m->format); return 1; }
     if (bytes != need) { set_error("array %d holds %zu bytes, caller passed %zu", which, need, bytes); return 1; }

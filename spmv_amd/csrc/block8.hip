@@ -1,0 +1,724 @@
+// Products with a matrix of 128 x 128 blocks in 8-bit floating point, one power-of-two scale per block:
+// y = A x, dx = A^T dy, the gradient of the stored blocks, and vectors to 8 bits and back.
+
+#include "internal.h"
+#include "device_utils.h"
+
+#include <new>
+#include <type_traits>
+#include <vector>
+
+namespace spmv {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kB = 128;                       // block edge, and length of a vector's group
+constexpr int kBlockBytes = kB * kB;
+
+// Place of (row, column) inside a block's 16 KB: 16 x 16 subtiles of 256 bytes, so that one 16-byte load per lane
+// is a contiguous 1 KB piece of a matrix-instruction operand (16 rows of one strip, 64 columns).  A strip holds the rows
+// {16 q + 4 s + r} of one 64-row half (s = strip in the half, q, r = 0..3): the accumulator keeps rows 4 q .. 4 q + 3 of
+// a tile in lane group q, which makes 4 tiles' results in a lane 16 consecutive rows of y.
+__host__ __device__ __forceinline__ int block8_offset(int row, int col)
+{
+    const int strip = (row >> 6) * 4 + ((row >> 2) & 3), i = ((row >> 4) & 3) * 4 + (row & 3);
+    return ((strip * 8 + (col >> 4)) * 16 + i) * 16 + (col & 15);
+}
+
+__device__ __forceinline__ float scale_value(int b) { return __int_as_float(b << 23); }      // 2^(b-127)
+
+// scale byte of a group whose largest finite magnitude is `amax`: the least e >= -126 with amax <= 448 * 2^e =
+// 1.75 * 2^(e+8), from the bits -- adding 0x1fffff to a float carries into its exponent where the mantissa is above 1.75
+__device__ __forceinline__ int scale_byte(float amax)
+{
+    if (amax == 0.0f) return 127;
+    const int e = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8;      // exponent byte of the scale
+    return e < 1 ? 1 : e;
+}
+__device__ __forceinline__ float scale_inverse(int b) { return __int_as_float((254 - b) << 23); }   // 2^(127-b), b <= 253
+__device__ __forceinline__ float finite_abs(float v)
+{
+    const float a = fabsf(v);
+    return a < __builtin_inff() ? a : 0.0f;                                  // false for NaN too
+}
+// four scaled values -> four e4m3 bytes, nearest even; beyond 448 (only +-inf here) and NaN -> NaN
+__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d)
+{
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+// four e4m3 bytes times a power of two -> four bf16, exact
+__device__ __forceinline__ void unpack4(unsigned w, float scale, __bf16 *out)
+{
+    const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
+    const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+    out[0] = lo[0]; out[1] = lo[1]; out[2] = hi[0]; out[3] = hi[1];
+}
+
+template <int DT> struct elem;
+template <> struct elem<SPMV_HIP_F32> { typedef float type; };
+template <> struct elem<SPMV_HIP_BF16> { typedef __bf16 type; };
+template <> struct elem<SPMV_HIP_F16> { typedef _Float16 type; };
+
+static size_t elem_size(int dtype) { return dtype == SPMV_HIP_F32 ? 4 : dtype == SPMV_HIP_E4M3 ? 1 : 2; }
+static bool wide_dtype(int dtype) { return dtype == SPMV_HIP_F32 || dtype == SPMV_HIP_BF16 || dtype == SPMV_HIP_F16; }
+
+// calls f with the element type of `dtype`
+template <typename F> static void with_elem(int dtype, F f)
+{
+    if (dtype == SPMV_HIP_F32) f(float());
+    else if (dtype == SPMV_HIP_BF16) f(__bf16());
+    else f(_Float16());
+}
+
+// ---- to 8 bits and back ---------------------------------------------------------------------------------------
+
+// 16 lanes per group of 128, 8 entries per lane
+template <typename T>
+__global__ __launch_bounds__(kBlock) void quantize8_kernel(int64_t ngroups, int groups, int columns, const T *__restrict__ x,
+                                                           int64_t ldx, uint8_t *__restrict__ x8, int64_t ldx8,
+                                                           uint8_t *__restrict__ scale, int64_t lds)
+{
+    const int64_t id = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> 4;
+    const int sub = threadIdx.x & 15;
+    if (id >= ngroups) return;                               // whole groups of 16 lanes leave together
+    const int64_t v = id / groups;
+    const int g = (int)(id % groups), c0 = g * kB + sub * 8;
+    float a[8], amax = 0.0f;
+    for (int k = 0; k < 8; k++) {
+        a[k] = c0 + k < columns ? (float)x[v * ldx + c0 + k] : 0.0f;
+        amax = fmaxf(amax, finite_abs(a[k]));
+    }
+    for (int d = 1; d < 16; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    const int b = scale_byte(amax);
+    const float inv = scale_inverse(b);
+    for (int k = 0; k < 8; k++) a[k] *= inv;
+    uint2 w = {pack4(a[0], a[1], a[2], a[3]), pack4(a[4], a[5], a[6], a[7])};
+    *(uint2 *)(x8 + v * ldx8 + c0) = w;
+    if (sub == 0) scale[(int64_t)g * lds + v] = (uint8_t)b;
+}
+
+template <typename T> __device__ __forceinline__ float largest_finite();
+template <> __device__ __forceinline__ float largest_finite<float>() { return 3.402823466e38f; }
+template <> __device__ __forceinline__ float largest_finite<__bf16>() { return 3.38953139e38f; }
+template <> __device__ __forceinline__ float largest_finite<_Float16>() { return 65504.0f; }
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void restore8_kernel(int64_t ngroups, int groups, int columns, const uint8_t *__restrict__ x8,
+                                                          int64_t ldx8, const uint8_t *__restrict__ scale, int64_t lds,
+                                                          T *__restrict__ x, int64_t ldx)
+{
+    const int64_t id = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> 4;
+    const int sub = threadIdx.x & 15;
+    if (id >= ngroups) return;
+    const int64_t v = id / groups;
+    const int g = (int)(id % groups), c0 = g * kB + sub * 8;
+    const uint2 w = *(const uint2 *)(x8 + v * ldx8 + c0);
+    const float s = scale_value(scale[(int64_t)g * lds + v]), top = largest_finite<T>();
+    float a[8];
+    for (int h = 0; h < 2; h++) {
+        const unsigned u = h ? w.y : w.x;
+        a[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8(u, 0) * s;
+        a[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(u, 1) * s;
+        a[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(u, 2) * s;
+        a[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(u, 3) * s;
+    }
+    for (int k = 0; k < 8; k++) {
+        const float y = a[k] > top ? top : a[k] < -top ? -top : a[k];        // NaN stays
+        if (c0 + k < columns) x[v * ldx + c0 + k] = (T)y;
+    }
+}
+
+// one workgroup per block; thread t holds half a row
+template <typename T>
+__global__ __launch_bounds__(kBlock) void set_values_kernel(int rows, int columns, const int *__restrict__ block_row,
+                                                            const int *__restrict__ block_col, const T *__restrict__ values,
+                                                            uint8_t *__restrict__ val8, int *__restrict__ scale8)
+{
+    __shared__ float part[kBlock / kWave];
+    const int64_t k = blockIdx.x;
+    const int r = threadIdx.x >> 1, c0 = (threadIdx.x & 1) * 64;
+    const bool row_in = block_row[k] * kB + r < rows;
+    const int cols_in = columns - block_col[k] * kB;
+    float a[64], amax = 0.0f;
+    for (int c = 0; c < 64; c++) {
+        a[c] = row_in && c0 + c < cols_in ? (float)values[k * kBlockBytes + r * kB + c0 + c] : 0.0f;
+        amax = fmaxf(amax, finite_abs(a[c]));
+    }
+    for (int d = 1; d < kWave; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    const int b = scale_byte(amax);
+    const float inv = scale_inverse(b);
+    for (int c = 0; c < 64; c += 16) {
+        u32x4 w;
+        for (int d = 0; d < 4; d++)
+            w[d] = pack4(a[c + 4 * d] * inv, a[c + 4 * d + 1] * inv, a[c + 4 * d + 2] * inv, a[c + 4 * d + 3] * inv);
+        *(u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c0 + c)) = w;
+    }
+    if (threadIdx.x == 0) scale8[k] = b;
+}
+
+// row-major 8-bit blocks into the handle's order and back
+__global__ __launch_bounds__(kBlock) void load8_kernel(int rows, int columns, const int *__restrict__ block_row,
+                                                       const int *__restrict__ block_col, const uint8_t *__restrict__ values8,
+                                                       const uint8_t *__restrict__ scale, uint8_t *__restrict__ val8,
+                                                       int *__restrict__ scale8)
+{
+    const int64_t k = blockIdx.x;
+    for (int p = threadIdx.x; p < kBlockBytes / 16; p += kBlock) {
+        const int r = p >> 3, c = (p & 7) * 16;
+        const int left = block_row[k] * kB + r < rows ? columns - block_col[k] * kB - c : 0;      // bytes inside the matrix
+        union { uint8_t b[16]; u32x4 w; } u;
+        for (int j = 0; j < 16; j++) u.b[j] = j < left ? values8[k * kBlockBytes + p * 16 + j] : (uint8_t)0;
+        *(u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c)) = u.w;
+    }
+    if (threadIdx.x == 0) scale8[k] = scale[k];
+}
+
+__global__ __launch_bounds__(kBlock) void store8_kernel(const uint8_t *__restrict__ val8, const int *__restrict__ scale8,
+                                                        uint8_t *__restrict__ values8, uint8_t *__restrict__ scale)
+{
+    const int64_t k = blockIdx.x;
+    for (int p = threadIdx.x; p < kBlockBytes / 16; p += kBlock) {
+        const int r = p >> 3, c = (p & 7) * 16;
+        union { uint8_t b[16]; u32x4 w; } u;
+        u.w = *(const u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c));
+        for (int j = 0; j < 16; j++) values8[k * kBlockBytes + p * 16 + j] = u.b[j];
+    }
+    if (threadIdx.x == 0) scale[k] = (uint8_t)scale8[k];
+}
+
+// ---- few vectors ----------------------------------------------------------------------------------------------
+
+// One workgroup per strip of 16 rows; its waves take the strip's blocks in turn and add their results in LDS.
+// Bound by reading the matrix once.  NT tiles of 16 vectors.  XT: uint8_t (x in 8 bits) or a wide type, rounded to 8 bits
+// here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.
+template <typename XT, int NT>
+__global__ __launch_bounds__(kBlock) void few_vectors_kernel(int n, int rows, int columns, const int *__restrict__ block_ptr,
+                                                             const int *__restrict__ block_col, const uint8_t *__restrict__ val8,
+                                                             const int *__restrict__ scale8, const XT *__restrict__ x,
+                                                             int64_t ldx, const uint8_t *__restrict__ xscale, int64_t lds,
+                                                             void *__restrict__ y, int y_dtype, int64_t ldy)
+{
+    constexpr int kWaves = kBlock / kWave;
+    __shared__ f32x4 part[kWaves][NT][kWave];
+    const int brow = blockIdx.x >> 3, strip = blockIdx.x & 7;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, i = lane & 15, q = lane >> 4;
+    f32x4 acc[NT];
+    for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
+    for (int b = block_ptr[brow] + wave; b < block_ptr[brow + 1]; b += kWaves) {
+        const int c0 = block_col[b] * kB;
+        const float sa = scale_value(scale8[b]);
+        bf16x8 a[4];
+        for (int h = 0; h < 2; h++) {
+            const u32x4 w = *(const u32x4 *)(val8 + (int64_t)b * kBlockBytes + ((strip * 2 + h) * kWave + lane) * 16);
+            for (int d = 0; d < 4; d++) unpack4(w[d], sa, (__bf16 *)&a[2 * h + (d >> 1)] + 4 * (d & 1));
+        }
+        for (int t = 0; t < NT; t++) {
+            const int v = t * 16 + i;
+            unsigned w8[8];
+            int sx = 127;
+            if constexpr (std::is_same<XT, uint8_t>::value) {
+                for (int d = 0; d < 8; d++)
+                    w8[d] = v < n ? *(const unsigned *)(x + (int64_t)v * ldx + c0 + 64 * (d >> 2) + 16 * q + 4 * (d & 3)) : 0u;
+                if (v < n) sx = xscale[(int64_t)block_col[b] * lds + v];
+            } else {
+                float f[32], amax = 0.0f;
+                for (int k = 0; k < 32; k++) {
+                    const int c = c0 + 64 * (k >> 4) + 16 * q + (k & 15);
+                    f[k] = v < n && c < columns ? (float)x[(int64_t)v * ldx + c] : 0.0f;
+                    amax = fmaxf(amax, finite_abs(f[k]));
+                }
+                amax = fmaxf(amax, __shfl_xor(amax, 16));
+                amax = fmaxf(amax, __shfl_xor(amax, 32));
+                sx = scale_byte(amax);
+                const float inv = scale_inverse(sx);
+                for (int d = 0; d < 8; d++)
+                    w8[d] = pack4(f[4 * d] * inv, f[4 * d + 1] * inv, f[4 * d + 2] * inv, f[4 * d + 3] * inv);
+            }
+            const float s = scale_value(sx);
+            for (int p = 0; p < 4; p++) {
+                bf16x8 xb;
+                unpack4(w8[2 * p], s, (__bf16 *)&xb);
+                unpack4(w8[2 * p + 1], s, (__bf16 *)&xb + 4);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], xb, acc[t], 0, 0, 0);
+            }
+        }
+    }
+    for (int t = 0; t < NT; t++) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int id = threadIdx.x; id < NT * kWave; id += kBlock) {
+        const int t = id / kWave, l = id & (kWave - 1), v = t * 16 + (l & 15);
+        f32x4 s = part[0][t][l];
+        for (int w = 1; w < kWaves; w++) s += part[w][t][l];
+        const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + 4 * (strip & 3);
+        if (v >= n) continue;
+        for (int k = 0; k < 4; k++) {
+            if (r0 + k >= rows) break;
+            const int64_t at = (int64_t)v * ldy + r0 + k;
+            if (y_dtype == SPMV_HIP_F32) ((float *)y)[at] = s[k];
+            else if (y_dtype == SPMV_HIP_BF16) ((__bf16 *)y)[at] = (__bf16)s[k];
+            else ((_Float16 *)y)[at] = (_Float16)s[k];
+        }
+    }
+}
+
+// ---- many vectors ---------------------------------------------------------------------------------------------
+
+// The three products share one tile: 128 (M) x 128 (N) results per workgroup, each wave a quarter, operands in LDS as
+// bf16, 64 deep (K) and contiguous along K.  What is staged differs:
+//   product     M = rows of a block row,     N = vectors,  K = its blocks' columns
+//   transposed  M = columns of a block column, N = vectors, K = its blocks' rows
+//   gradient    M = columns of a block, N = its rows, K = vectors
+// 8-bit values times their scales are exact in bf16.  dy is split into PARTS bf16 numbers that add up to it exactly
+// (1 for bf16, 2 for fp16, 3 for fp32: each holds 8 more bits), one matrix instruction each.
+enum { kProduct, kTransposed, kGradient };
+constexpr int kTile = 128, kDepth = 64, kPitch = kDepth + 8;
+
+template <int PARTS> __device__ __forceinline__ void split_bf16(float v, __bf16 *out)
+{
+    for (int p = 0; p < PARTS; p++) {
+        out[p] = (__bf16)v;
+        v -= (float)out[p];
+    }
+}
+
+struct MatrixArgs {
+    int n, rows, columns, accumulate;
+    const int *ptr, *idx, *id, *block_row;      // lists of blocks; gradient: idx = block column
+    const uint8_t *val8;
+    const int *scale8;
+    const uint8_t *x8, *xscale;
+    int64_t ldx8, lds, lddy, ldo;
+};
+
+template <int KIND, typename DT, int PARTS, typename OT>
+__global__ __launch_bounds__(kBlock) void many_vectors_kernel(MatrixArgs g, const DT *__restrict__ dy, OT *__restrict__ out)
+{
+    __shared__ __bf16 P[kTile][kPitch];
+    __shared__ __bf16 Q[PARTS][kTile][kPitch];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
+    const int m0 = (wave & 1) * 64, n0 = (wave >> 1) * 64;
+    const int major = blockIdx.x;                            // block row, block column, block
+    const int v0 = KIND == kGradient ? 0 : blockIdx.y * kTile;
+    f32x4 acc[4][4];
+    for (int a = 0; a < 4; a++)
+        for (int b = 0; b < 4; b++) acc[a][b] = f32x4{0, 0, 0, 0};
+
+    const int first = KIND == kGradient ? 0 : 2 * g.ptr[major];
+    const int last = KIND == kGradient ? (g.n + kDepth - 1) / kDepth : 2 * g.ptr[major + 1];
+    for (int step = first; step < last; step++) {
+        const int half = step & 1;
+        if (KIND == kProduct) {
+            const int b = step >> 1, c0 = g.idx[b] * kB + half * 64;
+            const float sa = scale_value(g.scale8[b]);
+            for (int p = tid; p < 512; p += kBlock) {        // 16-byte pieces of the block's half
+                const int strip = p >> 6, l = p & 63, ii = l & 15, qq = l >> 4;
+                const u32x4 w = *(const u32x4 *)(g.val8 + (int64_t)b * kBlockBytes + ((strip * 2 + half) * kWave + l) * 16);
+                const int r = (strip >> 2) * 64 + 16 * (ii >> 2) + 4 * (strip & 3) + (ii & 3);
+                for (int d = 0; d < 4; d++) unpack4(w[d], sa, &P[r][16 * qq + 4 * d]);
+            }
+            for (int p = tid; p < 512; p += kBlock) {
+                const int t = p >> 2, c = (p & 3) * 16;
+                u32x4 w = {0, 0, 0, 0};
+                float s = 1.0f;
+                if (v0 + t < g.n) {
+                    w = *(const u32x4 *)(g.x8 + (int64_t)(v0 + t) * g.ldx8 + c0 + c);
+                    s = scale_value(g.xscale[(int64_t)g.idx[b] * g.lds + v0 + t]);
+                }
+                for (int d = 0; d < 4; d++) unpack4(w[d], s, &Q[0][t][c + 4 * d]);
+            }
+        } else if (KIND == kTransposed) {
+            const int e = step >> 1, b = g.id[e], r0 = g.idx[e] * kB + half * 64;
+            const float sa = scale_value(g.scale8[b]);
+            for (int p = tid; p < 512; p += kBlock) {
+                const int strip = p >> 7, l = p & 127, ii = l & 15, qq = l >> 4;
+                const u32x4 w = *(const u32x4 *)(g.val8 + (int64_t)b * kBlockBytes + ((half * 4 + strip) * 128 + l) * 16);
+                const int r = 16 * (ii >> 2) + 4 * strip + (ii & 3);
+                __bf16 u[16];
+                for (int d = 0; d < 4; d++) unpack4(w[d], sa, u + 4 * d);
+                for (int d = 0; d < 16; d++) P[16 * qq + d][r] = u[d];
+            }
+            for (int p = tid; p < kTile * kDepth; p += kBlock) {
+                const int t = p >> 6, r = p & 63;
+                const float f = v0 + t < g.n && r0 + r < g.rows ? (float)dy[(int64_t)(v0 + t) * g.lddy + r0 + r] : 0.0f;
+                __bf16 u[PARTS];
+                split_bf16<PARTS>(f, u);
+                for (int k = 0; k < PARTS; k++) Q[k][t][r] = u[k];
+            }
+        } else {
+            const int t0 = step * kDepth, c0 = g.idx[major] * kB, r0 = g.block_row[major] * kB;
+            for (int p = tid; p < 512; p += kBlock) {
+                const int t = p >> 3, c = (p & 7) * 16;
+                u32x4 w = {0, 0, 0, 0};
+                float s = 1.0f;
+                if (t0 + t < g.n) {
+                    w = *(const u32x4 *)(g.x8 + (int64_t)(t0 + t) * g.ldx8 + c0 + c);
+                    s = scale_value(g.xscale[(int64_t)g.idx[major] * g.lds + t0 + t]);
+                }
+                __bf16 u[16];
+                for (int d = 0; d < 4; d++) unpack4(w[d], s, u + 4 * d);
+                for (int d = 0; d < 16; d++) P[c + d][t] = u[d];
+            }
+            for (int p = tid; p < kTile * kDepth; p += kBlock) {
+                const int t = p >> 7, r = p & 127;
+                const float f = t0 + t < g.n && r0 + r < g.rows ? (float)dy[(int64_t)(t0 + t) * g.lddy + r0 + r] : 0.0f;
+                __bf16 u[PARTS];
+                split_bf16<PARTS>(f, u);
+                for (int k = 0; k < PARTS; k++) Q[k][r][t] = u[k];
+            }
+        }
+        __syncthreads();
+        for (int k = 0; k < kDepth; k += 32) {
+            bf16x8 a[4];
+            for (int t = 0; t < 4; t++) a[t] = *(const bf16x8 *)&P[m0 + 16 * t + i][k + 8 * q];
+            for (int part = 0; part < PARTS; part++)
+                for (int u = 0; u < 4; u++) {
+                    const bf16x8 b = *(const bf16x8 *)&Q[part][n0 + 16 * u + i][k + 8 * q];
+                    for (int t = 0; t < 4; t++) acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t], b, acc[t][u], 0, 0, 0);
+                }
+        }
+        __syncthreads();
+    }
+    // lane (i, q) of a tile: N = i, M = 4 q .. 4 q + 3
+    for (int t = 0; t < 4; t++)
+        for (int u = 0; u < 4; u++) {
+            const int mm = m0 + 16 * t + 4 * q, nn = n0 + 16 * u + i;
+            if (KIND == kGradient) {
+                OT *o = out + (int64_t)major * kBlockBytes + nn * kB + mm;
+                const bool row_in = g.block_row[major] * kB + nn < g.rows;
+                for (int k = 0; k < 4; k++) {
+                    float v = row_in && g.idx[major] * kB + mm + k < g.columns ? acc[t][u][k] : 0.0f;
+                    if (g.accumulate) v += (float)o[k];
+                    o[k] = (OT)v;
+                }
+            } else {
+                const int limit = KIND == kProduct ? g.rows : g.columns;
+                if (v0 + nn >= g.n) continue;
+                for (int k = 0; k < 4; k++)
+                    if (major * kB + mm + k < limit) out[(int64_t)(v0 + nn) * g.ldo + major * kB + mm + k] = (OT)acc[t][u][k];
+            }
+        }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------
+
+static int launched(const char *what)
+{
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
+    return 1;
+}
+
+static int groups_of(int length) { return length / kB + (length % kB != 0); }
+
+static int launch_few(const spmv_hip_matrix *m, int n, const void *x, int x_dtype, int64_t ldx, const uint8_t *xscale,
+                      int64_t lds, void *y, int y_dtype, int64_t ldy, hipStream_t st)
+{
+    const dim3 grid(m->brows * 8), block(kBlock);
+    auto go = [&](auto t) {
+        typedef decltype(t) XT;
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, block, 0, st, n, m->rows, m->columns, m->d_block_ptr, m->d_block_col, m->d_val8,
+                               m->d_scale8, (const XT *)x, ldx, xscale, lds, y, y_dtype, ldy);
+        };
+        if (n <= 16) launch(few_vectors_kernel<XT, 1>);
+        else if (n <= 32) launch(few_vectors_kernel<XT, 2>);
+        else launch(few_vectors_kernel<XT, 4>);
+    };
+    if (x_dtype == SPMV_HIP_E4M3) go(uint8_t());
+    else with_elem(x_dtype, go);
+    return launched("block8_mult");
+}
+
+int launch_block8_f32(const spmv_hip_matrix *m, int n, const float *d_x, int64_t ldx, float *d_y, int64_t ldy,
+                      hipStream_t stream)
+{
+    if (m->rows == 0) return 0;
+    for (int v = 0; v < n; v += SPMV_HIP_BLOCK8_MAX_WIDE) {
+        const int k = n - v < SPMV_HIP_BLOCK8_MAX_WIDE ? n - v : (int)SPMV_HIP_BLOCK8_MAX_WIDE;
+        if (launch_few(m, k, d_x + v * ldx, SPMV_HIP_F32, ldx, nullptr, 0, d_y + v * ldy, SPMV_HIP_F32, ldy, stream)) return 1;
+    }
+    return 0;
+}
+
+static int bad_dtype(const char *what, int dtype)
+{
+    set_error("%s: element type %d must be F32, BF16 or F16", what, dtype);
+    return 1;
+}
+static int check_vectors(const char *what, int n, const void *p, int64_t ld, int length)
+{
+    if (n < 0) { set_error("%s: negative vector count %d", what, n); return 1; }
+    if (n > 0 && length > 0 && !p) { set_error("%s: NULL vector block", what); return 1; }
+    if (n > 1 && ld < length) { set_error("%s: vectors %lld apart are shorter than their length %d", what, (long long)ld, length); return 1; }
+    return 0;
+}
+static int check_eight(const char *what, int n, int columns, const void *x8, int64_t ldx8, const void *scale, int64_t lds)
+{
+    if (n < 0) { set_error("%s: negative vector count %d", what, n); return 1; }
+    if (n == 0 || columns == 0) return 0;
+    if (!x8 || !scale) { set_error("%s: NULL 8-bit vectors or scales", what); return 1; }
+    if (ldx8 % kB || ldx8 < (int64_t)groups_of(columns) * kB) {
+        set_error("%s: 8-bit vectors %lld apart, need a multiple of 128 of at least %lld", what, (long long)ldx8, (long long)groups_of(columns) * kB);
+        return 1;
+    }
+    if ((uintptr_t)x8 % 16) { set_error("%s: 8-bit vectors are not 16-byte aligned", what); return 1; }
+    if (lds < n) { set_error("%s: %lld scales per group for %d vectors", what, (long long)lds, n); return 1; }
+    return 0;
+}
+static int check_block8(const char *what, const spmv_hip_matrix *m)
+{
+    if (!m) { set_error("NULL handle"); return 1; }
+    if (m->format != SPMV_HIP_BLOCK8) { set_error("%s needs a handle of 8-bit blocks (format %d)", what, m->format); return 1; }
+    return 0;
+}
+// groups of 16 lanes in workgroups of 256: at most 2^31 - 1 workgroups
+static int check_groups(const char *what, int64_t ngroups)
+{
+    if (ngroups <= (int64_t)0x7fffffff * (kBlock / 16)) return 0;
+    set_error("%s: %lld groups of 128 are more than one launch takes", what, (long long)ngroups);
+    return 1;
+}
+
+} // namespace spmv
+
+using namespace spmv;
+
+extern "C" {
+
+spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, const int *block_ptr, const int *block_col)
+{
+    clear_error();
+    if (rows < 0 || columns < 0 || nblocks < 0) { set_error("negative dimension"); return nullptr; }
+    if (!block_ptr || (nblocks > 0 && !block_col)) { set_error("NULL block array"); return nullptr; }
+    const int brows = groups_of(rows), bcols = groups_of(columns);
+    if (block_ptr[0] != 0 || block_ptr[brows] != nblocks) {
+        set_error("block_ptr[0] must be 0 and block_ptr[%d] must equal nblocks", brows);
+        return nullptr;
+    }
+    for (int r = 0; r < brows; r++)
+        if (block_ptr[r + 1] < block_ptr[r]) { set_error("block_ptr decreases at block row %d", r); return nullptr; }
+    for (int k = 0; k < nblocks; k++)
+        if (block_col[k] < 0 || block_col[k] >= bcols) { set_error("block column %d out of range at block %d", block_col[k], k); return nullptr; }
+    spmv_hip_matrix *m = new (std::nothrow) spmv_hip_matrix();
+    if (!m) { set_error("out of host memory"); return nullptr; }
+    m->format = SPMV_HIP_BLOCK8; m->dtype = SPMV_HIP_F32; m->rows = rows; m->columns = columns;
+    m->nblocks = nblocks; m->brows = brows; m->bcols = bcols;
+    m->stored = (int64_t)nblocks * kBlockBytes;
+    if (hipGetDevice(&m->device) != hipSuccess) { set_error("no HIP device available"); delete m; return nullptr; }
+    (void)hipGetLastError();
+    bool ok = false;
+    try {
+        // the blocks once more, by block column; inside one in ascending block row
+        std::vector<int> row((size_t)nblocks), tptr((size_t)bcols + 1, 0), trow((size_t)nblocks), tid((size_t)nblocks);
+        for (int r = 0; r < brows; r++)
+            for (int k = block_ptr[r]; k < block_ptr[r + 1]; k++) {
+                row[(size_t)k] = r;
+                tptr[(size_t)block_col[k] + 1]++;
+                m->nnz += (int64_t)(rows - r * kB < kB ? rows - r * kB : kB) *
+                          (columns - block_col[k] * kB < kB ? columns - block_col[k] * kB : kB);
+            }
+        for (int c = 0; c < bcols; c++) tptr[(size_t)c + 1] += tptr[(size_t)c];
+        std::vector<int> at(tptr.begin(), tptr.end());
+        for (int k = 0; k < nblocks; k++) {
+            const int w = at[(size_t)block_col[k]]++;
+            trow[(size_t)w] = row[(size_t)k];
+            tid[(size_t)w] = k;
+        }
+        const std::vector<int> scale((size_t)nblocks, 127);
+        auto up = [&](int **d, const int *h, size_t count) {
+            if (dev_alloc(m, d, count)) return false;
+            if (count) SPMV_HIP_TRY(hipMemcpy(*d, h, count * sizeof(int), hipMemcpyHostToDevice), return false);
+            return true;
+        };
+        ok = up(&m->d_block_ptr, block_ptr, (size_t)brows + 1) && up(&m->d_block_col, block_col, (size_t)nblocks) &&
+             up(&m->d_block_row, row.data(), (size_t)nblocks) && up(&m->d_bt_ptr, tptr.data(), (size_t)bcols + 1) &&
+             up(&m->d_bt_row, trow.data(), (size_t)nblocks) && up(&m->d_bt_id, tid.data(), (size_t)nblocks) &&
+             up(&m->d_scale8, scale.data(), (size_t)nblocks) && dev_alloc(m, &m->d_val8, (size_t)nblocks * kBlockBytes) == 0;
+        if (ok && nblocks) {
+            ok = hipMemset(m->d_val8, 0, (size_t)nblocks * kBlockBytes) == hipSuccess && hipDeviceSynchronize() == hipSuccess;
+            if (!ok) set_error("clearing the blocks failed");
+        }
+    } catch (const std::bad_alloc &) { set_error("out of host memory"); ok = false; }
+    if (!ok) { spmv_hip_free(m); return nullptr; }
+    return m;
+}
+
+int spmv_hip_block8_set_values_dev(spmv_hip_matrix *m, const void *d_values, int dtype, void *stream)
+{
+    if (check_block8("block8_set_values", m)) return 1;
+    if (!wide_dtype(dtype)) return bad_dtype("block8_set_values", dtype);
+    if (m->nblocks == 0) return 0;
+    if (!d_values) { set_error("block8_set_values: NULL values"); return 1; }
+    DeviceGuard on(m->device);
+    if (!on.ok) return 1;
+    with_elem(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((set_values_kernel<T>), dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream, m->rows, m->columns,
+                           m->d_block_row, m->d_block_col, (const T *)d_values, m->d_val8, m->d_scale8);
+    });
+    return launched("block8_set_values");
+}
+
+int spmv_hip_block8_load_dev(spmv_hip_matrix *m, const uint8_t *d_values8, const uint8_t *d_scale, void *stream)
+{
+    if (check_block8("block8_load", m)) return 1;
+    if (m->nblocks == 0) return 0;
+    if (!d_values8 || !d_scale) { set_error("block8_load: NULL argument"); return 1; }
+    DeviceGuard on(m->device);
+    if (!on.ok) return 1;
+    hipLaunchKernelGGL(load8_kernel, dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream, m->rows, m->columns, m->d_block_row,
+                       m->d_block_col, d_values8, d_scale, m->d_val8, m->d_scale8);
+    return launched("block8_load");
+}
+
+int spmv_hip_block8_store_dev(const spmv_hip_matrix *m, uint8_t *d_values8, uint8_t *d_scale, void *stream)
+{
+    if (check_block8("block8_store", m)) return 1;
+    if (m->nblocks == 0) return 0;
+    if (!d_values8 || !d_scale) { set_error("block8_store: NULL argument"); return 1; }
+    DeviceGuard on(m->device);
+    if (!on.ok) return 1;
+    hipLaunchKernelGGL(store8_kernel, dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream, m->d_val8, m->d_scale8, d_values8, d_scale);
+    return launched("block8_store");
+}
+
+int spmv_hip_quantize8_dev(int n, int columns, const void *d_x, int dtype, int64_t ldx, uint8_t *d_x8, int64_t ldx8,
+                           uint8_t *d_scale, int64_t lds, void *stream)
+{
+    if (!wide_dtype(dtype)) return bad_dtype("quantize8", dtype);
+    if (columns < 0) { set_error("quantize8: negative length %d", columns); return 1; }
+    if (check_vectors("quantize8", n, d_x, ldx, columns) || check_eight("quantize8", n, columns, d_x8, ldx8, d_scale, lds)) return 1;
+    const int groups = groups_of(columns);
+    const int64_t ngroups = (int64_t)n * groups;
+    if (ngroups == 0) return 0;
+    if (check_groups("quantize8", ngroups)) return 1;
+    with_elem(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((quantize8_kernel<T>), dim3((unsigned)((ngroups + 15) / 16)), dim3(kBlock), 0, (hipStream_t)stream,
+                           ngroups, groups, columns, (const T *)d_x, ldx, d_x8, ldx8, d_scale, lds);
+    });
+    return launched("quantize8");
+}
+
+int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds,
+                          void *d_x, int dtype, int64_t ldx, void *stream)
+{
+    if (!wide_dtype(dtype)) return bad_dtype("restore8", dtype);
+    if (columns < 0) { set_error("restore8: negative length %d", columns); return 1; }
+    if (check_vectors("restore8", n, d_x, ldx, columns) || check_eight("restore8", n, columns, d_x8, ldx8, d_scale, lds)) return 1;
+    const int groups = groups_of(columns);
+    const int64_t ngroups = (int64_t)n * groups;
+    if (ngroups == 0) return 0;
+    if (check_groups("restore8", ngroups)) return 1;
+    with_elem(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((restore8_kernel<T>), dim3((unsigned)((ngroups + 15) / 16)), dim3(kBlock), 0, (hipStream_t)stream,
+                           ngroups, groups, columns, d_x8, ldx8, d_scale, lds, (T *)d_x, ldx);
+    });
+    return launched("restore8");
+}
+
+int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, int x_dtype, int64_t ldx,
+                             const uint8_t *d_scale, int64_t lds, void *d_y, int y_dtype, int64_t ldy, void *stream)
+{
+    const char *what = "block8_mult";
+    if (check_block8(what, m)) return 1;
+    if (!wide_dtype(y_dtype)) return bad_dtype(what, y_dtype);
+    if (x_dtype == SPMV_HIP_E4M3) {
+        if (check_eight(what, n, m->columns, d_x, ldx, d_scale, lds)) return 1;
+    } else {
+        if (!wide_dtype(x_dtype)) { set_error("%s: element type %d must be F32, BF16, F16 or E4M3", what, x_dtype); return 1; }
+        if (check_vectors(what, n, d_x, ldx, m->columns)) return 1;
+        if (d_scale) { set_error("%s: scales belong to vectors in 8 bits", what); return 1; }
+        if (n > SPMV_HIP_BLOCK8_MAX_WIDE) {
+            set_error("%s: %d wide vectors, at most %d are rounded inside the product (quantize8 first)", what, n, (int)SPMV_HIP_BLOCK8_MAX_WIDE);
+            return 1;
+        }
+    }
+    if (check_vectors(what, n, d_y, ldy, m->rows)) return 1;
+    if (n == 0 || m->rows == 0) return 0;
+    DeviceGuard on(m->device);
+    if (!on.ok) return 1;
+    if (n <= SPMV_HIP_BLOCK8_MAX_WIDE)
+        return launch_few(m, n, d_x, x_dtype, ldx, d_scale, lds, d_y, y_dtype, ldy, (hipStream_t)stream);
+    MatrixArgs a{};
+    a.n = n; a.rows = m->rows; a.columns = m->columns;
+    a.ptr = m->d_block_ptr; a.idx = m->d_block_col; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
+    a.x8 = (const uint8_t *)d_x; a.xscale = d_scale; a.ldx8 = ldx; a.lds = lds; a.ldo = ldy;
+    const dim3 grid(m->brows, (n + kTile - 1) / kTile);
+    if (grid.y > 65535) { set_error("%s: %d vectors are more than one launch takes", what, n); return 1; }
+    with_elem(y_dtype, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((many_vectors_kernel<kProduct, float, 1, T>), grid, dim3(kBlock), 0, (hipStream_t)stream, a,
+                           (const float *)nullptr, (T *)d_y);
+    });
+    return launched(what);
+}
+
+int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, void *d_dx,
+                               int dx_dtype, int64_t lddx, void *stream)
+{
+    const char *what = "block8_mult_t";
+    if (check_block8(what, m)) return 1;
+    if (!wide_dtype(dy_dtype)) return bad_dtype(what, dy_dtype);
+    if (!wide_dtype(dx_dtype)) return bad_dtype(what, dx_dtype);
+    if (check_vectors(what, n, d_dy, lddy, m->rows) || check_vectors(what, n, d_dx, lddx, m->columns)) return 1;
+    if (n == 0 || m->columns == 0) return 0;
+    DeviceGuard on(m->device);
+    if (!on.ok) return 1;
+    MatrixArgs a{};
+    a.n = n; a.rows = m->rows; a.columns = m->columns;
+    a.ptr = m->d_bt_ptr; a.idx = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
+    a.lddy = lddy; a.ldo = lddx;
+    const dim3 grid(m->bcols, (n + kTile - 1) / kTile);
+    if (grid.y > 65535) { set_error("%s: %d vectors are more than one launch takes", what, n); return 1; }
+    with_elem(dy_dtype, [&](auto t) {
+        typedef decltype(t) T;
+        constexpr int parts = std::is_same<T, float>::value ? 3 : std::is_same<T, __bf16>::value ? 1 : 2;
+        with_elem(dx_dtype, [&](auto o) {
+            typedef decltype(o) O;
+            hipLaunchKernelGGL((many_vectors_kernel<kTransposed, T, parts, O>), grid, dim3(kBlock), 0, (hipStream_t)stream, a,
+                               (const T *)d_dy, (O *)d_dx);
+        });
+    });
+    return launched(what);
+}
+
+int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
+                                 const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dvalues,
+                                 int dtype, int accumulate, void *stream)
+{
+    const char *what = "block8_gradient";
+    if (check_block8(what, m)) return 1;
+    if (!wide_dtype(dy_dtype)) return bad_dtype(what, dy_dtype);
+    if (!wide_dtype(dtype)) return bad_dtype(what, dtype);
+    if (check_vectors(what, n, d_dy, lddy, m->rows) || check_eight(what, n, m->columns, d_x8, ldx8, d_scale, lds)) return 1;
+    if (m->nblocks == 0) return 0;
+    if (!d_dvalues) { set_error("%s: NULL gradient", what); return 1; }
+    DeviceGuard on(m->device);
+    if (!on.ok) return 1;
+    MatrixArgs a{};
+    a.n = n; a.rows = m->rows; a.columns = m->columns; a.accumulate = accumulate;
+    a.idx = m->d_block_col; a.block_row = m->d_block_row;
+    a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.lddy = lddy;
+    with_elem(dy_dtype, [&](auto t) {
+        typedef decltype(t) T;
+        constexpr int parts = std::is_same<T, float>::value ? 3 : std::is_same<T, __bf16>::value ? 1 : 2;
+        with_elem(dtype, [&](auto o) {
+            typedef decltype(o) O;
+            hipLaunchKernelGGL((many_vectors_kernel<kGradient, T, parts, O>), dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream,
+                               a, (const T *)d_dy, (O *)d_dvalues);
+        });
+    });
+    return launched(what);
+}
+
+} // extern "C"

@@ -128,6 +128,14 @@ struct spmv_hip_matrix {
     int xcd_used_cpx = 0;           // labels per group that the matrix references (the rest of a group never needs x)
     int64_t xcd_bytes = 0;          // what the stacked handle and its vectors added to device_bytes
 
+    // 8-bit blocks (BLOCK8): the blocks by block row (block_ptr, block_col) and by block column (bt_ptr over block
+    // columns, bt_row = block row, bt_id = block)
+    int nblocks = 0, brows = 0, bcols = 0;
+    int *d_block_ptr = nullptr, *d_block_col = nullptr, *d_block_row = nullptr;
+    int *d_bt_ptr = nullptr, *d_bt_row = nullptr, *d_bt_id = nullptr;
+    uint8_t *d_val8 = nullptr;      // [nblocks][16384] in the order of block8_offset
+    int *d_scale8 = nullptr;        // [nblocks] scale byte, one per word (read by scalar loads)
+
     // staging vectors for the host-pointer multiply and the bench loop
     void *d_x = nullptr, *d_y = nullptr;
     double *d_norm = nullptr;
@@ -179,6 +187,10 @@ int build_sliced(spmv_hip_matrix *m, const int *d_row_ptr, const int *d_col, con
                  bool val_is_f64, bool sorted, hipStream_t stream);
 int build_sell_dfc(spmv_hip_matrix *m, const int *d_row_ptr, const int *d_col, const void *d_val,
                    bool val_is_f64, hipStream_t stream);
+
+// block8.hip -- products of a BLOCK8 handle with F32 vectors, rounded to 8 bits on the way in
+int launch_block8_f32(const spmv_hip_matrix *m, int n, const float *d_x, int64_t ldx, float *d_y, int64_t ldy,
+                      hipStream_t stream);
 
 template <typename T> int dev_alloc(spmv_hip_matrix *m, T **p, size_t count)
 {

@@ -1425,6 +1425,7 @@ constexpr int kSlicedVariants[] = {0, 1, 2, 3, 4, 9, 10, 11, 12};
 int variant_candidates(const spmv_hip_matrix *m, int *out, int max_out)
 {
     int n = 0;
+    if (m->format == SPMV_HIP_BLOCK8) return 0;             // kernels chosen by the number of vectors, not by trial
     const bool sliced64 = m->d_slice_ptr && m->slice_height == kWave && m->format != SPMV_HIP_SELL_DFC;
     if (m->format == SPMV_HIP_SELL_DFC) {
         for (int v = 0; v <= 8; v++)                          // see launch_sell_dfc
@@ -1910,6 +1911,8 @@ static int launch_mult_xcd(const spmv_hip_matrix *m, const T *x, T *y, hipStream
 
 int launch_mult(const spmv_hip_matrix *m, const void *d_x, void *d_y, hipStream_t stream)
 {
+    if (m->format == SPMV_HIP_BLOCK8)
+        return launch_block8_f32(m, 1, (const float *)d_x, m->columns, (float *)d_y, m->rows, stream);
     if (m->xcd_sub && m->rows > 0) {
         if (m->d_row_map) { set_error("hot_columns 2 does not combine with a row map"); return 1; }
         return m->dtype == SPMV_HIP_F32 ? launch_mult_xcd<float>(m, (const float *)d_x, (float *)d_y, stream)

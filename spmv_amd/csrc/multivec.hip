@@ -784,6 +784,8 @@ static int launch_mult_mv_t(const spmv_hip_matrix *m, int n, const T *x, int64_t
 int launch_mult_mv(const spmv_hip_matrix *m, int n, const void *d_x, int64_t ldx, void *d_y, int64_t ldy,
                    hipStream_t stream)
 {
+    if (m->format == SPMV_HIP_BLOCK8)
+        return launch_block8_f32(m, n, (const float *)d_x, ldx, (float *)d_y, ldy, stream);
     if (m->dtype == SPMV_HIP_F32)
         return launch_mult_mv_t<float>(m, n, (const float *)d_x, ldx, (float *)d_y, ldy, stream);
     return launch_mult_mv_t<double>(m, n, (const double *)d_x, ldx, (double *)d_y, ldy, stream);

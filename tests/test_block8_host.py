@@ -1,0 +1,105 @@
+"""8-bit block matrices without a GPU: the oracle against torch's own e4m3 conversion, and every refusal that the library
+or the Python layer makes before it needs a device."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import spmv_amd as S
+from spmv_amd import block8
+from tests import block8_oracle as O
+
+
+def _fails(rc, text):
+    assert rc != 0
+    assert text in S.lib().spmv_hip_last_error().decode(), S.lib().spmv_hip_last_error()
+
+
+def test_oracle_rounds_like_torchs_e4m3():
+    x = np.concatenate([np.linspace(-448, 448, 20001), np.exp2(np.linspace(-12, 8, 4001)), [0.0, -0.0, 2.0 ** -10, 1.5 * 2.0 ** -9]])
+    x = x.astype(np.float32)
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).to(torch.float64).numpy()
+    assert np.array_equal(O.nearest(x), want)
+    codes = np.arange(256, dtype=np.uint8)
+    t = torch.from_numpy(codes).view(torch.float8_e4m3fn).to(torch.float64).numpy()
+    assert np.array_equal(np.nan_to_num(O.decode(codes), nan=-1e9), np.nan_to_num(t, nan=-1e9))
+
+
+def test_oracle_scale_is_the_least_power_of_two_that_fits():
+    rng = np.random.default_rng(0)
+    a = np.abs(rng.standard_normal(1000)) * np.exp2(rng.integers(-130, 120, 1000))
+    a = np.concatenate([a, [448.0, 448.0 * (1 + 2.0 ** -20), 449.0, 3.4e38, 1e-45]])
+    b = O.scale_byte(a[:, None]).astype(np.float64)
+    assert np.all(a <= 448 * np.exp2(b - 127))
+    assert np.all((a > 448 * np.exp2(b - 128)) | (b == 1))
+    assert O.scale_byte(np.zeros((1, 4)))[0] == 127
+    assert O.scale_byte(np.array([[np.inf, np.nan, 2.0]]))[0] == O.scale_byte(np.array([[2.0]]))[0]
+
+
+def _create(rows, columns, ptr, col):
+    ptr, col = np.array(ptr, np.int32), np.array(col, np.int32)
+    return S.lib().spmv_hip_create_block8(rows, columns, len(col), ptr.ctypes.data, col.ctypes.data)
+
+
+@pytest.mark.parametrize("rows,columns,ptr,col,text", [
+    (-1, 5, [0], [], "negative dimension"),
+    (130, 130, [0, 1, 1], [2], "block column 2 out of range"),
+    (130, 130, [0, 1, 1], [-1], "block column -1 out of range"),
+    (130, 130, [0, 2, 1], [0], "block_ptr decreases"),
+    (130, 130, [0, 0, 2], [0], "must equal nblocks"),
+    (130, 130, [1, 1, 1], [0], "block_ptr[0] must be 0"),
+    (130, 0, [0, 1, 1], [0], "out of range"),
+])
+def test_creator_refuses_bad_patterns(rows, columns, ptr, col, text):
+    assert not _create(rows, columns, ptr, col)
+    assert text in S.lib().spmv_hip_last_error().decode()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="needs a machine without a GPU")
+def test_no_gpu_is_an_error():
+    assert not _create(130, 130, [0, 1, 1], [0])
+    assert "no HIP device" in S.lib().spmv_hip_last_error().decode()
+
+
+def test_vector_calls_refuse_bad_arguments():
+    L = S.lib()
+    p = 4096                                                 # an address that no refused call touches
+    q = lambda n=2, cols=200, x=p, dt=S.F32, ldx=200, x8=p, ld8=256, sc=p, lds=2: L.spmv_hip_quantize8_dev(n, cols, x, dt, ldx, x8, ld8, sc, lds, None)
+    _fails(q(dt=S.F64), "must be F32, BF16 or F16")
+    _fails(q(dt=S.E4M3), "must be F32, BF16 or F16")
+    _fails(q(n=-1), "negative vector count")
+    _fails(q(cols=-1), "negative length")
+    _fails(q(x=None), "NULL vector block")
+    _fails(q(ldx=199), "shorter than their length")
+    _fails(q(x8=None), "NULL 8-bit")
+    _fails(q(sc=None), "NULL 8-bit")
+    _fails(q(ld8=128), "multiple of 128 of at least 256")
+    _fails(q(ld8=300), "multiple of 128")
+    _fails(q(x8=p + 8), "16-byte aligned")
+    _fails(q(lds=1), "1 scales per group for 2 vectors")
+    r = lambda n=2, cols=200, x8=p, ld8=256, sc=p, lds=2, x=p, dt=S.F32, ldx=200: L.spmv_hip_restore8_dev(n, cols, x8, ld8, sc, lds, x, dt, ldx, None)
+    _fails(r(dt=9), "must be F32, BF16 or F16")
+    _fails(r(ldx=3), "shorter than their length")
+    _fails(r(ld8=255), "multiple of 128")
+    assert q(n=0) == 0 and r(n=0) == 0 and q(cols=0) == 0    # nothing to do
+    for name, args in (("mult", (None, 1, p, S.F32, 9, None, 0, p, S.F32, 9, None)), ("mult_t", (None, 1, p, S.F32, 9, p, S.F32, 9, None)),
+                       ("gradient", (None, 1, p, S.F32, 9, p, 128, p, 1, p, S.F32, 0, None)), ("set_values", (None, p, S.F32, None)),
+                       ("load", (None, p, p, None)), ("store", (None, p, p, None))):
+        _fails(getattr(L, f"spmv_hip_block8_{name}_dev")(*args), "NULL handle")
+
+
+def test_python_layer_refuses_what_is_not_on_a_gpu():
+    with pytest.raises(ValueError, match="no CPU path"):
+        block8.quantize(torch.zeros(2, 128))
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        block8.quantize(torch.zeros(2, 128, dtype=torch.float64))
+    with pytest.raises(TypeError):
+        block8.quantize([1.0, 2.0])
+    with pytest.raises(ValueError, match="on one GPU"):
+        block8.Packed8(torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 200, torch.float32)
+    with pytest.raises(ValueError, match="contiguous uint8"):
+        block8.Packed8(torch.zeros(2, 200, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 200, torch.float32)
+    with pytest.raises(ValueError, match="block_ptr has shape"):
+        block8.Block8(300, 300, [0, 1], [0])
+    assert C.sizeof(S._lib.Info) > 0 and S.FORMAT_NAMES[S.BLOCK8] == "block8"
