@@ -374,8 +374,8 @@ int spmv_hip_dist_free(spmv_hip_dist *d);
  * any order; two blocks at one place add up.
  *
  * Vectors: vector v starts at p + v * ld (ld in elements).  In 8 bits (SPMV_HIP_E4M3)
- * ld8 is a multiple of 128 and >= columns rounded up to 128, the base is 16-byte
- * aligned, the bytes past `columns` are zero (spmv_hip_quantize8_dev writes them),
+ * ld8 is a multiple of 128, >= columns rounded up to 128 and < 2^24, the base is
+ * 16-byte aligned, the bytes past `columns` are zero (spmv_hip_quantize8_dev writes them),
  * and scale[g * lds + v] is the scale byte of its entries 128 g .. 128 g + 127
  * (lds >= n).  In F32, BF16 or F16 nothing is asked of the alignment beyond the
  * element's own; 16-byte aligned bases and strides are faster.

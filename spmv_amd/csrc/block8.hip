@@ -14,6 +14,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kB = 128;                       // block edge, and length of a vector's group
 constexpr int kBlockBytes = kB * kB;
@@ -270,140 +272,420 @@ __global__ __launch_bounds__(kBlock) void few_vectors_kernel(int n, int rows, in
 
 // ---- many vectors ---------------------------------------------------------------------------------------------
 
-// The three products share one tile: 128 (M) x 128 (N) results per workgroup, each wave a quarter, operands in LDS as
-// bf16, 64 deep (K) and contiguous along K.  What is staged differs:
-//   product     M = rows of a block row,     N = vectors,  K = its blocks' columns
-//   transposed  M = columns of a block column, N = vectors, K = its blocks' rows
-//   gradient    M = columns of a block, N = its rows, K = vectors
-// 8-bit values times their scales are exact in bf16.  dy is split into PARTS bf16 numbers that add up to it exactly
-// (1 for bf16, 2 for fp16, 3 for fp32: each holds 8 more bits), one matrix instruction each.
-enum { kProduct, kTransposed, kGradient };
-constexpr int kTile = 128, kDepth = 64, kPitch = kDepth + 8;
+// Three products on 128-row tiles, 4 waves, operands staged through registers into two LDS buffers: while the matrix
+// instructions run on one, the loads for the other are in flight; one barrier a step.  Two workgroups share a CU, so one
+// computes where the other waits.  Registers rather than direct loads to LDS, because the staging masks edges, takes any
+// alignment and converts.
 
-template <int PARTS> __device__ __forceinline__ void split_bf16(float v, __bf16 *out)
+// logical tile of a workgroup: every XCD walks its own eighth of the tiles, in it 8 block rows (columns) side by side
+// and then the next vectors, so that the blocks and the vectors of the workgroups that run together stay in its L2
+__device__ __forceinline__ void tile_of_block(unsigned bid, int majors, int vtiles, int *major, int *vtile)
 {
-    for (int p = 0; p < PARTS; p++) {
-        out[p] = (__bf16)v;
-        v -= (float)out[p];
+    const unsigned id = xcd_contiguous_block(bid, (unsigned)majors * vtiles);
+    const unsigned per = 8u * vtiles, group = id / per, in = id % per;
+    const unsigned wide = (unsigned)majors - group * 8 < 8 ? (unsigned)majors - group * 8 : 8;
+    *major = (int)(group * 8 + in % wide);
+    *vtile = (int)(in / wide);
+}
+
+__device__ __forceinline__ u32x4 load16(const void *p)       // any alignment
+{
+    u32x4 w;
+    __builtin_memcpy(&w, p, 16);
+    return w;
+}
+
+// results m .. m + 4 COUNT - 1 of one vector, as many as there are below `limit`
+template <typename OT, int COUNT>
+__device__ __forceinline__ void store_row(OT *o, int left, const f32x4 *a)
+{
+    if (left >= 4 * COUNT) {
+        OT v[4 * COUNT];
+#pragma unroll
+        for (int k = 0; k < 4 * COUNT; k++) v[k] = (OT)a[k >> 2][k & 3];
+        __builtin_memcpy(o, v, sizeof v);
+    } else {
+        for (int k = 0; k < 4 * COUNT; k++)
+            if (k < left) o[k] = (OT)a[k >> 2][k & 3];
     }
 }
 
-struct MatrixArgs {
-    int n, rows, columns, accumulate;
-    const int *ptr, *idx, *id, *block_row;      // lists of blocks; gradient: idx = block column
-    const uint8_t *val8;
-    const int *scale8;
-    const uint8_t *x8, *xscale;
-    int64_t ldx8, lds, lddy, ldo;
+struct ProductArgs {
+    int n, rows, brows, vtiles;
+    const int *ptr, *col, *scale8;
+    const uint8_t *val8, *x8, *xscale;
+    int64_t ldx8, lds, ldy;
 };
 
-template <int KIND, typename DT, int PARTS, typename OT>
-__global__ __launch_bounds__(kBlock) void many_vectors_kernel(MatrixArgs g, const DT *__restrict__ dy, OT *__restrict__ out)
+// y = A x.  Tile: one block row x TOK vectors; a wave has 64 rows x TOK / 2 vectors.  The blocks go straight from memory
+// to registers (their layout is the operand's), the vectors through LDS: rows of 128 bytes, their 16-byte pieces
+// exchanged by XOR so that the 8 lanes of a read cycle meet 8 different pieces.  Vector NU i + u belongs to lane i of
+// tile u: a lane's scale bytes are then neighbours.
+// EXACT: operands widened to bf16 in registers (exact), 32-bit sums.  Otherwise the 8-bit matrix instruction, which applies
+// both scales and runs at twice the rate, but whose sums of 128 products are good to about 16 bits: only for bf16 results.
+template <bool EXACT, int TOK, typename OT>
+__global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *__restrict__ y)
 {
-    __shared__ __bf16 P[kTile][kPitch];
-    __shared__ __bf16 Q[PARTS][kTile][kPitch];
+    constexpr int NU = TOK / 32, PIECES = TOK / 32;
+    __shared__ uint8_t X[2][TOK * kB];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
-    const int m0 = (wave & 1) * 64, n0 = (wave >> 1) * 64;
-    const int major = blockIdx.x;                            // block row, block column, block
-    const int v0 = KIND == kGradient ? 0 : blockIdx.y * kTile;
-    f32x4 acc[4][4];
-    for (int a = 0; a < 4; a++)
-        for (int b = 0; b < 4; b++) acc[a][b] = f32x4{0, 0, 0, 0};
+    const int wm = wave & 1, wn = wave >> 1;
+    int major, vtile;
+    tile_of_block(blockIdx.x, g.brows, g.vtiles, &major, &vtile);
+    const int v0 = vtile * TOK, first = g.ptr[major], last = g.ptr[major + 1];
+    f32x4 acc[NU][4];
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    const int first = KIND == kGradient ? 0 : 2 * g.ptr[major];
-    const int last = KIND == kGradient ? (g.n + kDepth - 1) / kDepth : 2 * g.ptr[major + 1];
-    for (int step = first; step < last; step++) {
-        const int half = step & 1;
-        if (KIND == kProduct) {
-            const int b = step >> 1, c0 = g.idx[b] * kB + half * 64;
-            const float sa = scale_value(g.scale8[b]);
-            for (int p = tid; p < 512; p += kBlock) {        // 16-byte pieces of the block's half
-                const int strip = p >> 6, l = p & 63, ii = l & 15, qq = l >> 4;
-                const u32x4 w = *(const u32x4 *)(g.val8 + (int64_t)b * kBlockBytes + ((strip * 2 + half) * kWave + l) * 16);
-                const int r = (strip >> 2) * 64 + 16 * (ii >> 2) + 4 * (strip & 3) + (ii & 3);
-                for (int d = 0; d < 4; d++) unpack4(w[d], sa, &P[r][16 * qq + 4 * d]);
-            }
-            for (int p = tid; p < 512; p += kBlock) {
-                const int t = p >> 2, c = (p & 3) * 16;
-                u32x4 w = {0, 0, 0, 0};
-                float s = 1.0f;
-                if (v0 + t < g.n) {
-                    w = *(const u32x4 *)(g.x8 + (int64_t)(v0 + t) * g.ldx8 + c0 + c);
-                    s = scale_value(g.xscale[(int64_t)g.idx[b] * g.lds + v0 + t]);
+    u32x4 xr[PIECES];
+    unsigned at[PIECES];                                     // past the last vector: any, it is not stored
+#pragma unroll
+    for (int j = 0; j < PIECES; j++) at[j] = (unsigned)min(j * 32 + (tid >> 3), g.n - 1 - v0) * (unsigned)g.ldx8 + (tid & 7) * 16;
+    auto fetch = [&](int b) {
+        const uint8_t *base = g.x8 + (int64_t)v0 * g.ldx8 + g.col[b] * kB;
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) xr[j] = *(const u32x4 *)(base + at[j]);
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            const int t = j * 32 + (tid >> 3);
+            *(u32x4 *)&X[buf][t * kB + (((tid & 7) ^ ((t / NU) & 7)) << 4)] = xr[j];
+        }
+    };
+    if (first < last) { fetch(first); put(0); }
+    __syncthreads();
+    for (int b = first; b < last; b++) {
+        const int buf = (b - first) & 1;
+        u32x4 a[4][2];
+        const uint8_t *block = g.val8 + (int64_t)b * kBlockBytes + (wm * 8 * kWave + lane) * 16;
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) a[s][h] = *(const u32x4 *)(block + (s * 2 + h) * kWave * 16);
+        const int sa = g.scale8[b];
+        // scale bytes of vectors v, v + 1, .. v + NU - 1; n > NU, so the load can move back from the end of the scales
+        const int v = v0 + wn * 16 * NU + NU * i, back = max(v + NU - g.n, 0);
+        uint64_t sx = 0;
+        __builtin_memcpy(&sx, g.xscale + (int64_t)g.col[b] * g.lds + (v - back), NU);
+        sx >>= 8 * min(back, 7);
+        auto scale_of = [&](int u) { return (unsigned)(sx >> (8 * u)); };    // in the low byte
+        fetch(min(b + 1, last - 1));                         // unconditional, like put below: one basic block, so that
+                                                             // nothing is moved across the loads and the barrier
+        if constexpr (EXACT) {
+            const float fa = scale_value(sa);
+            bf16x8 aw[4][4];
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int d = 0; d < 8; d++) unpack4(a[s][d >> 2][d & 3], fa, (__bf16 *)&aw[s][d >> 1] + 4 * (d & 1));
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                const int t = wn * 16 * NU + NU * i + u;
+                const float fx = scale_value(scale_of(u) & 255);
+                u32x4 x[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) x[h] = *(const u32x4 *)&X[buf][t * kB + (((h * 4 + q) ^ (i & 7)) << 4)];
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    bf16x8 xw;
+                    unpack4(x[p >> 1][2 * (p & 1)], fx, (__bf16 *)&xw);
+                    unpack4(x[p >> 1][2 * (p & 1) + 1], fx, (__bf16 *)&xw + 4);
+#pragma unroll
+                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw[s][p], xw, acc[u][s], 0, 0, 0);
                 }
-                for (int d = 0; d < 4; d++) unpack4(w[d], s, &Q[0][t][c + 4 * d]);
-            }
-        } else if (KIND == kTransposed) {
-            const int e = step >> 1, b = g.id[e], r0 = g.idx[e] * kB + half * 64;
-            const float sa = scale_value(g.scale8[b]);
-            for (int p = tid; p < 512; p += kBlock) {
-                const int strip = p >> 7, l = p & 127, ii = l & 15, qq = l >> 4;
-                const u32x4 w = *(const u32x4 *)(g.val8 + (int64_t)b * kBlockBytes + ((half * 4 + strip) * 128 + l) * 16);
-                const int r = 16 * (ii >> 2) + 4 * strip + (ii & 3);
-                __bf16 u[16];
-                for (int d = 0; d < 4; d++) unpack4(w[d], sa, u + 4 * d);
-                for (int d = 0; d < 16; d++) P[16 * qq + d][r] = u[d];
-            }
-            for (int p = tid; p < kTile * kDepth; p += kBlock) {
-                const int t = p >> 6, r = p & 63;
-                const float f = v0 + t < g.n && r0 + r < g.rows ? (float)dy[(int64_t)(v0 + t) * g.lddy + r0 + r] : 0.0f;
-                __bf16 u[PARTS];
-                split_bf16<PARTS>(f, u);
-                for (int k = 0; k < PARTS; k++) Q[k][t][r] = u[k];
             }
         } else {
-            const int t0 = step * kDepth, c0 = g.idx[major] * kB, r0 = g.block_row[major] * kB;
-            for (int p = tid; p < 512; p += kBlock) {
-                const int t = p >> 3, c = (p & 7) * 16;
-                u32x4 w = {0, 0, 0, 0};
-                float s = 1.0f;
-                if (t0 + t < g.n) {
-                    w = *(const u32x4 *)(g.x8 + (int64_t)(t0 + t) * g.ldx8 + c0 + c);
-                    s = scale_value(g.xscale[(int64_t)g.idx[major] * g.lds + t0 + t]);
+            auto read = [&](int u) {
+                const int t = wn * 16 * NU + NU * i + u;
+                i32x8 x;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const u32x4 w = *(const u32x4 *)&X[buf][t * kB + (((h * 4 + q) ^ (i & 7)) << 4)];
+#pragma unroll
+                    for (int d = 0; d < 4; d++) x[4 * h + d] = (int)w[d];
                 }
-                __bf16 u[16];
-                for (int d = 0; d < 4; d++) unpack4(w[d], s, u + 4 * d);
-                for (int d = 0; d < 16; d++) P[c + d][t] = u[d];
-            }
-            for (int p = tid; p < kTile * kDepth; p += kBlock) {
-                const int t = p >> 7, r = p & 127;
-                const float f = t0 + t < g.n && r0 + r < g.rows ? (float)dy[(int64_t)(t0 + t) * g.lddy + r0 + r] : 0.0f;
-                __bf16 u[PARTS];
-                split_bf16<PARTS>(f, u);
-                for (int k = 0; k < PARTS; k++) Q[k][r][t] = u[k];
+                return x;
+            };
+            i32x8 x = read(0);
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                // one tile's operand ahead and no more: left alone, the compiler reads all of them first and spills
+                i32x8 ahead = x;
+                if (u + 1 < NU) ahead = read(u + 1);
+                const int su = (int)scale_of(u);                             // the instruction reads the low byte
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    i32x8 aw;
+#pragma unroll
+                    for (int d = 0; d < 8; d++) aw[d] = (int)a[s][d >> 2][d & 3];
+                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aw, x, acc[u][s], 0, 0, 0, sa, 0, su);
+                }
+                x = ahead;
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        __syncthreads();
-        for (int k = 0; k < kDepth; k += 32) {
-            bf16x8 a[4];
-            for (int t = 0; t < 4; t++) a[t] = *(const bf16x8 *)&P[m0 + 16 * t + i][k + 8 * q];
-            for (int part = 0; part < PARTS; part++)
-                for (int u = 0; u < 4; u++) {
-                    const bf16x8 b = *(const bf16x8 *)&Q[part][n0 + 16 * u + i][k + 8 * q];
-                    for (int t = 0; t < 4; t++) acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[t], b, acc[t][u], 0, 0, 0);
-                }
-        }
+        put(buf ^ 1);
         __syncthreads();
     }
-    // lane (i, q) of a tile: N = i, M = 4 q .. 4 q + 3
-    for (int t = 0; t < 4; t++)
-        for (int u = 0; u < 4; u++) {
-            const int mm = m0 + 16 * t + 4 * q, nn = n0 + 16 * u + i;
-            if (KIND == kGradient) {
-                OT *o = out + (int64_t)major * kBlockBytes + nn * kB + mm;
-                const bool row_in = g.block_row[major] * kB + nn < g.rows;
-                for (int k = 0; k < 4; k++) {
-                    float v = row_in && g.idx[major] * kB + mm + k < g.columns ? acc[t][u][k] : 0.0f;
-                    if (g.accumulate) v += (float)o[k];
-                    o[k] = (OT)v;
+    // a lane has rows 16 q .. 16 q + 15 of its wave's 64 for NU vectors
+    const int r0 = major * kB + wm * 64 + 16 * q;
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+        const int v = v0 + wn * 16 * NU + NU * i + u;
+        if (v < g.n && r0 < g.rows) store_row<OT, 4>(y + (int64_t)v * g.ldy + r0, g.rows - r0, acc[u]);
+    }
+}
+
+// dy is used as it is: split into PARTS bf16 numbers that add up to it exactly (1 for bf16, 2 for fp16, 3 for fp32:
+// each holds 8 bits of the mantissa), one matrix instruction each
+template <typename DT> struct parts_of { static constexpr int value = 1; };
+template <> struct parts_of<_Float16> { static constexpr int value = 2; };
+template <> struct parts_of<float> { static constexpr int value = 3; };
+
+// 8 entries of dy as they lie in memory, zero from `left` on
+template <typename DT> struct Raw8 {
+    DT v[8];
+    __device__ __forceinline__ void load(const DT *p, int left)
+    {
+        if (left >= 8) __builtin_memcpy(v, p, sizeof v);
+        else
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = k < left ? p[k] : (DT)0.0f;
+    }
+    __device__ __forceinline__ void split(bf16x8 *part) const
+    {
+        if constexpr (std::is_same<DT, __bf16>::value) {
+            __builtin_memcpy(part, v, 16);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                float f = (float)v[k];
+#pragma unroll
+                for (int p = 0; p < parts_of<DT>::value; p++) {
+                    part[p][k] = (__bf16)f;
+                    f -= (float)part[p][k];
                 }
-            } else {
-                const int limit = KIND == kProduct ? g.rows : g.columns;
-                if (v0 + nn >= g.n) continue;
-                for (int k = 0; k < 4; k++)
-                    if (major * kB + mm + k < limit) out[(int64_t)(v0 + nn) * g.ldo + major * kB + mm + k] = (OT)acc[t][u][k];
             }
         }
+    }
+};
+
+struct TransposedArgs {
+    int n, rows, columns, bcols, vtiles;
+    const int *ptr, *row, *id, *scale8;
+    const uint8_t *val8;
+    int64_t lddy, lddx;
+};
+
+// dx = A^T dy.  Tile: one block column x TOK vectors, steps of half a block (64 rows); a wave has 64 columns x TOK / 2
+// vectors.  The block's bytes lie in LDS as in memory; ds_read_b64_tr_b8 hands every lane one column of 8 rows, widened
+// to bf16 (exact) on the way to the matrix instruction.  Those 8 rows are 4 s .. 4 s + 3 and 16 + 4 s .. of a
+// quarter (block8_offset), so dy is read in two 8-byte halves; its 16-byte pieces are exchanged by XOR in LDS.
+template <typename DT, int TOK, typename OT>
+__global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g, const DT *__restrict__ dy, OT *__restrict__ dx)
+{
+    constexpr int PARTS = parts_of<DT>::value, NU = TOK / 32, PIECES = TOK / 32;
+    __shared__ __bf16 Y[2][PARTS][TOK * 64];
+    __shared__ uint8_t A[2][kBlockBytes / 2];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
+    const int wm = wave & 1, wn = wave >> 1;
+    int major, vtile;
+    tile_of_block(blockIdx.x, g.bcols, g.vtiles, &major, &vtile);
+    const int v0 = vtile * TOK, first = 2 * g.ptr[major], last = 2 * g.ptr[major + 1];
+    f32x4 acc[NU][4];
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
+
+    Raw8<DT> yr[PIECES];
+    u32x4 ar[2];
+    auto fetch = [&](int step) {
+        const uint8_t *block = g.val8 + (int64_t)g.id[step >> 1] * kBlockBytes + (step & 1) * (kBlockBytes / 2) + tid * 16;
+        ar[0] = *(const u32x4 *)block;
+        ar[1] = *(const u32x4 *)(block + kBlock * 16);
+        const int r = g.row[step >> 1] * kB + (step & 1) * 64 + (tid & 7) * 8;
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            const int v = min(v0 + j * 32 + (tid >> 3), g.n - 1);
+            yr[j].load(dy + (int64_t)v * g.lddy + r, g.rows - r);
+        }
+    };
+    auto put = [&](int buf) {
+        *(u32x4 *)&A[buf][tid * 16] = ar[0];
+        *(u32x4 *)&A[buf][(kBlock + tid) * 16] = ar[1];
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            const int t = j * 32 + (tid >> 3);
+            bf16x8 part[PARTS];
+            yr[j].split(part);
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][t * 64 + (((tid & 7) ^ ((t >> 1) & 7)) << 3)] = part[p];
+        }
+    };
+    if (first < last) { fetch(first); put(0); }
+    __syncthreads();
+    for (int step = first; step < last; step++) {
+        const int buf = step & 1;                            // first is even
+        const float sa = scale_value(g.scale8[g.id[step >> 1]]);
+        fetch(min(step + 1, last - 1));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int strip = 2 * k + (q >> 1);
+            bf16x8 a[4];
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2 *)&A[buf][(strip * 8 + wm * 4 + s) * 256 + (q & 1) * 128 + i * 8]);
+                unpack4((unsigned)w[0], sa, (__bf16 *)&a[s]);
+                unpack4((unsigned)w[1], sa, (__bf16 *)&a[s] + 4);
+            }
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                for (int u = 0; u < NU; u++) {
+                    const int t = wn * 16 * NU + 16 * u + i, f = (t >> 1) & 7, c = 4 * (q & 1) + k, o = t * 64 + 4 * (q >> 1);
+                    bf16x8 b;
+                    __builtin_memcpy(&b, &Y[buf][p][o + ((c ^ f) << 3)], 8);
+                    __builtin_memcpy((__bf16 *)&b + 4, &Y[buf][p][o + (((c + 2) ^ f) << 3)], 8);
+#pragma unroll
+                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
+                }
+        }
+        put(buf ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+        const int v = v0 + wn * 16 * NU + 16 * u + i;
+        if (v >= g.n) continue;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const int c = major * kB + wm * 64 + 16 * s + 4 * q;
+            if (c < g.columns) store_row<OT, 1>(dx + (int64_t)v * g.lddx + c, g.columns - c, &acc[u][s]);
+        }
+    }
+}
+
+struct GradientArgs {
+    int n, rows, columns, accumulate;
+    const int *list;               // NB blocks of one block row per workgroup, -1 = none
+    const int *block_row, *block_col;
+    const uint8_t *x8, *xscale;
+    int64_t ldx8, lds, lddy;
+};
+
+// dA = dy^T x at the stored blocks.  Tile: NB blocks of one block row, steps of 32 vectors; with two blocks a wave has 64
+// rows x 128 columns, with one 64 x 64.  Both operands lie vector by vector, along the sum, and are turned by ds_read_b64_tr_b16
+// on their way out of LDS; x is widened with its scales (exact) on its way in.  The 32 bytes between the rows of LDS
+// put the 4 rows of a read on different banks.
+template <typename DT, int NB, typename OT>
+__global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, const DT *__restrict__ dy, OT *__restrict__ dv)
+{
+    constexpr int PARTS = parts_of<DT>::value, STEP = 32, NM = 4 * NB, XP = NB * kB + 16, YP = kB + 16;
+    __shared__ __bf16 X[2][STEP * XP];
+    __shared__ __bf16 Y[2][PARTS][STEP * YP];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
+    const int wm = wave & 1, wn = wave >> 1;
+    const int wg = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
+    int id[NB], col[NB];
+#pragma unroll
+    for (int k = 0; k < NB; k++) {
+        id[k] = g.list ? g.list[NB * wg + k] : wg;
+        col[k] = g.block_col[id[k] < 0 ? id[0] : id[k]];                     // the second one may be missing: computed, not stored
+    }
+    const int row0 = g.block_row[id[0]] * kB;
+    f32x4 acc[4][NM];
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int s = 0; s < NM; s++) acc[u][s] = f32x4{0, 0, 0, 0};
+
+    Raw8<DT> yr[2];
+    u32x4 xr[NB];
+    int sx[NB];
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int t = t0 + j * 16 + (tid >> 4), r = row0 + (tid & 15) * 8;
+            yr[j].load(dy + (int64_t)min(t, g.n - 1) * g.lddy + r, t < g.n ? g.rows - r : 0);
+        }
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            const int t = t0 + (tid >> 3), v = min(t, g.n - 1);
+            xr[k] = *(const u32x4 *)(g.x8 + (int64_t)v * g.ldx8 + col[k] * kB + (tid & 7) * 16);
+            sx[k] = g.xscale[(int64_t)col[k] * g.lds + v];
+            if (t >= g.n) xr[k] = u32x4{0, 0, 0, 0};
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            bf16x8 part[PARTS];
+            yr[j].split(part);
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][(j * 16 + (tid >> 4)) * YP + (tid & 15) * 8] = part[p];
+        }
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            bf16x8 w[2];
+            const float s = scale_value(sx[k]);
+#pragma unroll
+            for (int d = 0; d < 4; d++) unpack4(xr[k][d], s, (__bf16 *)&w[d >> 1] + 4 * (d & 1));
+            *(bf16x8 *)&X[buf][(tid >> 3) * XP + k * kB + (tid & 7) * 16] = w[0];
+            *(bf16x8 *)&X[buf][(tid >> 3) * XP + k * kB + (tid & 7) * 16 + 8] = w[1];
+        }
+    };
+    // lane (i, q) of an operand: column `at` + i, vectors 8 q .. 8 q + 7
+    auto turned = [&](const __bf16 *p, int pitch, int at) {
+        typedef short i16x4 __attribute__((ext_vector_type(4)));
+        union { i16x4 h[2]; bf16x8 v; } u;
+        const __bf16 *a = p + (8 * q + (i >> 2)) * pitch + at + (i & 3) * 4;
+        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)a);
+        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + 4 * pitch));
+        return u.v;
+    };
+    if (g.n > 0) { fetch(0); put(0); }
+    __syncthreads();
+    for (int t0 = 0; t0 < g.n; t0 += STEP) {
+        const int buf = (t0 / STEP) & 1;
+        fetch(t0 + STEP);                                    // past the end: zeros
+        bf16x8 a[NM];
+#pragma unroll
+        for (int s = 0; s < NM; s++) a[s] = turned(X[buf], XP, wm * 64 * NB + 16 * s);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const bf16x8 b = turned(Y[buf][p], YP, wn * 64 + 16 * u);
+#pragma unroll
+                for (int s = 0; s < NM; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
+            }
+        put(buf ^ 1);
+        __syncthreads();
+    }
+    const int mine = NB == 2 ? wm : 0;
+    if (id[mine] < 0) return;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int r = wn * 64 + 16 * u + i;
+#pragma unroll
+        for (int s = 0; s < NM; s++) {
+            const int c = (NB == 2 ? 0 : wm * 64) + 16 * s + 4 * q;
+            OT *o = dv + (int64_t)id[mine] * kBlockBytes + r * kB + c;
+            f32x4 v = acc[u][s];
+            // beyond the edge: dy is zero there along the rows, x along the columns unless it holds what is not finite
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (row0 + r >= g.rows || col[mine] * kB + c + k >= g.columns) v[k] = 0.0f;
+                if (g.accumulate) v[k] += (float)o[k];
+            }
+            store_row<OT, 1>(o, 4, &v);
+        }
+    }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------
@@ -470,6 +752,10 @@ static int check_eight(const char *what, int n, int columns, const void *x8, int
         return 1;
     }
     if ((uintptr_t)x8 % 16) { set_error("%s: 8-bit vectors are not 16-byte aligned", what); return 1; }
+    if (ldx8 >= (int64_t)1 << 24) {          // 256 of them stay inside 32-bit offsets
+        set_error("%s: 8-bit vectors %lld apart, at most 2^24 - 128", what, (long long)ldx8);
+        return 1;
+    }
     if (lds < n) { set_error("%s: %lld scales per group for %d vectors", what, (long long)lds, n); return 1; }
     return 0;
 }
@@ -484,6 +770,20 @@ static int check_groups(const char *what, int64_t ngroups)
 {
     if (ngroups <= (int64_t)0x7fffffff * (kBlock / 16)) return 0;
     set_error("%s: %lld groups of 128 are more than one launch takes", what, (long long)ngroups);
+    return 1;
+}
+
+// Vectors a workgroup takes: `most` where that still gives every CU a tile, else half, down to 64
+static int vectors_per_tile(const spmv_hip_matrix *m, int majors, int n, int most)
+{
+    int tile = most;
+    while (tile > 64 && (int64_t)majors * ((n + tile - 1) / tile) < m->cus) tile /= 2;
+    return tile;
+}
+static int check_tiles(const char *what, int majors, int vtiles)
+{
+    if ((int64_t)majors * vtiles <= 0x7fffffff) return 0;
+    set_error("%s: %d x %d tiles are more than one launch takes", what, majors, vtiles);
     return 1;
 }
 
@@ -513,6 +813,7 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
     m->nblocks = nblocks; m->brows = brows; m->bcols = bcols;
     m->stored = (int64_t)nblocks * kBlockBytes;
     if (hipGetDevice(&m->device) != hipSuccess) { set_error("no HIP device available"); delete m; return nullptr; }
+    if (hipDeviceGetAttribute(&m->cus, hipDeviceAttributeMultiprocessorCount, m->device) != hipSuccess) m->cus = 0;
     (void)hipGetLastError();
     bool ok = false;
     try {
@@ -532,6 +833,14 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
             trow[(size_t)w] = row[(size_t)k];
             tid[(size_t)w] = k;
         }
+        // two neighbours of a block row each, for the gradient
+        std::vector<int> pair;
+        for (int r = 0; r < brows; r++)
+            for (int k = block_ptr[r]; k < block_ptr[r + 1]; k += 2) {
+                pair.push_back(k);
+                pair.push_back(k + 1 < block_ptr[r + 1] ? k + 1 : -1);
+            }
+        m->npairs = (int)(pair.size() / 2);
         const std::vector<int> scale((size_t)nblocks, 127);
         auto up = [&](int **d, const int *h, size_t count) {
             if (dev_alloc(m, d, count)) return false;
@@ -541,7 +850,7 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
         ok = up(&m->d_block_ptr, block_ptr, (size_t)brows + 1) && up(&m->d_block_col, block_col, (size_t)nblocks) &&
              up(&m->d_block_row, row.data(), (size_t)nblocks) && up(&m->d_bt_ptr, tptr.data(), (size_t)bcols + 1) &&
              up(&m->d_bt_row, trow.data(), (size_t)nblocks) && up(&m->d_bt_id, tid.data(), (size_t)nblocks) &&
-             up(&m->d_scale8, scale.data(), (size_t)nblocks) && dev_alloc(m, &m->d_val8, (size_t)nblocks * kBlockBytes) == 0;
+             up(&m->d_pair, pair.data(), pair.size()) && up(&m->d_scale8, scale.data(), (size_t)nblocks) && dev_alloc(m, &m->d_val8, (size_t)nblocks * kBlockBytes) == 0;
         if (ok && nblocks) {
             ok = hipMemset(m->d_val8, 0, (size_t)nblocks * kBlockBytes) == hipSuccess && hipDeviceSynchronize() == hipSuccess;
             if (!ok) set_error("clearing the blocks failed");
@@ -649,16 +958,22 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     if (!on.ok) return 1;
     if (n <= SPMV_HIP_BLOCK8_MAX_WIDE)
         return launch_few(m, n, d_x, x_dtype, ldx, d_scale, lds, d_y, y_dtype, ldy, (hipStream_t)stream);
-    MatrixArgs a{};
-    a.n = n; a.rows = m->rows; a.columns = m->columns;
-    a.ptr = m->d_block_ptr; a.idx = m->d_block_col; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
-    a.x8 = (const uint8_t *)d_x; a.xscale = d_scale; a.ldx8 = ldx; a.lds = lds; a.ldo = ldy;
-    const dim3 grid(m->brows, (n + kTile - 1) / kTile);
-    if (grid.y > 65535) { set_error("%s: %d vectors are more than one launch takes", what, n); return 1; }
+    ProductArgs a{};
+    a.n = n; a.rows = m->rows; a.brows = m->brows;
+    a.ptr = m->d_block_ptr; a.col = m->d_block_col; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
+    a.x8 = (const uint8_t *)d_x; a.xscale = d_scale; a.ldx8 = ldx; a.lds = lds; a.ldy = ldy;
+    const int tile = vectors_per_tile(m, m->brows, n, y_dtype == SPMV_HIP_BF16 ? 256 : 128);
+    a.vtiles = (n + tile - 1) / tile;
+    if (check_tiles(what, m->brows, a.vtiles)) return 1;
     with_elem(y_dtype, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((many_vectors_kernel<kProduct, float, 1, T>), grid, dim3(kBlock), 0, (hipStream_t)stream, a,
-                           (const float *)nullptr, (T *)d_y);
+        constexpr bool exact = !std::is_same<T, __bf16>::value;
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(m->brows * a.vtiles), dim3(kBlock), 0, (hipStream_t)stream, a, (T *)d_y);
+        };
+        if constexpr (!exact) if (tile == 256) { go(product_kernel<exact, 256, T>); return; }
+        if (tile == 128) go(product_kernel<exact, 128, T>);
+        else go(product_kernel<exact, 64, T>);
     });
     return launched(what);
 }
@@ -674,19 +989,23 @@ int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy
     if (n == 0 || m->columns == 0) return 0;
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
-    MatrixArgs a{};
-    a.n = n; a.rows = m->rows; a.columns = m->columns;
-    a.ptr = m->d_bt_ptr; a.idx = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
-    a.lddy = lddy; a.ldo = lddx;
-    const dim3 grid(m->bcols, (n + kTile - 1) / kTile);
-    if (grid.y > 65535) { set_error("%s: %d vectors are more than one launch takes", what, n); return 1; }
+    TransposedArgs a{};
+    a.n = n; a.rows = m->rows; a.columns = m->columns; a.bcols = m->bcols;
+    a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
+    a.lddy = lddy; a.lddx = lddx;
+    const int tile = vectors_per_tile(m, m->bcols, n, dy_dtype == SPMV_HIP_BF16 ? 256 : 128);
+    a.vtiles = (n + tile - 1) / tile;
+    if (check_tiles(what, m->bcols, a.vtiles)) return 1;
     with_elem(dy_dtype, [&](auto t) {
         typedef decltype(t) T;
-        constexpr int parts = std::is_same<T, float>::value ? 3 : std::is_same<T, __bf16>::value ? 1 : 2;
         with_elem(dx_dtype, [&](auto o) {
             typedef decltype(o) O;
-            hipLaunchKernelGGL((many_vectors_kernel<kTransposed, T, parts, O>), grid, dim3(kBlock), 0, (hipStream_t)stream, a,
-                               (const T *)d_dy, (O *)d_dx);
+            auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles), dim3(kBlock), 0, (hipStream_t)stream, a, (const T *)d_dy, (O *)d_dx);
+            };
+            if constexpr (std::is_same<T, __bf16>::value) if (tile == 256) { go(transposed_kernel<T, 256, O>); return; }
+            if (tile == 128) go(transposed_kernel<T, 128, O>);
+            else go(transposed_kernel<T, 64, O>);
         });
     });
     return launched(what);
@@ -705,17 +1024,21 @@ int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_
     if (!d_dvalues) { set_error("%s: NULL gradient", what); return 1; }
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
-    MatrixArgs a{};
+    GradientArgs a{};
     a.n = n; a.rows = m->rows; a.columns = m->columns; a.accumulate = accumulate;
-    a.idx = m->d_block_col; a.block_row = m->d_block_row;
+    a.block_row = m->d_block_row; a.block_col = m->d_block_col;
     a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.lddy = lddy;
+    const bool pairs = m->npairs >= m->cus;                  // two blocks a workgroup once they fill the GPU
+    a.list = pairs ? m->d_pair : nullptr;
     with_elem(dy_dtype, [&](auto t) {
         typedef decltype(t) T;
-        constexpr int parts = std::is_same<T, float>::value ? 3 : std::is_same<T, __bf16>::value ? 1 : 2;
         with_elem(dtype, [&](auto o) {
             typedef decltype(o) O;
-            hipLaunchKernelGGL((many_vectors_kernel<kGradient, T, parts, O>), dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream,
-                               a, (const T *)d_dy, (O *)d_dvalues);
+            auto go = [&](auto kernel, int count) {
+                hipLaunchKernelGGL(kernel, dim3(count), dim3(kBlock), 0, (hipStream_t)stream, a, (const T *)d_dy, (O *)d_dvalues);
+            };
+            if (pairs) go(gradient_kernel<T, 2, O>, m->npairs);
+            else go(gradient_kernel<T, 1, O>, m->nblocks);
         });
     });
     return launched(what);
