@@ -40,18 +40,6 @@ __device__ __forceinline__ int scale_byte(float amax)
     const int e = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8;      // exponent byte of the scale
     return e < 1 ? 1 : e;
 }
-__device__ __forceinline__ float scale_inverse(int b) { return __int_as_float((254 - b) << 23); }   // 2^(127-b), b <= 253
-__device__ __forceinline__ float finite_abs(float v)
-{
-    const float a = fabsf(v);
-    return a < __builtin_inff() ? a : 0.0f;                                  // false for NaN too
-}
-// four scaled values -> four e4m3 bytes, nearest even; beyond 448 (only +-inf here) and NaN -> NaN
-__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d)
-{
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-}
 // four e4m3 bytes times a power of two -> four bf16, exact
 __device__ __forceinline__ void unpack4(unsigned w, float scale, __bf16 *out)
 {
@@ -76,31 +64,122 @@ template <typename F> static void with_elem(int dtype, F f)
     else f(_Float16());
 }
 
+// K entries of a vector as they lie in memory (any alignment), zero from `left` on
+template <typename T, int K> struct Raw {
+    T v[K];
+    __device__ __forceinline__ void load(const T *p, int left)
+    {
+        if (left >= K) __builtin_memcpy(v, p, sizeof v);
+        else
+#pragma unroll
+            for (int k = 0; k < K; k++) v[k] = k < left ? p[k] : (T)0.0f;
+    }
+    // the largest magnitude's bits, of numbers that are not finite too
+    __device__ __forceinline__ unsigned top() const
+    {
+        unsigned m = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < K; k++) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+            return m;
+        } else {
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 w[K / 2], t = {0, 0};
+            __builtin_memcpy(w, v, sizeof v);
+#pragma unroll
+            for (int k = 0; k < K / 2; k++) t = __builtin_elementwise_max(t, (u16x2)(w[k] & (unsigned short)0x7fff));
+            return max((unsigned)t[0], (unsigned)t[1]);
+        }
+    }
+    // K / 4 words of e4m3 of v / scale, scale a power of two; infinities and NaN give NaN
+    __device__ __forceinline__ void pack(float scale, unsigned *w) const
+    {
+        typedef short i16x2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int k = 0; k < K; k += 4) {
+            i16x2 o = {0, 0};
+            if constexpr (std::is_same<T, float>::value) {
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, v[k], v[k + 1], scale, false);
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, v[k + 2], v[k + 3], scale, true);
+            } else if constexpr (std::is_same<T, __bf16>::value) {
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, bf16x2{v[k], v[k + 1]}, scale, false);
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, bf16x2{v[k + 2], v[k + 3]}, scale, true);
+            } else {
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, f16x2{v[k], v[k + 1]}, scale, false);
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, f16x2{v[k + 2], v[k + 3]}, scale, true);
+            }
+            __builtin_memcpy(&w[k / 4], &o, 4);
+        }
+    }
+};
+
+// the largest finite magnitude of a lane's entries
+template <typename T, int K> __device__ __forceinline__ float finite_top(const Raw<T, K> &r)
+{
+    constexpr unsigned inf = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+    unsigned m = r.top();
+    if (m >= inf) {                                          // rare: leave out what is not finite
+        m = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            Raw<T, 2> one{{r.v[k], (T)0.0f}};
+            const unsigned t = one.top();
+            m = t < inf ? max(m, t) : m;
+        }
+    }
+    if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+    else {
+        const unsigned short h = (unsigned short)m;
+        T v;
+        __builtin_memcpy(&v, &h, 2);
+        return (float)v;
+    }
+}
+
 // ---- to 8 bits and back ---------------------------------------------------------------------------------------
 
-// 16 lanes per group of 128, 8 entries per lane
-template <typename T>
-__global__ __launch_bounds__(kBlock) void quantize8_kernel(int64_t ngroups, int groups, int columns, const T *__restrict__ x,
-                                                           int64_t ldx, uint8_t *__restrict__ x8, int64_t ldx8,
-                                                           uint8_t *__restrict__ scale, int64_t lds)
+// Bound by memory.  A wave takes 4 neighbouring groups of R vectors in turn (16 lanes a group, 8 entries a lane), four loads
+// in flight; the scale bytes meet in LDS, because those of one group lie vector by vector.  R = 16 where that leaves
+// 2048 workgroups, else 1: few vectors are all latency.
+constexpr int kQuantGroups = 4, kQuantWaves = kBlock / kWave;
+
+template <typename T, int R>
+__global__ __launch_bounds__(kBlock) void quantize8_kernel(int n, int groups, int columns, const T *__restrict__ x, int64_t ldx,
+                                                           uint8_t *__restrict__ x8, int64_t ldx8, uint8_t *__restrict__ scale,
+                                                           int64_t lds)
 {
-    const int64_t id = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> 4;
-    const int sub = threadIdx.x & 15;
-    if (id >= ngroups) return;                               // whole groups of 16 lanes leave together
-    const int64_t v = id / groups;
-    const int g = (int)(id % groups), c0 = g * kB + sub * 8;
-    float a[8], amax = 0.0f;
-    for (int k = 0; k < 8; k++) {
-        a[k] = c0 + k < columns ? (float)x[v * ldx + c0 + k] : 0.0f;
-        amax = fmaxf(amax, finite_abs(a[k]));
+    constexpr int U = R < 4 ? R : 4, TV = R * kQuantWaves;
+    __shared__ uint8_t bytes[kQuantGroups][TV];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, gq = lane >> 4;
+    const int g0 = blockIdx.y * kQuantGroups, c = (g0 + gq) * kB + (lane & 15) * 8;
+    const int64_t v0 = (int64_t)blockIdx.x * TV;
+    for (int r = 0; r < R; r += U) {
+        Raw<T, 8> a[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t v = v0 + wave * R + r + u;
+            a[u].load(x + (v < n ? v : n - 1) * ldx + c, columns - c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t v = v0 + wave * R + r + u;
+            float top = finite_top(a[u]);
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+            const int b = scale_byte(top);
+            unsigned w[2];
+            a[u].pack(scale_value(b), w);
+            if (v < n && g0 + gq < groups) *(uint2 *)(x8 + v * ldx8 + c) = uint2{w[0], w[1]};
+            if ((lane & 15) == 0) bytes[gq][wave * R + r + u] = (uint8_t)b;
+        }
     }
-    for (int d = 1; d < 16; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-    const int b = scale_byte(amax);
-    const float inv = scale_inverse(b);
-    for (int k = 0; k < 8; k++) a[k] *= inv;
-    uint2 w = {pack4(a[0], a[1], a[2], a[3]), pack4(a[4], a[5], a[6], a[7])};
-    *(uint2 *)(x8 + v * ldx8 + c0) = w;
-    if (sub == 0) scale[(int64_t)g * lds + v] = (uint8_t)b;
+    __syncthreads();
+    for (int t = threadIdx.x; t < kQuantGroups * TV; t += kBlock) {
+        const int g = g0 + t / TV;
+        const int64_t v = v0 + t % TV;
+        if (g < groups && v < n) scale[(int64_t)g * lds + v] = bytes[t / TV][t % TV];
+    }
 }
 
 template <typename T> __device__ __forceinline__ float largest_finite();
@@ -108,61 +187,93 @@ template <> __device__ __forceinline__ float largest_finite<float>() { return 3.
 template <> __device__ __forceinline__ float largest_finite<__bf16>() { return 3.38953139e38f; }
 template <> __device__ __forceinline__ float largest_finite<_Float16>() { return 65504.0f; }
 
-template <typename T>
-__global__ __launch_bounds__(kBlock) void restore8_kernel(int64_t ngroups, int groups, int columns, const uint8_t *__restrict__ x8,
+template <typename T, int R>
+__global__ __launch_bounds__(kBlock) void restore8_kernel(int n, int groups, int columns, const uint8_t *__restrict__ x8,
                                                           int64_t ldx8, const uint8_t *__restrict__ scale, int64_t lds,
                                                           T *__restrict__ x, int64_t ldx)
 {
-    const int64_t id = ((int64_t)blockIdx.x * kBlock + threadIdx.x) >> 4;
-    const int sub = threadIdx.x & 15;
-    if (id >= ngroups) return;
-    const int64_t v = id / groups;
-    const int g = (int)(id % groups), c0 = g * kB + sub * 8;
-    const uint2 w = *(const uint2 *)(x8 + v * ldx8 + c0);
-    const float s = scale_value(scale[(int64_t)g * lds + v]), top = largest_finite<T>();
-    float a[8];
-    for (int h = 0; h < 2; h++) {
-        const unsigned u = h ? w.y : w.x;
-        a[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8(u, 0) * s;
-        a[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(u, 1) * s;
-        a[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(u, 2) * s;
-        a[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(u, 3) * s;
-    }
-    for (int k = 0; k < 8; k++) {
-        const float y = a[k] > top ? top : a[k] < -top ? -top : a[k];        // NaN stays
-        if (c0 + k < columns) x[v * ldx + c0 + k] = (T)y;
+    constexpr int U = R < 4 ? R : 4;
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int g = blockIdx.y * kQuantGroups + (lane >> 4), c = g * kB + (lane & 15) * 8;
+    if (g >= groups) return;
+    const int64_t v0 = ((int64_t)blockIdx.x * kQuantWaves + wave) * R;
+    const float top = largest_finite<T>();
+    for (int r = 0; r < R; r += U) {
+        uint2 w[U];
+        int b[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t v = v0 + r + u < n ? v0 + r + u : n - 1;
+            w[u] = *(const uint2 *)(x8 + v * ldx8 + c);
+            b[u] = scale[(int64_t)g * lds + v];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float s = scale_value(b[u]);
+            T y[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                typedef float f32x2 __attribute__((ext_vector_type(2)));
+                const f32x2 p = (k & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(k < 4 ? w[u].x : w[u].y, true)
+                                        : __builtin_amdgcn_cvt_pk_f32_fp8(k < 4 ? w[u].x : w[u].y, false);
+                const float f = p[k & 1] * s;
+                y[k] = (T)(f > top ? top : f < -top ? -top : f);             // NaN stays
+            }
+            if (v0 + r + u >= n) continue;
+            T *o = x + (v0 + r + u) * ldx + c;
+            if (columns - c >= 8) __builtin_memcpy(o, y, sizeof y);
+            else
+                for (int k = 0; k < 8; k++)
+                    if (k < columns - c) o[k] = y[k];
+        }
     }
 }
 
-// one workgroup per block; thread t holds half a row
+// One workgroup per block, its 16384 values in registers; the 8-bit block is put in the handle's order in LDS.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void set_values_kernel(int rows, int columns, const int *__restrict__ block_row,
                                                             const int *__restrict__ block_col, const T *__restrict__ values,
                                                             uint8_t *__restrict__ val8, int *__restrict__ scale8)
 {
     __shared__ float part[kBlock / kWave];
+    __shared__ uint8_t out[kBlockBytes];
     const int64_t k = blockIdx.x;
-    const int r = threadIdx.x >> 1, c0 = (threadIdx.x & 1) * 64;
-    const bool row_in = block_row[k] * kB + r < rows;
-    const int cols_in = columns - block_col[k] * kB;
-    float a[64], amax = 0.0f;
-    for (int c = 0; c < 64; c++) {
-        a[c] = row_in && c0 + c < cols_in ? (float)values[k * kBlockBytes + r * kB + c0 + c] : 0.0f;
-        amax = fmaxf(amax, finite_abs(a[c]));
+    const int r0 = threadIdx.x >> 4, c = (threadIdx.x & 15) * 8;
+    const int rows_in = rows - block_row[k] * kB, cols_in = columns - block_col[k] * kB;
+    Raw<T, 8> a[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int r = j * 16 + r0;
+        a[j].load(values + k * kBlockBytes + r * kB + c, r < rows_in ? cols_in - c : 0);
     }
-    for (int d = 1; d < kWave; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-    if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = amax;
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = fmaxf(top, finite_top(a[j]));
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    if ((threadIdx.x & (kWave - 1)) == 0) part[threadIdx.x / kWave] = top;
     __syncthreads();
-    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const int b = scale_byte(amax);
-    const float inv = scale_inverse(b);
-    for (int c = 0; c < 64; c += 16) {
-        u32x4 w;
-        for (int d = 0; d < 4; d++)
-            w[d] = pack4(a[c + 4 * d] * inv, a[c + 4 * d + 1] * inv, a[c + 4 * d + 2] * inv, a[c + 4 * d + 3] * inv);
-        *(u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c0 + c)) = w;
+    const int b = scale_byte(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        unsigned w[2];
+        a[j].pack(scale_value(b), w);
+        *(uint2 *)&out[block8_offset(j * 16 + r0, c)] = uint2{w[0], w[1]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int at = (j * kBlock + threadIdx.x) * 16;
+        *(u32x4 *)(val8 + k * kBlockBytes + at) = *(const u32x4 *)&out[at];
     }
     if (threadIdx.x == 0) scale8[k] = b;
+}
+
+__device__ __forceinline__ u32x4 load16(const void *p)       // any alignment
+{
+    u32x4 w;
+    __builtin_memcpy(&w, p, 16);
+    return w;
 }
 
 // row-major 8-bit blocks into the handle's order and back
@@ -175,9 +286,13 @@ __global__ __launch_bounds__(kBlock) void load8_kernel(int rows, int columns, co
     for (int p = threadIdx.x; p < kBlockBytes / 16; p += kBlock) {
         const int r = p >> 3, c = (p & 7) * 16;
         const int left = block_row[k] * kB + r < rows ? columns - block_col[k] * kB - c : 0;      // bytes inside the matrix
-        union { uint8_t b[16]; u32x4 w; } u;
-        for (int j = 0; j < 16; j++) u.b[j] = j < left ? values8[k * kBlockBytes + p * 16 + j] : (uint8_t)0;
-        *(u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c)) = u.w;
+        u32x4 w = load16(values8 + k * kBlockBytes + p * 16);
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            const int keep = left - 4 * d;
+            if (keep < 4) w[d] &= keep <= 0 ? 0u : (1u << (8 * keep)) - 1;
+        }
+        *(u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c)) = w;
     }
     if (threadIdx.x == 0) scale8[k] = scale[k];
 }
@@ -187,77 +302,119 @@ __global__ __launch_bounds__(kBlock) void store8_kernel(const uint8_t *__restric
 {
     const int64_t k = blockIdx.x;
     for (int p = threadIdx.x; p < kBlockBytes / 16; p += kBlock) {
-        const int r = p >> 3, c = (p & 7) * 16;
-        union { uint8_t b[16]; u32x4 w; } u;
-        u.w = *(const u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c));
-        for (int j = 0; j < 16; j++) values8[k * kBlockBytes + p * 16 + j] = u.b[j];
+        const u32x4 w = *(const u32x4 *)(val8 + k * kBlockBytes + block8_offset(p >> 3, (p & 7) * 16));
+        __builtin_memcpy(values8 + k * kBlockBytes + p * 16, &w, 16);
     }
     if (threadIdx.x == 0) scale[k] = (uint8_t)scale8[k];
 }
 
 // ---- few vectors ----------------------------------------------------------------------------------------------
 
-// One workgroup per strip of 16 rows; its waves take the strip's blocks in turn and add their results in LDS.
-// Bound by reading the matrix once.  NT tiles of 16 vectors.  XT: uint8_t (x in 8 bits) or a wide type, rounded to 8 bits
-// here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.
-template <typename XT, int NT>
-__global__ __launch_bounds__(kBlock) void few_vectors_kernel(int n, int rows, int columns, const int *__restrict__ block_ptr,
-                                                             const int *__restrict__ block_col, const uint8_t *__restrict__ val8,
-                                                             const int *__restrict__ scale8, const XT *__restrict__ x,
-                                                             int64_t ldx, const uint8_t *__restrict__ xscale, int64_t lds,
-                                                             void *__restrict__ y, int y_dtype, int64_t ldy)
+// One workgroup per strip of 16 rows; its W waves take the strip's blocks in turn and add their results in LDS.
+// Bound by reading the matrix once, and for small matrices by latency: a wave's next block is on its way while
+// it works on one.  NT tiles of 16 vectors.  XT: uint8_t (x in 8 bits) or a wide type, rounded to 8 bits
+// here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.  Operands are widened
+// to bf16 (exact), sums are 32 bits.
+template <typename XT, int NT, int W>
+__global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, int columns, const int *__restrict__ block_ptr,
+                                                               const int *__restrict__ block_col, const uint8_t *__restrict__ val8,
+                                                               const int *__restrict__ scale8, const XT *__restrict__ x,
+                                                               int64_t ldx, const uint8_t *__restrict__ xscale, int64_t lds,
+                                                               void *__restrict__ y, int y_dtype, int64_t ldy)
 {
-    constexpr int kWaves = kBlock / kWave;
-    __shared__ f32x4 part[kWaves][NT][kWave];
+    constexpr bool kEight = std::is_same<XT, uint8_t>::value;
+    __shared__ f32x4 part[W][NT][kWave];
     const int brow = blockIdx.x >> 3, strip = blockIdx.x & 7;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, i = lane & 15, q = lane >> 4;
     f32x4 acc[NT];
+#pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
-    for (int b = block_ptr[brow] + wave; b < block_ptr[brow + 1]; b += kWaves) {
-        const int c0 = block_col[b] * kB;
-        const float sa = scale_value(scale8[b]);
-        bf16x8 a[4];
-        for (int h = 0; h < 2; h++) {
-            const u32x4 w = *(const u32x4 *)(val8 + (int64_t)b * kBlockBytes + ((strip * 2 + h) * kWave + lane) * 16);
-            for (int d = 0; d < 4; d++) unpack4(w[d], sa, (__bf16 *)&a[2 * h + (d >> 1)] + 4 * (d & 1));
+    // vectors past the last read the last: a column of the result that is not stored
+    int64_t vec[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) vec[t] = min(t * 16 + i, n - 1);
+
+    constexpr int AHEAD = NT == 1;                           // x ahead too; with more tiles registers run out
+    struct Vector {
+        Raw<XT, 16> h[2];
+        int scale;
+    };
+    struct Stage {
+        u32x4 a[2];
+        int scale, group;
+        Vector x;
+    };
+    auto load_x = [&](int t, int group) {
+        Vector r;
+        const int c = group * kB + 16 * q;
+        const XT *p = x + vec[t] * ldx + c;
+        if constexpr (kEight) {
+            r.h[0].load(p, 16);
+            r.h[1].load(p + 64, 16);
+            r.scale = xscale[(int64_t)group * lds + vec[t]];
+        } else {
+            r.h[0].load(p, columns - c);
+            r.h[1].load(p + 64, columns - c - 64);
         }
+        return r;
+    };
+    auto load = [&](int b) {
+        Stage s;
+        const uint8_t *block = val8 + (int64_t)b * kBlockBytes + (strip * 2 * kWave + lane) * 16;
+        s.a[0] = *(const u32x4 *)block;
+        s.a[1] = *(const u32x4 *)(block + kWave * 16);
+        s.scale = scale8[b];
+        s.group = block_col[b];
+        if (AHEAD) s.x = load_x(0, s.group);
+        return s;
+    };
+    auto use = [&](const Stage &s) {
+        const float sa = scale_value(s.scale);
+        bf16x8 a[4];
+#pragma unroll
+        for (int d = 0; d < 8; d++) unpack4(s.a[d >> 2][d & 3], sa, (__bf16 *)&a[d >> 1] + 4 * (d & 1));
+#pragma unroll
         for (int t = 0; t < NT; t++) {
-            const int v = t * 16 + i;
+            const Vector v = AHEAD ? s.x : load_x(t, s.group);
             unsigned w8[8];
-            int sx = 127;
-            if constexpr (std::is_same<XT, uint8_t>::value) {
-                for (int d = 0; d < 8; d++)
-                    w8[d] = v < n ? *(const unsigned *)(x + (int64_t)v * ldx + c0 + 64 * (d >> 2) + 16 * q + 4 * (d & 3)) : 0u;
-                if (v < n) sx = xscale[(int64_t)block_col[b] * lds + v];
+            float sx;
+            if constexpr (kEight) {
+                __builtin_memcpy(w8, v.h, 32);
+                sx = scale_value(v.scale);
             } else {
-                float f[32], amax = 0.0f;
-                for (int k = 0; k < 32; k++) {
-                    const int c = c0 + 64 * (k >> 4) + 16 * q + (k & 15);
-                    f[k] = v < n && c < columns ? (float)x[(int64_t)v * ldx + c] : 0.0f;
-                    amax = fmaxf(amax, finite_abs(f[k]));
-                }
-                amax = fmaxf(amax, __shfl_xor(amax, 16));
-                amax = fmaxf(amax, __shfl_xor(amax, 32));
-                sx = scale_byte(amax);
-                const float inv = scale_inverse(sx);
-                for (int d = 0; d < 8; d++)
-                    w8[d] = pack4(f[4 * d] * inv, f[4 * d + 1] * inv, f[4 * d + 2] * inv, f[4 * d + 3] * inv);
+                float top = fmaxf(finite_top(v.h[0]), finite_top(v.h[1]));
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                sx = scale_value(scale_byte(top));
+                v.h[0].pack(sx, w8);
+                v.h[1].pack(sx, w8 + 4);
             }
-            const float s = scale_value(sx);
+#pragma unroll
             for (int p = 0; p < 4; p++) {
-                bf16x8 xb;
-                unpack4(w8[2 * p], s, (__bf16 *)&xb);
-                unpack4(w8[2 * p + 1], s, (__bf16 *)&xb + 4);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], xb, acc[t], 0, 0, 0);
+                bf16x8 b;
+                unpack4(w8[2 * p], sx, (__bf16 *)&b);
+                unpack4(w8[2 * p + 1], sx, (__bf16 *)&b + 4);
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], b, acc[t], 0, 0, 0);
             }
+        }
+    };
+    const int first = block_ptr[brow] + wave, last = block_ptr[brow + 1];
+    if (first < last) {
+        Stage now = load(first);
+        for (int b = first; b < last; b += W) {
+            const Stage next = load(b + W < last ? b + W : b);
+            use(now);
+            now = next;
         }
     }
+#pragma unroll
     for (int t = 0; t < NT; t++) part[wave][t][lane] = acc[t];
     __syncthreads();
-    for (int id = threadIdx.x; id < NT * kWave; id += kBlock) {
+    for (int id = threadIdx.x; id < NT * kWave; id += W * kWave) {
         const int t = id / kWave, l = id & (kWave - 1), v = t * 16 + (l & 15);
         f32x4 s = part[0][t][l];
-        for (int w = 1; w < kWaves; w++) s += part[w][t][l];
+#pragma unroll
+        for (int w = 1; w < W; w++) s += part[w][t][l];
         const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + 4 * (strip & 3);
         if (v >= n) continue;
         for (int k = 0; k < 4; k++) {
@@ -286,13 +443,6 @@ __device__ __forceinline__ void tile_of_block(unsigned bid, int majors, int vtil
     const unsigned wide = (unsigned)majors - group * 8 < 8 ? (unsigned)majors - group * 8 : 8;
     *major = (int)(group * 8 + in % wide);
     *vtile = (int)(in / wide);
-}
-
-__device__ __forceinline__ u32x4 load16(const void *p)       // any alignment
-{
-    u32x4 w;
-    __builtin_memcpy(&w, p, 16);
-    return w;
 }
 
 // results m .. m + 4 COUNT - 1 of one vector, as many as there are below `limit`
@@ -445,33 +595,22 @@ template <typename DT> struct parts_of { static constexpr int value = 1; };
 template <> struct parts_of<_Float16> { static constexpr int value = 2; };
 template <> struct parts_of<float> { static constexpr int value = 3; };
 
-// 8 entries of dy as they lie in memory, zero from `left` on
-template <typename DT> struct Raw8 {
-    DT v[8];
-    __device__ __forceinline__ void load(const DT *p, int left)
-    {
-        if (left >= 8) __builtin_memcpy(v, p, sizeof v);
-        else
+template <typename DT> __device__ __forceinline__ void split8(const Raw<DT, 8> &r, bf16x8 *part)
+{
+    if constexpr (std::is_same<DT, __bf16>::value) {
+        __builtin_memcpy(part, r.v, 16);
+    } else {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = k < left ? p[k] : (DT)0.0f;
-    }
-    __device__ __forceinline__ void split(bf16x8 *part) const
-    {
-        if constexpr (std::is_same<DT, __bf16>::value) {
-            __builtin_memcpy(part, v, 16);
-        } else {
+        for (int k = 0; k < 8; k++) {
+            float f = (float)r.v[k];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                float f = (float)v[k];
-#pragma unroll
-                for (int p = 0; p < parts_of<DT>::value; p++) {
-                    part[p][k] = (__bf16)f;
-                    f -= (float)part[p][k];
-                }
+            for (int p = 0; p < parts_of<DT>::value; p++) {
+                part[p][k] = (__bf16)f;
+                f -= (float)part[p][k];
             }
         }
     }
-};
+}
 
 struct TransposedArgs {
     int n, rows, columns, bcols, vtiles;
@@ -501,7 +640,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 #pragma unroll
         for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    Raw8<DT> yr[PIECES];
+    Raw<DT, 8> yr[PIECES];
     u32x4 ar[2];
     auto fetch = [&](int step) {
         const uint8_t *block = g.val8 + (int64_t)g.id[step >> 1] * kBlockBytes + (step & 1) * (kBlockBytes / 2) + tid * 16;
@@ -521,7 +660,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         for (int j = 0; j < PIECES; j++) {
             const int t = j * 32 + (tid >> 3);
             bf16x8 part[PARTS];
-            yr[j].split(part);
+            split8(yr[j], part);
 #pragma unroll
             for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][t * 64 + (((tid & 7) ^ ((t >> 1) & 7)) << 3)] = part[p];
         }
@@ -604,7 +743,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
 #pragma unroll
         for (int s = 0; s < NM; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    Raw8<DT> yr[2];
+    Raw<DT, 8> yr[2];
     u32x4 xr[NB];
     int sx[NB];
     auto fetch = [&](int t0) {
@@ -625,7 +764,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             bf16x8 part[PARTS];
-            yr[j].split(part);
+            split8(yr[j], part);
 #pragma unroll
             for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][(j * 16 + (tid >> 4)) * YP + (tid & 15) * 8] = part[p];
         }
@@ -703,16 +842,22 @@ static int groups_of(int length) { return length / kB + (length % kB != 0); }
 static int launch_few(const spmv_hip_matrix *m, int n, const void *x, int x_dtype, int64_t ldx, const uint8_t *xscale,
                       int64_t lds, void *y, int y_dtype, int64_t ldy, hipStream_t st)
 {
-    const dim3 grid(m->brows * 8), block(kBlock);
+    // 16 waves a strip where every one of them gets a block, else 4
+    const bool many_waves = m->nblocks >= 16 * (int64_t)m->brows;
     auto go = [&](auto t) {
         typedef decltype(t) XT;
-        auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, grid, block, 0, st, n, m->rows, m->columns, m->d_block_ptr, m->d_block_col, m->d_val8,
-                               m->d_scale8, (const XT *)x, ldx, xscale, lds, y, y_dtype, ldy);
+        auto launch = [&](auto kernel, int waves) {
+            hipLaunchKernelGGL(kernel, dim3(m->brows * 8), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
+                               m->d_block_col, m->d_val8, m->d_scale8, (const XT *)x, ldx, xscale, lds, y, y_dtype, ldy);
         };
-        if (n <= 16) launch(few_vectors_kernel<XT, 1>);
-        else if (n <= 32) launch(few_vectors_kernel<XT, 2>);
-        else launch(few_vectors_kernel<XT, 4>);
+        auto tiles = [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            if (n <= 16) launch(few_vectors_kernel<XT, 1, W>, W);
+            else if (n <= 32) launch(few_vectors_kernel<XT, 2, W>, W);
+            else launch(few_vectors_kernel<XT, 4, W>, W);
+        };
+        if (many_waves) tiles(std::integral_constant<int, 16>());
+        else tiles(std::integral_constant<int, 4>());
     };
     if (x_dtype == SPMV_HIP_E4M3) go(uint8_t());
     else with_elem(x_dtype, go);
@@ -765,12 +910,12 @@ static int check_block8(const char *what, const spmv_hip_matrix *m)
     if (m->format != SPMV_HIP_BLOCK8) { set_error("%s needs a handle of 8-bit blocks (format %d)", what, m->format); return 1; }
     return 0;
 }
-// groups of 16 lanes in workgroups of 256: at most 2^31 - 1 workgroups
-static int check_groups(const char *what, int64_t ngroups)
+// launch shape of quantize8 / restore8; R vectors a wave
+static bool many_groups(int n, int groups) { return (int64_t)(n / 64) * ((groups + kQuantGroups - 1) / kQuantGroups) >= 2048; }
+static dim3 group_grid(int n, int groups, int r)
 {
-    if (ngroups <= (int64_t)0x7fffffff * (kBlock / 16)) return 0;
-    set_error("%s: %lld groups of 128 are more than one launch takes", what, (long long)ngroups);
-    return 1;
+    const int64_t per = (int64_t)kQuantWaves * r;
+    return dim3((unsigned)((n + per - 1) / per), (groups + kQuantGroups - 1) / kQuantGroups);
 }
 
 // Vectors a workgroup takes: `most` where that still gives every CU a tile, else half, down to 64
@@ -906,13 +1051,14 @@ int spmv_hip_quantize8_dev(int n, int columns, const void *d_x, int dtype, int64
     if (columns < 0) { set_error("quantize8: negative length %d", columns); return 1; }
     if (check_vectors("quantize8", n, d_x, ldx, columns) || check_eight("quantize8", n, columns, d_x8, ldx8, d_scale, lds)) return 1;
     const int groups = groups_of(columns);
-    const int64_t ngroups = (int64_t)n * groups;
-    if (ngroups == 0) return 0;
-    if (check_groups("quantize8", ngroups)) return 1;
+    if (n == 0 || groups == 0) return 0;
     with_elem(dtype, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((quantize8_kernel<T>), dim3((unsigned)((ngroups + 15) / 16)), dim3(kBlock), 0, (hipStream_t)stream,
-                           ngroups, groups, columns, (const T *)d_x, ldx, d_x8, ldx8, d_scale, lds);
+        auto go = [&](auto kernel, int r) {
+            hipLaunchKernelGGL(kernel, group_grid(n, groups, r), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, (const T *)d_x, ldx, d_x8, ldx8, d_scale, lds);
+        };
+        if (many_groups(n, groups)) go(quantize8_kernel<T, 16>, 16);
+        else go(quantize8_kernel<T, 1>, 1);
     });
     return launched("quantize8");
 }
@@ -924,13 +1070,14 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
     if (columns < 0) { set_error("restore8: negative length %d", columns); return 1; }
     if (check_vectors("restore8", n, d_x, ldx, columns) || check_eight("restore8", n, columns, d_x8, ldx8, d_scale, lds)) return 1;
     const int groups = groups_of(columns);
-    const int64_t ngroups = (int64_t)n * groups;
-    if (ngroups == 0) return 0;
-    if (check_groups("restore8", ngroups)) return 1;
+    if (n == 0 || groups == 0) return 0;
     with_elem(dtype, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((restore8_kernel<T>), dim3((unsigned)((ngroups + 15) / 16)), dim3(kBlock), 0, (hipStream_t)stream,
-                           ngroups, groups, columns, d_x8, ldx8, d_scale, lds, (T *)d_x, ldx);
+        auto go = [&](auto kernel, int r) {
+            hipLaunchKernelGGL(kernel, group_grid(n, groups, r), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, d_x8, ldx8, d_scale, lds, (T *)d_x, ldx);
+        };
+        if (many_groups(n, groups)) go(restore8_kernel<T, 16>, 16);
+        else go(restore8_kernel<T, 1>, 1);
     });
     return launched("restore8");
 }
