@@ -308,6 +308,13 @@ __global__ __launch_bounds__(kBlock) void store8_kernel(const uint8_t *__restric
     if (threadIdx.x == 0) scale[k] = (uint8_t)scale8[k];
 }
 
+// p[k] for a wave-uniform k, of a table no kernel writes while it runs: a scalar load.  Left to the compiler it becomes a
+// vector load behind the memory barriers, and waiting for it waits for every load of the stage before.
+__device__ __forceinline__ int table(const int *p, int k)
+{
+    return ((const __attribute__((address_space(4))) int *)p)[__builtin_amdgcn_readfirstlane(k)];
+}
+
 // ---- few vectors ----------------------------------------------------------------------------------------------
 
 // One workgroup per strip of 16 rows; its W waves take the strip's blocks in turn and add their results in LDS.
@@ -325,7 +332,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
     constexpr bool kEight = std::is_same<XT, uint8_t>::value;
     __shared__ f32x4 part[W][NT][kWave];
     const int brow = blockIdx.x >> 3, strip = blockIdx.x & 7;
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, i = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), i = lane & 15, q = lane >> 4;
     f32x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
 #pragma unroll
     for (int t = 0; t < NT; t++) vec[t] = min(t * 16 + i, n - 1);
 
-    constexpr int AHEAD = NT == 1;                           // x ahead too; with more tiles registers run out
+    constexpr bool AHEAD = NT * sizeof(XT) <= 4;             // x ahead too, in up to 32 registers
     struct Vector {
         Raw<XT, 16> h[2];
         int scale;
@@ -342,7 +349,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
     struct Stage {
         u32x4 a[2];
         int scale, group;
-        Vector x;
+        Vector x[AHEAD ? NT : 1];
     };
     auto load_x = [&](int t, int group) {
         Vector r;
@@ -363,9 +370,11 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         const uint8_t *block = val8 + (int64_t)b * kBlockBytes + (strip * 2 * kWave + lane) * 16;
         s.a[0] = *(const u32x4 *)block;
         s.a[1] = *(const u32x4 *)(block + kWave * 16);
-        s.scale = scale8[b];
-        s.group = block_col[b];
-        if (AHEAD) s.x = load_x(0, s.group);
+        s.scale = table(scale8, b);
+        s.group = table(block_col, b);
+        if constexpr (AHEAD)
+#pragma unroll
+            for (int t = 0; t < NT; t++) s.x[t] = load_x(t, s.group);
         return s;
     };
     auto use = [&](const Stage &s) {
@@ -375,7 +384,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         for (int d = 0; d < 8; d++) unpack4(s.a[d >> 2][d & 3], sa, (__bf16 *)&a[d >> 1] + 4 * (d & 1));
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const Vector v = AHEAD ? s.x : load_x(t, s.group);
+            const Vector v = AHEAD ? s.x[AHEAD ? t : 0] : load_x(t, s.group);
             unsigned w8[8];
             float sx;
             if constexpr (kEight) {
@@ -398,7 +407,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
             }
         }
     };
-    const int first = block_ptr[brow] + wave, last = block_ptr[brow + 1];
+    const int first = table(block_ptr, brow) + wave, last = table(block_ptr, brow + 1);
     if (first < last) {
         Stage now = load(first);
         for (int b = first; b < last; b += W) {
@@ -429,10 +438,51 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
 
 // ---- many vectors ---------------------------------------------------------------------------------------------
 
-// Three products on 128-row tiles, 4 waves, operands staged through registers into two LDS buffers: while the matrix
-// instructions run on one, the loads for the other are in flight; one barrier a step.  Two workgroups share a CU, so one
-// computes where the other waits.  Registers rather than direct loads to LDS, because the staging masks edges, takes any
-// alignment and converts.
+// One workgroup: 128 rows (or columns, of one block row or column) x 32 NU vectors; a wave has half the rows and half the
+// vectors, 64 x 16 NU.  What comes from LDS is read as 16 bytes a lane where the layout allows: such a read takes the LDS 7
+// cycles a wave, an 8-byte read as long, a 16-byte write from registers 13.  R stages are in flight or in use; a stage's
+// loads are issued R - 1 steps ahead: one step where two workgroups of 256 vectors share a CU and cover each other's waits,
+// three where there are few workgroups and a step is short.
+
+template <int V> using ic = std::integral_constant<int, V>;
+
+// Wait until at most N of the wave's loads are outstanding and its LDS reads are done, then meet the others.  What the
+// compiler does not see, it does not move: the asm statements order the memory accesses around them.
+template <int N> __device__ __forceinline__ void stage_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b)
+{
+    return (i32x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 64 lanes x 16 bytes into LDS, lane l to lds + 16 l (lds is the wave's), from a 32-bit offset a lane into the `records`
+// bytes at base, zeros from past them.
+__device__ __forceinline__ void load_to_lds(const void *base, unsigned records, unsigned offset, uint8_t *lds)
+{
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)records, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, (int)offset, 0, 0, 0);
+}
+
+// step(slot, k) for k = first .. last - 1, slot = (k - first) % R as a constant: whole rounds, then what is left (exits
+// from inside a round would cost the accumulators copies)
+template <int R, typename F> __device__ __forceinline__ void ring(int first, int last, F step)
+{
+    int k = first;
+    for (; k + R <= last; k += R) {
+        step(ic<0>(), k);
+        step(ic<1>(), k + 1);
+        if constexpr (R > 2) step(ic<2>(), k + 2);
+        if constexpr (R > 3) step(ic<3>(), k + 3);
+    }
+    if (k < last) step(ic<0>(), k);
+    if constexpr (R > 2) if (k + 1 < last) step(ic<1>(), k + 1);
+    if constexpr (R > 3) if (k + 2 < last) step(ic<2>(), k + 2);
+}
 
 // logical tile of a workgroup: every XCD walks its own eighth of the tiles, in it 8 block rows (columns) side by side
 // and then the next vectors, so that the blocks and the vectors of the workgroups that run together stay in its L2
@@ -467,126 +517,113 @@ struct ProductArgs {
     int64_t ldx8, lds, ldy;
 };
 
-// y = A x.  Tile: one block row x TOK vectors; a wave has 64 rows x TOK / 2 vectors.  The blocks go straight from memory
-// to registers (their layout is the operand's), the vectors through LDS: rows of 128 bytes, their 16-byte pieces
-// exchanged by XOR so that the 8 lanes of a read cycle meet 8 different pieces.  Vector NU i + u belongs to lane i of
-// tile u: a lane's scale bytes are then neighbours.
+// y = A x, a block a step.  The vectors go to LDS by direct loads, rows of 128 bytes, their 16-byte pieces exchanged by
+// XOR so that the 8 lanes of a read cycle meet 8 different pieces; the blocks, whose layout is the operand's, go straight
+// to the registers of the two waves that need each half.  Vector NU i + u belongs to lane i of tile u: a lane's scale
+// bytes are neighbours.
 // EXACT: operands widened to bf16 in registers (exact), 32-bit sums.  Otherwise the 8-bit matrix instruction, which applies
-// both scales and runs at twice the rate, but whose sums of 128 products are good to about 16 bits: only for bf16 results.
-template <bool EXACT, int TOK, typename OT>
+// both scales and runs at twice the rate, but aligns 8 products at a time and drops what lies 13 bits below the largest:
+// good to about 16 bits, for bf16 results only.
+template <bool EXACT, int NU, typename OT>
 __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *__restrict__ y)
 {
-    constexpr int NU = TOK / 32, PIECES = TOK / 32;
-    __shared__ uint8_t X[2][TOK * kB];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
+    constexpr int R = NU == 8 ? 2 : NU == 4 ? 3 : 4, TOK = 32 * NU;
+    __shared__ uint8_t X[R][TOK * kB];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), i = lane & 15, q = lane >> 4;
     const int wm = wave & 1, wn = wave >> 1;
     int major, vtile;
     tile_of_block(blockIdx.x, g.brows, g.vtiles, &major, &vtile);
-    const int v0 = vtile * TOK, first = g.ptr[major], last = g.ptr[major + 1];
+    const int t0 = vtile * TOK, v0 = t0 + wn * 16 * NU + NU * i;             // the tile's and the lane's first vector
+    const int first = table(g.ptr, major), last = table(g.ptr, major + 1);
     f32x4 acc[NU][4];
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
         for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    u32x4 xr[PIECES];
-    unsigned at[PIECES];                                     // past the last vector: any, it is not stored
+    // piece j of a thread: 16 bytes of vector 32 j + t.  The 16-byte pieces of vector v are exchanged by v / NU, which
+    // for 256 vectors differs between even and odd j.  Past the last vector zeros.
+    const int t = wave * 8 + (lane >> 3);
+    const unsigned at = (unsigned)t * (unsigned)g.ldx8 + (((lane & 7) ^ ((t / NU) & 7)) << 4), flip = NU == 8 ? 64 : 0;
+    const uint8_t *xbase = g.x8 + (int64_t)t0 * g.ldx8;
+    const unsigned ldx8 = (unsigned)g.ldx8, records = (unsigned)min(g.n - t0, TOK) * ldx8;
+    const int back = max(v0 + NU - g.n, 0);                  // n > NU, so the load of scale bytes can move back from the end
+
+    i32x8 a[R][4];
+    uint64_t sx[R];
+    int sa[R], c = 0, scale = 0;                             // c, scale: of the block issued next, loaded a step before
+    auto look_up = [&](int b) { c = table(g.col, b); scale = table(g.scale8, b); };
+    auto issue = [&](auto slot, int b) {
+        constexpr int S = decltype(slot)::value;
 #pragma unroll
-    for (int j = 0; j < PIECES; j++) at[j] = (unsigned)min(j * 32 + (tid >> 3), g.n - 1 - v0) * (unsigned)g.ldx8 + (tid & 7) * 16;
-    auto fetch = [&](int b) {
-        const uint8_t *base = g.x8 + (int64_t)v0 * g.ldx8 + g.col[b] * kB;
-#pragma unroll
-        for (int j = 0; j < PIECES; j++) xr[j] = *(const u32x4 *)(base + at[j]);
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int j = 0; j < PIECES; j++) {
-            const int t = j * 32 + (tid >> 3);
-            *(u32x4 *)&X[buf][t * kB + (((tid & 7) ^ ((t / NU) & 7)) << 4)] = xr[j];
+        for (int j = 0; j < NU; j++) {
+            const unsigned skip = min((unsigned)j * 32 * ldx8 + c * kB, records);
+            load_to_lds(xbase + skip, records - skip, j & 1 ? at ^ flip : at, &X[S][(j * 32 + wave * 8) * kB]);
         }
+        const uint8_t *half = g.val8 + (int64_t)b * kBlockBytes + wm * (kBlockBytes / 2);
+#pragma unroll
+        for (int s = 0; s < 4; s++) a[S][s] = join(*(const u32x4 *)(half + (lane * 16u + s * 2048)), *(const u32x4 *)(half + (lane * 16u + s * 2048 + 1024)));
+        sa[S] = scale;
+        sx[S] = 0;
+        __builtin_memcpy(&sx[S], g.xscale + (int64_t)c * g.lds + (v0 - back), NU);
+        look_up(min(b + 1, last - 1));
     };
-    if (first < last) { fetch(first); put(0); }
-    __syncthreads();
-    for (int b = first; b < last; b++) {
-        const int buf = (b - first) & 1;
-        u32x4 a[4][2];
-        const uint8_t *block = g.val8 + (int64_t)b * kBlockBytes + (wm * 8 * kWave + lane) * 16;
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) a[s][h] = *(const u32x4 *)(block + (s * 2 + h) * kWave * 16);
-        const int sa = g.scale8[b];
-        // scale bytes of vectors v, v + 1, .. v + NU - 1; n > NU, so the load can move back from the end of the scales
-        const int v = v0 + wn * 16 * NU + NU * i, back = max(v + NU - g.n, 0);
-        uint64_t sx = 0;
-        __builtin_memcpy(&sx, g.xscale + (int64_t)g.col[b] * g.lds + (v - back), NU);
-        sx >>= 8 * min(back, 7);
-        auto scale_of = [&](int u) { return (unsigned)(sx >> (8 * u)); };    // in the low byte
-        fetch(min(b + 1, last - 1));                         // unconditional, like put below: one basic block, so that
-                                                             // nothing is moved across the loads and the barrier
+    auto step = [&](auto slot, int b) {
+        constexpr int S = decltype(slot)::value;
+        stage_barrier<(R - 2) * (NU + 8)>();
+        issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
+        const uint64_t bytes = sx[S] >> (8 * min(back, 7));
+        auto operand = [&](int u) {
+            const uint8_t *row = &X[S][(wn * 16 * NU + NU * i + u) * kB];
+            return join(*(const u32x4 *)(row + ((q ^ (i & 7)) << 4)), *(const u32x4 *)(row + (((q + 4) ^ (i & 7)) << 4)));
+        };
+        bf16x8 aw[4][EXACT ? 4 : 1];
         if constexpr (EXACT) {
-            const float fa = scale_value(sa);
-            bf16x8 aw[4][4];
+            const float fa = scale_value(sa[S]);
 #pragma unroll
             for (int s = 0; s < 4; s++)
 #pragma unroll
-                for (int d = 0; d < 8; d++) unpack4(a[s][d >> 2][d & 3], fa, (__bf16 *)&aw[s][d >> 1] + 4 * (d & 1));
+                for (int d = 0; d < 8; d++) unpack4((unsigned)a[S][s][d], fa, (__bf16 *)&aw[s][d >> 1] + 4 * (d & 1));
+        }
+        i32x8 w = operand(0);
 #pragma unroll
-            for (int u = 0; u < NU; u++) {
-                const int t = wn * 16 * NU + NU * i + u;
-                const float fx = scale_value(scale_of(u) & 255);
-                u32x4 x[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) x[h] = *(const u32x4 *)&X[buf][t * kB + (((h * 4 + q) ^ (i & 7)) << 4)];
+        for (int u = 0; u < NU; u++) {
+            // one tile ahead and no more: left alone, the compiler reads all of them first and runs out of registers
+            i32x8 ahead = w;
+            if (u + 1 < NU) ahead = operand(u + 1);
+            const int su = (int)(bytes >> (8 * u)) & 255;
+            if constexpr (EXACT) {
+                const float fx = scale_value(su);
 #pragma unroll
                 for (int p = 0; p < 4; p++) {
                     bf16x8 xw;
-                    unpack4(x[p >> 1][2 * (p & 1)], fx, (__bf16 *)&xw);
-                    unpack4(x[p >> 1][2 * (p & 1) + 1], fx, (__bf16 *)&xw + 4);
+                    unpack4((unsigned)w[2 * p], fx, (__bf16 *)&xw);
+                    unpack4((unsigned)w[2 * p + 1], fx, (__bf16 *)&xw + 4);
 #pragma unroll
                     for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw[s][p], xw, acc[u][s], 0, 0, 0);
                 }
+            } else {
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[S][s], w, acc[u][s], 0, 0, 0, sa[S], 0, su);
             }
-        } else {
-            auto read = [&](int u) {
-                const int t = wn * 16 * NU + NU * i + u;
-                i32x8 x;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const u32x4 w = *(const u32x4 *)&X[buf][t * kB + (((h * 4 + q) ^ (i & 7)) << 4)];
-#pragma unroll
-                    for (int d = 0; d < 4; d++) x[4 * h + d] = (int)w[d];
-                }
-                return x;
-            };
-            i32x8 x = read(0);
-#pragma unroll
-            for (int u = 0; u < NU; u++) {
-                // one tile's operand ahead and no more: left alone, the compiler reads all of them first and spills
-                i32x8 ahead = x;
-                if (u + 1 < NU) ahead = read(u + 1);
-                const int su = (int)scale_of(u);                             // the instruction reads the low byte
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    i32x8 aw;
-#pragma unroll
-                    for (int d = 0; d < 8; d++) aw[d] = (int)a[s][d >> 2][d & 3];
-                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aw, x, acc[u][s], 0, 0, 0, sa, 0, su);
-                }
-                x = ahead;
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            w = ahead;
+            __builtin_amdgcn_sched_barrier(0);
         }
-        put(buf ^ 1);
-        __syncthreads();
+    };
+    if (first < last) {
+        look_up(first);
+        issue(ic<0>(), first);
+        if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
+        if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
+        ring<R>(first, last, step);
     }
+    stage_barrier<0>();                                      // no load to LDS outlives the workgroup
     // a lane has rows 16 q .. 16 q + 15 of its wave's 64 for NU vectors
-    const int r0 = major * kB + wm * 64 + 16 * q;
+    const int r = major * kB + wm * 64 + 16 * q;
 #pragma unroll
-    for (int u = 0; u < NU; u++) {
-        const int v = v0 + wn * 16 * NU + NU * i + u;
-        if (v < g.n && r0 < g.rows) store_row<OT, 4>(y + (int64_t)v * g.ldy + r0, g.rows - r0, acc[u]);
-    }
+    for (int u = 0; u < NU; u++)
+        if (v0 + u < g.n && r < g.rows) store_row<OT, 4>(y + (int64_t)(v0 + u) * g.ldy + r, g.rows - r, acc[u]);
 }
 
 // dy is used as it is: split into PARTS bf16 numbers that add up to it exactly (1 for bf16, 2 for fp16, 3 for fp32:
@@ -595,20 +632,12 @@ template <typename DT> struct parts_of { static constexpr int value = 1; };
 template <> struct parts_of<_Float16> { static constexpr int value = 2; };
 template <> struct parts_of<float> { static constexpr int value = 3; };
 
-template <typename DT> __device__ __forceinline__ void split8(const Raw<DT, 8> &r, bf16x8 *part)
+template <int PARTS> __device__ __forceinline__ void split1(float f, __bf16 *part, int stride)
 {
-    if constexpr (std::is_same<DT, __bf16>::value) {
-        __builtin_memcpy(part, r.v, 16);
-    } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            float f = (float)r.v[k];
-#pragma unroll
-            for (int p = 0; p < parts_of<DT>::value; p++) {
-                part[p][k] = (__bf16)f;
-                f -= (float)part[p][k];
-            }
-        }
+    for (int p = 0; p < PARTS; p++) {
+        part[p * stride] = (__bf16)f;
+        f -= (float)part[p * stride];
     }
 }
 
@@ -619,87 +648,159 @@ struct TransposedArgs {
     int64_t lddy, lddx;
 };
 
-// dx = A^T dy.  Tile: one block column x TOK vectors, steps of half a block (64 rows); a wave has 64 columns x TOK / 2
-// vectors.  The block's bytes lie in LDS as in memory; ds_read_b64_tr_b8 hands every lane one column of 8 rows, widened
-// to bf16 (exact) on the way to the matrix instruction.  Those 8 rows are 4 s .. 4 s + 3 and 16 + 4 s .. of a
-// quarter (block8_offset), so dy is read in two 8-byte halves; its 16-byte pieces are exchanged by XOR in LDS.
-template <typename DT, int TOK, typename OT>
+// 8 entries of dy as PARTS operands
+template <typename DT> __device__ __forceinline__ void operands8(const Raw<DT, 8> &r, bf16x8 *part)
+{
+    if constexpr (parts_of<DT>::value == 1) __builtin_memcpy(part, r.v, 16);
+    else
+#pragma unroll
+        for (int e = 0; e < 8; e++) split1<parts_of<DT>::value>((float)r.v[e], (__bf16 *)part + e, 8);
+}
+
+// dx = A^T dy, half a block (64 rows) a step, blocks and vectors through LDS.  ds_read_b64_tr_b8 hands every lane one
+// column of 8 rows of the block, widened to bf16 (exact) on the way to the matrix instruction.  8 rows of dy are 4 rows in
+// each of two strips of the block (block8_offset); in LDS the 4-row pieces of a 16 x 16 subtile are exchanged by XOR
+// with the strip, which puts the two on different banks.  DIRECT (bf16, rows of dy 16-byte aligned): dy goes to LDS by
+// direct loads, otherwise through registers, which take any alignment and split it.  The blocks of a last block row that is
+// not whole come last in every list: they are taken after the others, one by one, with the entries past the end masked.
+template <typename DT, bool DIRECT, int NU, typename OT>
 __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g, const DT *__restrict__ dy, OT *__restrict__ dx)
 {
-    constexpr int PARTS = parts_of<DT>::value, NU = TOK / 32, PIECES = TOK / 32;
-    __shared__ __bf16 Y[2][PARTS][TOK * 64];
-    __shared__ uint8_t A[2][kBlockBytes / 2];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
+    constexpr int PARTS = parts_of<DT>::value, R = !DIRECT || NU == 8 ? 2 : NU == 4 ? 3 : 4, TOK = 32 * NU;
+    __shared__ uint8_t Y[R][PARTS][TOK * 128];
+    __shared__ uint8_t A[R][kBlockBytes / 2];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), i = lane & 15, q = lane >> 4;
     const int wm = wave & 1, wn = wave >> 1;
     int major, vtile;
     tile_of_block(blockIdx.x, g.bcols, g.vtiles, &major, &vtile);
-    const int v0 = vtile * TOK, first = 2 * g.ptr[major], last = 2 * g.ptr[major + 1];
+    const int t0 = vtile * TOK;
+    const int begin = table(g.ptr, major), end = table(g.ptr, major + 1);
+    int whole = end;
+    if (g.rows % kB)
+        while (whole > begin && table(g.row, whole - 1) == g.rows / kB) whole--;
+    const int first = 2 * begin, last = 2 * whole;
     f32x4 acc[NU][4];
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
         for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    Raw<DT, 8> yr[PIECES];
-    u32x4 ar[2];
-    auto fetch = [&](int step) {
-        const uint8_t *block = g.val8 + (int64_t)g.id[step >> 1] * kBlockBytes + (step & 1) * (kBlockBytes / 2) + tid * 16;
-        ar[0] = *(const u32x4 *)block;
-        ar[1] = *(const u32x4 *)(block + kBlock * 16);
-        const int r = g.row[step >> 1] * kB + (step & 1) * 64 + (tid & 7) * 8;
+    // piece j of a thread: 8 entries of vector 32 j + 8 wave + lane / 8, in place lane % 8 of its row in LDS; a
+    // row's pieces are exchanged by XOR.  Past the last vector: the last, its result is not stored.
+    const DT *ybase = dy + (int64_t)t0 * g.lddy;
+    const int row_of_lane = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((row_of_lane >> 1) & 7);
+    const unsigned lddy = (unsigned)g.lddy, near = row_of_lane * lddy + 8 * piece;
+    const unsigned records = (unsigned)min(g.n - t0, TOK) * lddy * 2;        // bytes, DIRECT
+    unsigned at[DIRECT ? 1 : NU];
+    if constexpr (!DIRECT)
 #pragma unroll
-        for (int j = 0; j < PIECES; j++) {
-            const int v = min(v0 + j * 32 + (tid >> 3), g.n - 1);
-            yr[j].load(dy + (int64_t)v * g.lddy + r, g.rows - r);
-        }
+        for (int j = 0; j < NU; j++) at[j] = (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * lddy + 8 * piece;
+
+    Raw<DT, 8> yr[DIRECT ? 1 : NU];
+    int sa[R], id = 0, row = 0;                              // id, row: of the half block issued next, loaded a step before
+    auto look_up = [&](int k) {
+        id = table(g.id, k >> 1);
+        row = table(g.row, k >> 1);
     };
-    auto put = [&](int buf) {
-        *(u32x4 *)&A[buf][tid * 16] = ar[0];
-        *(u32x4 *)&A[buf][(kBlock + tid) * 16] = ar[1];
-#pragma unroll
-        for (int j = 0; j < PIECES; j++) {
-            const int t = j * 32 + (tid >> 3);
-            bf16x8 part[PARTS];
-            split8(yr[j], part);
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][t * 64 + (((tid & 7) ^ ((t >> 1) & 7)) << 3)] = part[p];
-        }
+    auto issue_block = [&](auto slot, int k) {
+        constexpr int S = decltype(slot)::value;
+        const uint8_t *half = g.val8 + (int64_t)id * kBlockBytes + (k & 1) * (kBlockBytes / 2);
+        sa[S] = table(g.scale8, id);
+        // wave w brings strip w: 2 x 4 subtiles of 256 bytes
+        const int from = wave * 2048 + q * 256 + ((i ^ (wave << 2)) << 4);
+        load_to_lds(half, kBlockBytes / 2, from, &A[S][wave * 2048]);
+        load_to_lds(half, kBlockBytes / 2, from + 1024, &A[S][wave * 2048 + 1024]);
     };
-    if (first < last) { fetch(first); put(0); }
-    __syncthreads();
-    for (int step = first; step < last; step++) {
-        const int buf = step & 1;                            // first is even
-        const float sa = scale_value(g.scale8[g.id[step >> 1]]);
-        fetch(min(step + 1, last - 1));
+    auto issue = [&](auto slot, int k) {
+        constexpr int S = decltype(slot)::value;
+        issue_block(slot, k);
+        const unsigned r = row * kB + (k & 1) * 64;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int strip = 2 * k + (q >> 1);
+        for (int j = 0; j < NU; j++)
+            if constexpr (DIRECT) {
+                const unsigned skip = min((j * 32 * lddy + r) * 2, records);
+                load_to_lds((const uint8_t *)ybase + skip, records - skip, near * 2, &Y[S][0][(j * 32 + wave * 8) * 128]);
+            } else {
+                __builtin_memcpy(yr[j].v, ybase + r + at[j], sizeof yr[j].v);
+            }
+        look_up(min(k + 1, last - 1));
+    };
+    auto put = [&](int slot, const Raw<DT, 8> &r, int j) {
+        bf16x8 part[PARTS];
+        operands8(r, part);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[slot][p][(j * 32 + wave * 8) * 128 + lane * 16] = part[p];
+    };
+    auto compute = [&](auto slot) {
+        constexpr int S = decltype(slot)::value;
+        const float fa = scale_value(sa[S]);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            // row 32 h + 8 q + w, w = i >> 1, columns 8 (i & 1) .. + 7 of a subtile
+            const int strip = (2 * q + (i >> 3)) & 3, quad = 2 * h + (q >> 1);
+            const uint8_t *p = &A[S][strip * 2048 + wm * 1024 + ((quad ^ strip) << 6) + ((i >> 1) & 3) * 16 + (i & 1) * 8];
             bf16x8 a[4];
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (__attribute__((address_space(3))) i32x2 *)&A[buf][(strip * 8 + wm * 4 + s) * 256 + (q & 1) * 128 + i * 8]);
-                unpack4((unsigned)w[0], sa, (__bf16 *)&a[s]);
-                unpack4((unsigned)w[1], sa, (__bf16 *)&a[s] + 4);
+                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2 *)(p + s * 256));
+                unpack4((unsigned)w[0], fa, (__bf16 *)&a[s]);
+                unpack4((unsigned)w[1], fa, (__bf16 *)&a[s] + 4);
             }
+            auto operand = [&](int part, int u) {
+                const int t = wn * 16 * NU + 16 * u + i;
+                return *(const bf16x8 *)&Y[S][part][t * 128 + (((4 * h + q) ^ ((t >> 1) & 7)) << 4)];
+            };
 #pragma unroll
-            for (int p = 0; p < PARTS; p++)
+            for (int part = 0; part < PARTS; part++) {
+                bf16x8 b = operand(part, 0);
 #pragma unroll
                 for (int u = 0; u < NU; u++) {
-                    const int t = wn * 16 * NU + 16 * u + i, f = (t >> 1) & 7, c = 4 * (q & 1) + k, o = t * 64 + 4 * (q >> 1);
-                    bf16x8 b;
-                    __builtin_memcpy(&b, &Y[buf][p][o + ((c ^ f) << 3)], 8);
-                    __builtin_memcpy((__bf16 *)&b + 4, &Y[buf][p][o + (((c + 2) ^ f) << 3)], 8);
+                    bf16x8 ahead = b;                        // one tile ahead and no more
+                    if (u + 1 < NU) ahead = operand(part, u + 1);
 #pragma unroll
                     for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
+                    b = ahead;
+                    if (u & 1) __builtin_amdgcn_sched_barrier(0);
                 }
+            }
         }
-        put(buf ^ 1);
-        __syncthreads();
+    };
+    auto step = [&](auto slot, int k) {
+        constexpr int S = decltype(slot)::value;
+        stage_barrier<DIRECT ? (R - 2) * (2 + NU) : 0>();
+        issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1));
+        compute(slot);
+        if constexpr (!DIRECT)
+#pragma unroll
+            for (int j = 0; j < NU; j++) put((S + 1) % R, yr[j], j);
+    };
+    if (first < last) {
+        look_up(first);
+        issue(ic<0>(), first);
+        if constexpr (!DIRECT)
+#pragma unroll
+            for (int j = 0; j < NU; j++) put(0, yr[j], j);
+        if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
+        if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
+        ring<R>(first, last, step);
+    }
+    stage_barrier<0>();                                      // no load to LDS outlives the workgroup, or meets the next
+    for (int k = last; k < 2 * end; k++) {
+        look_up(k);
+        issue_block(ic<0>(), k);
+        const int r = row * kB + (k & 1) * 64;
+        for (int j = 0; j < NU; j++) {
+            Raw<DT, 8> one;
+            one.load(ybase + r + (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * (unsigned)g.lddy + 8 * piece, g.rows - (r + 8 * piece));
+            put(0, one, j);
+        }
+        stage_barrier<0>();
+        compute(ic<0>());
+        stage_barrier<0>();
     }
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-        const int v = v0 + wn * 16 * NU + 16 * u + i;
+        const int v = t0 + wn * 16 * NU + 16 * u + i;
         if (v >= g.n) continue;
 #pragma unroll
         for (int s = 0; s < 4; s++) {
@@ -717,113 +818,160 @@ struct GradientArgs {
     int64_t ldx8, lds, lddy;
 };
 
-// dA = dy^T x at the stored blocks.  Tile: NB blocks of one block row, steps of 32 vectors; with two blocks a wave has 64
-// rows x 128 columns, with one 64 x 64.  Both operands lie vector by vector, along the sum, and are turned by ds_read_b64_tr_b16
-// on their way out of LDS; x is widened with its scales (exact) on its way in.  The 32 bytes between the rows of LDS
-// put the 4 rows of a read on different banks.
+// dA = dy^T x at the stored blocks, 32 vectors a step.  With NB = 2 a workgroup has two blocks of one block row, a wave
+// 128 rows x 64 columns; with NB = 1 one block, a wave 64 x 64.  Both operands lie vector by vector, along the sum,
+// and have to be turned.  dy, which all waves share, is turned on its way into LDS (a thread has 2 rows of 8
+// vectors).  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane: widened there with
+// the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane i's columns are
+// 4 i + s: its results are 16 neighbours.
 template <typename DT, int NB, typename OT>
 __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, const DT *__restrict__ dy, OT *__restrict__ dv)
 {
-    constexpr int PARTS = parts_of<DT>::value, STEP = 32, NM = 4 * NB, XP = NB * kB + 16, YP = kB + 16;
-    __shared__ __bf16 X[2][STEP * XP];
-    __shared__ __bf16 Y[2][PARTS][STEP * YP];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, i = lane & 15, q = lane >> 4;
-    const int wm = wave & 1, wn = wave >> 1;
+    constexpr int PARTS = parts_of<DT>::value, STEP = 32, NU = 4 * NB, R = NB == 2 ? 2 : 4;
+    __shared__ uint8_t Y[2][PARTS][kB * STEP * 2];           // [row][32 vectors], 16-byte pieces exchanged by XOR
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
     const int wg = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
-    int id[NB], col[NB];
+    const int which = NB == 2 ? wave >> 1 : 0;               // the wave's block, its columns and rows in it
+    const int id0 = NB == 2 ? g.list[2 * wg] : wg, id = NB == 2 ? g.list[2 * wg + which] : wg;
+    const int col = g.block_col[id < 0 ? id0 : id], c0 = (wave & 1) * 64, n0 = NB == 2 ? 0 : (wave >> 1) * 64;
+    const int row0 = g.block_row[id0] * kB;
+    f32x4 acc[NU][4];
 #pragma unroll
-    for (int k = 0; k < NB; k++) {
-        id[k] = g.list ? g.list[NB * wg + k] : wg;
-        col[k] = g.block_col[id[k] < 0 ? id[0] : id[k]];                     // the second one may be missing: computed, not stored
-    }
-    const int row0 = g.block_row[id[0]] * kB;
-    f32x4 acc[4][NM];
+    for (int u = 0; u < NU; u++)
 #pragma unroll
-    for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int s = 0; s < NM; s++) acc[u][s] = f32x4{0, 0, 0, 0};
+        for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    Raw<DT, 8> yr[2];
-    u32x4 xr[NB];
-    int sx[NB];
-    auto fetch = [&](int t0) {
+    Raw<DT, 2> yr[R][8];
+    unsigned xr[R][8];
+    uint64_t sx[R];
+    // A lane's two rows of dy are r and r + 1, loaded from rp, which moves back where they run past the last row: then its
+    // first row is the second loaded, or both are past the end.
+    const int r = row0 + 2 * lane, rp = min(r, max(g.rows - 2, 0));
+    const bool natural = r == rp, shifted = r == rp + 1 && r < g.rows;
+    const unsigned xat = 8 * (unsigned)q * (unsigned)g.ldx8 + 4 * i;
+    auto fetch = [&](auto slot, int t0) {                    // 32 whole vectors, two rows or more
+        constexpr int S = decltype(slot)::value;
+        const uint8_t *xp = g.x8 + (int64_t)t0 * g.ldx8 + col * kB + c0;
+        const DT *yp = dy + (int64_t)(t0 + 8 * wave) * g.lddy;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int t = t0 + j * 16 + (tid >> 4), r = row0 + (tid & 15) * 8;
-            yr[j].load(dy + (int64_t)min(t, g.n - 1) * g.lddy + r, t < g.n ? g.rows - r : 0);
-        }
+        for (int w = 0; w < 8; w++) xr[S][w] = *(const unsigned *)(xp + w * g.ldx8 + xat);
+        __builtin_memcpy(&sx[S], g.xscale + (int64_t)col * g.lds + t0 + 8 * q, 8);
 #pragma unroll
-        for (int k = 0; k < NB; k++) {
-            const int t = t0 + (tid >> 3), v = min(t, g.n - 1);
-            xr[k] = *(const u32x4 *)(g.x8 + (int64_t)v * g.ldx8 + col[k] * kB + (tid & 7) * 16);
-            sx[k] = g.xscale[(int64_t)col[k] * g.lds + v];
-            if (t >= g.n) xr[k] = u32x4{0, 0, 0, 0};
+        for (int w = 0; w < 8; w++) __builtin_memcpy(yr[S][w].v, yp + w * g.lddy + (unsigned)rp, sizeof yr[S][w].v);
+    };
+    // the vectors after the last whole 32; past the last dy is zero, and x the last one's, so that nothing new that is not
+    // finite comes in
+    auto fetch_rest = [&](int t0) {
+        const uint8_t *xp = g.x8 + (int64_t)t0 * g.ldx8 + col * kB + c0 + 4 * i;
+        const DT *yp = dy + (int64_t)t0 * g.lddy + rp;
+        const uint8_t *sp = g.xscale + (int64_t)col * g.lds + t0;
+        const int top = g.n - 1 - t0;
+        sx[0] = 0;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            const int ty = 8 * wave + w, tx = 8 * q + w;
+            yr[0][w].load(yp + (int64_t)min(ty, top) * g.lddy, ty <= top ? min(g.rows, 2) : 0);
+            xr[0][w] = *(const unsigned *)(xp + (int64_t)min(tx, top) * g.ldx8);
+            sx[0] |= (uint64_t)sp[min(tx, top)] << (8 * w);
         }
     };
-    auto put = [&](int buf) {
+    // bytes of two vectors' words that make a row's pair: the first or the second half of each, or zeros
+    const unsigned lo = 0x05040100u, hi = 0x07060302u, none = 0x0c0c0c0cu;
+    const unsigned pick[2] = {natural ? lo : shifted ? hi : none, natural ? hi : none};
+    auto put = [&](auto slot, int buf) {
+        constexpr int S = decltype(slot)::value;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
+        for (int k = 0; k < 2; k++) {
             bf16x8 part[PARTS];
-            split8(yr[j], part);
+            if constexpr (PARTS == 1) {
+                unsigned v[4];
 #pragma unroll
-            for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][(j * 16 + (tid >> 4)) * YP + (tid & 15) * 8] = part[p];
-        }
+                for (int w = 0; w < 4; w++) {
+                    unsigned two[2];
+                    __builtin_memcpy(&two[0], yr[S][2 * w].v, 4);
+                    __builtin_memcpy(&two[1], yr[S][2 * w + 1].v, 4);
+                    v[w] = __builtin_amdgcn_perm(two[1], two[0], pick[k]);
+                }
+                __builtin_memcpy(&part[0], v, 16);
+            } else {
 #pragma unroll
-        for (int k = 0; k < NB; k++) {
-            bf16x8 w[2];
-            const float s = scale_value(sx[k]);
+                for (int w = 0; w < 8; w++) {
+                    const float f = natural ? (float)yr[S][w].v[k] : shifted && k == 0 ? (float)yr[S][w].v[1] : 0.0f;
+                    split1<PARTS>(f, (__bf16 *)&part[0] + w, 8);
+                }
+            }
+            const int row = 2 * lane + k;
 #pragma unroll
-            for (int d = 0; d < 4; d++) unpack4(xr[k][d], s, (__bf16 *)&w[d >> 1] + 4 * (d & 1));
-            *(bf16x8 *)&X[buf][(tid >> 3) * XP + k * kB + (tid & 7) * 16] = w[0];
-            *(bf16x8 *)&X[buf][(tid >> 3) * XP + k * kB + (tid & 7) * 16 + 8] = w[1];
+            for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][row * 64 + ((wave ^ ((row >> 1) & 3)) << 4)] = part[p];
         }
     };
-    // lane (i, q) of an operand: column `at` + i, vectors 8 q .. 8 q + 7
-    auto turned = [&](const __bf16 *p, int pitch, int at) {
-        typedef short i16x4 __attribute__((ext_vector_type(4)));
-        union { i16x4 h[2]; bf16x8 v; } u;
-        const __bf16 *a = p + (8 * q + (i >> 2)) * pitch + at + (i & 3) * 4;
-        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)a);
-        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(a + 4 * pitch));
-        return u.v;
-    };
-    if (g.n > 0) { fetch(0); put(0); }
-    __syncthreads();
-    for (int t0 = 0; t0 < g.n; t0 += STEP) {
-        const int buf = (t0 / STEP) & 1;
-        fetch(t0 + STEP);                                    // past the end: zeros
-        bf16x8 a[NM];
+    auto compute = [&](auto slot, int buf) {
+        constexpr int S = decltype(slot)::value;
+        bf16x8 a[4];
+        {
+            unsigned pair[8][2];                             // columns (0, 1) and (2, 3) of 8 vectors
 #pragma unroll
-        for (int s = 0; s < NM; s++) a[s] = turned(X[buf], XP, wm * 64 * NB + 16 * s);
+            for (int w = 0; w < 8; w++) {
+                const float f = scale_value((int)((unsigned)(sx[S] >> (8 * w)) & 255));
+                __bf16 u[4];
+                unpack4(xr[S][w], f, u);
+                __builtin_memcpy(pair[w], u, 8);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                unsigned v[4];
+#pragma unroll
+                for (int w = 0; w < 4; w++) v[w] = __builtin_amdgcn_perm(pair[2 * w + 1][s >> 1], pair[2 * w][s >> 1], s & 1 ? 0x07060302 : 0x05040100);
+                __builtin_memcpy(&a[s], v, 16);
+            }
+        }
 #pragma unroll
         for (int p = 0; p < PARTS; p++)
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const bf16x8 b = turned(Y[buf][p], YP, wn * 64 + 16 * u);
+            for (int u = 0; u < NU; u++) {
+                const int row = n0 + 16 * u + i;
+                const bf16x8 b = *(const bf16x8 *)&Y[buf][p][row * 64 + ((q ^ ((row >> 1) & 3)) << 4)];
 #pragma unroll
-                for (int s = 0; s < NM; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
+                for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
             }
-        put(buf ^ 1);
+    };
+    const int whole = g.rows < 2 ? 0 : g.n / STEP;           // the rest one by one, a matrix of one row altogether
+    if (whole) {
+        fetch(ic<0>(), 0);
+        if constexpr (R > 2) fetch(ic<1>(), min(1, whole - 1) * STEP);
+        if constexpr (R > 3) fetch(ic<2>(), min(2, whole - 1) * STEP);
+        put(ic<0>(), 0);
+        __syncthreads();
+        ring<R>(0, whole, [&](auto slot, int k) {
+            constexpr int S = decltype(slot)::value;
+            fetch(ic<(S + R - 1) % R>(), min(k + R - 1, whole - 1) * STEP);
+            compute(slot, k & 1);
+            put(ic<(S + 1) % R>(), (k & 1) ^ 1);             // after the last: once more the last, read by nobody
+            __syncthreads();
+        });
+    }
+    for (int t0 = whole * STEP; t0 < g.n; t0 += STEP) {
+        fetch_rest(t0);
+        put(ic<0>(), 0);
+        __syncthreads();
+        compute(ic<0>(), 0);
         __syncthreads();
     }
-    const int mine = NB == 2 ? wm : 0;
-    if (id[mine] < 0) return;
+    if (id < 0) return;
+    // a lane has columns 16 q .. 16 q + 15 of its wave's 64, row 16 u + i; result r of tile s is column 16 q + 4 r + s
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const int r = wn * 64 + 16 * u + i;
+    for (int u = 0; u < NU; u++) {
+        const int row = n0 + 16 * u + i;
+        OT *o = dv + (int64_t)id * kBlockBytes + row * kB + c0 + 16 * q;
+        const int left = row0 + row < g.rows ? g.columns - (col * kB + c0 + 16 * q) : 0;
+        f32x4 v[4];
 #pragma unroll
-        for (int s = 0; s < NM; s++) {
-            const int c = (NB == 2 ? 0 : wm * 64) + 16 * s + 4 * q;
-            OT *o = dv + (int64_t)id[mine] * kBlockBytes + r * kB + c;
-            f32x4 v = acc[u][s];
-            // beyond the edge: dy is zero there along the rows, x along the columns unless it holds what is not finite
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (row0 + r >= g.rows || col[mine] * kB + c + k >= g.columns) v[k] = 0.0f;
-                if (g.accumulate) v[k] += (float)o[k];
-            }
-            store_row<OT, 1>(o, 4, &v);
+        for (int k = 0; k < 16; k++) {
+            // beyond the edge x is zero, but for 8-bit vectors that were not made by quantize8
+            v[k >> 2][k & 3] = k < left ? acc[u][k & 3][k >> 2] : 0.0f;
+            if (g.accumulate) v[k >> 2][k & 3] += (float)o[k];
         }
+        store_row<OT, 4>(o, 16, v);
     }
 }
 
@@ -918,12 +1066,12 @@ static dim3 group_grid(int n, int groups, int r)
     return dim3((unsigned)((n + per - 1) / per), (groups + kQuantGroups - 1) / kQuantGroups);
 }
 
-// Vectors a workgroup takes: `most` where that still gives every CU a tile, else half, down to 64
-static int vectors_per_tile(const spmv_hip_matrix *m, int majors, int n, int most)
+// Tiles of 16 vectors a wave takes: `most` where that still gives every CU a workgroup, else half, down to 2
+static int vector_tiles(const spmv_hip_matrix *m, int majors, int n, int most)
 {
-    int tile = most;
-    while (tile > 64 && (int64_t)majors * ((n + tile - 1) / tile) < m->cus) tile /= 2;
-    return tile;
+    int nu = most;
+    while (nu > 2 && (int64_t)majors * ((n + 32 * nu - 1) / (32 * nu)) < m->cus) nu /= 2;
+    return nu;
 }
 static int check_tiles(const char *what, int majors, int vtiles)
 {
@@ -1109,8 +1257,8 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     a.n = n; a.rows = m->rows; a.brows = m->brows;
     a.ptr = m->d_block_ptr; a.col = m->d_block_col; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
     a.x8 = (const uint8_t *)d_x; a.xscale = d_scale; a.ldx8 = ldx; a.lds = lds; a.ldy = ldy;
-    const int tile = vectors_per_tile(m, m->brows, n, y_dtype == SPMV_HIP_BF16 ? 256 : 128);
-    a.vtiles = (n + tile - 1) / tile;
+    const int nu = vector_tiles(m, m->brows, n, y_dtype == SPMV_HIP_BF16 ? 8 : 4);
+    a.vtiles = (n + 32 * nu - 1) / (32 * nu);
     if (check_tiles(what, m->brows, a.vtiles)) return 1;
     with_elem(y_dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -1118,9 +1266,9 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(m->brows * a.vtiles), dim3(kBlock), 0, (hipStream_t)stream, a, (T *)d_y);
         };
-        if constexpr (!exact) if (tile == 256) { go(product_kernel<exact, 256, T>); return; }
-        if (tile == 128) go(product_kernel<exact, 128, T>);
-        else go(product_kernel<exact, 64, T>);
+        if constexpr (!exact) if (nu == 8) { go(product_kernel<exact, 8, T>); return; }
+        if (nu == 4) go(product_kernel<exact, 4, T>);
+        else go(product_kernel<exact, 2, T>);
     });
     return launched(what);
 }
@@ -1133,6 +1281,10 @@ int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy
     if (!wide_dtype(dy_dtype)) return bad_dtype(what, dy_dtype);
     if (!wide_dtype(dx_dtype)) return bad_dtype(what, dx_dtype);
     if (check_vectors(what, n, d_dy, lddy, m->rows) || check_vectors(what, n, d_dx, lddx, m->columns)) return 1;
+    if (n > 1 && lddy >= (int64_t)1 << 23) {                  // 256 of them stay inside 32-bit offsets
+        set_error("%s: vectors %lld apart, at most 2^23 - 1", what, (long long)lddy);
+        return 1;
+    }
     if (n == 0 || m->columns == 0) return 0;
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
@@ -1140,8 +1292,9 @@ int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy
     a.n = n; a.rows = m->rows; a.columns = m->columns; a.bcols = m->bcols;
     a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
     a.lddy = lddy; a.lddx = lddx;
-    const int tile = vectors_per_tile(m, m->bcols, n, dy_dtype == SPMV_HIP_BF16 ? 256 : 128);
-    a.vtiles = (n + tile - 1) / tile;
+    const int nu = vector_tiles(m, m->bcols, n, dy_dtype == SPMV_HIP_BF16 ? 8 : 4);
+    a.vtiles = (n + 32 * nu - 1) / (32 * nu);
+    const bool direct = dy_dtype == SPMV_HIP_BF16 && (uintptr_t)d_dy % 16 == 0 && lddy % 8 == 0;
     if (check_tiles(what, m->bcols, a.vtiles)) return 1;
     with_elem(dy_dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -1150,9 +1303,17 @@ int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy
             auto go = [&](auto kernel) {
                 hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles), dim3(kBlock), 0, (hipStream_t)stream, a, (const T *)d_dy, (O *)d_dx);
             };
-            if constexpr (std::is_same<T, __bf16>::value) if (tile == 256) { go(transposed_kernel<T, 256, O>); return; }
-            if (tile == 128) go(transposed_kernel<T, 128, O>);
-            else go(transposed_kernel<T, 64, O>);
+            if constexpr (std::is_same<T, __bf16>::value) {
+                if (direct) {
+                    if (nu == 8) go(transposed_kernel<T, true, 8, O>);
+                    else if (nu == 4) go(transposed_kernel<T, true, 4, O>);
+                    else go(transposed_kernel<T, true, 2, O>);
+                    return;
+                }
+                if (nu == 8) { go(transposed_kernel<T, false, 8, O>); return; }
+            }
+            if (nu == 4) go(transposed_kernel<T, false, 4, O>);
+            else go(transposed_kernel<T, false, 2, O>);
         });
     });
     return launched(what);
@@ -1175,7 +1336,8 @@ int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_
     a.n = n; a.rows = m->rows; a.columns = m->columns; a.accumulate = accumulate;
     a.block_row = m->d_block_row; a.block_col = m->d_block_col;
     a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.lddy = lddy;
-    const bool pairs = m->npairs >= m->cus;                  // two blocks a workgroup once they fill the GPU
+    // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the registers
+    const bool pairs = dy_dtype == SPMV_HIP_BF16 && m->npairs >= m->cus;
     a.list = pairs ? m->d_pair : nullptr;
     with_elem(dy_dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -1184,8 +1346,8 @@ int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_
             auto go = [&](auto kernel, int count) {
                 hipLaunchKernelGGL(kernel, dim3(count), dim3(kBlock), 0, (hipStream_t)stream, a, (const T *)d_dy, (O *)d_dvalues);
             };
-            if (pairs) go(gradient_kernel<T, 2, O>, m->npairs);
-            else go(gradient_kernel<T, 1, O>, m->nblocks);
+            if constexpr (std::is_same<T, __bf16>::value) if (pairs) { go(gradient_kernel<T, 2, O>, m->npairs); return; }
+            go(gradient_kernel<T, 1, O>, m->nblocks);
         });
     });
     return launched(what);
