@@ -487,7 +487,7 @@ int spmv_hip_free(spmv_hip_matrix *m)
     void *ptrs[] = {m->d_tile_coord, m->d_row_carry, m->d_val_carry, m->d_nzr_id, m->d_nzr_end, m->d_slice_ptr,
                     m->d_row_order, m->d_scol, m->d_sval, m->d_sorted_len, m->d_vop_ptr, m->d_vop_len,
                     m->d_x, m->d_y, m->d_norm, m->d_hot_col, m->d_hot_old, m->d_hot_x, m->d_xcd_y, m->d_xcd_presence, m->d_xcd_base, m->d_sdiag, m->d_block_pat, m->d_tile_pat,
-                    m->d_block_ptr, m->d_block_col, m->d_block_row, m->d_bt_ptr, m->d_bt_row, m->d_bt_id, m->d_pair, m->d_val8, m->d_scale8};
+                    m->d_block_ptr, m->d_block_col, m->d_block_row, m->d_bt_ptr, m->d_bt_row, m->d_bt_id, m->d_bt_at, m->d_bt_scale8, m->d_pair, m->d_order, m->d_val8, m->d_scale8};
     if (m->xcd_sub) spmv_hip_free(m->xcd_sub);
     for (void *p : ptrs)
         if (p) (void)hipFree(p);

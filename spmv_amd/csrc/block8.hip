@@ -4,8 +4,10 @@
 #include "internal.h"
 #include "device_utils.h"
 
+#include <algorithm>
 #include <new>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 namespace spmv {
@@ -233,7 +235,8 @@ __global__ __launch_bounds__(kBlock) void restore8_kernel(int n, int groups, int
 template <typename T>
 __global__ __launch_bounds__(kBlock) void set_values_kernel(int rows, int columns, const int *__restrict__ block_row,
                                                             const int *__restrict__ block_col, const T *__restrict__ values,
-                                                            uint8_t *__restrict__ val8, int *__restrict__ scale8)
+                                                            uint8_t *__restrict__ val8, const int *__restrict__ bt_at,
+                                                            int *__restrict__ scale8, int *__restrict__ bt_scale8)
 {
     __shared__ float part[kBlock / kWave];
     __shared__ uint8_t out[kBlockBytes];
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(kBlock) void set_values_kernel(int rows, int column
         const int at = (j * kBlock + threadIdx.x) * 16;
         *(u32x4 *)(val8 + k * kBlockBytes + at) = *(const u32x4 *)&out[at];
     }
-    if (threadIdx.x == 0) scale8[k] = b;
+    if (threadIdx.x == 0) { scale8[k] = b; bt_scale8[bt_at[k]] = b; }
 }
 
 __device__ __forceinline__ u32x4 load16(const void *p)       // any alignment
@@ -280,7 +283,8 @@ __device__ __forceinline__ u32x4 load16(const void *p)       // any alignment
 __global__ __launch_bounds__(kBlock) void load8_kernel(int rows, int columns, const int *__restrict__ block_row,
                                                        const int *__restrict__ block_col, const uint8_t *__restrict__ values8,
                                                        const uint8_t *__restrict__ scale, uint8_t *__restrict__ val8,
-                                                       int *__restrict__ scale8)
+                                                       const int *__restrict__ bt_at, int *__restrict__ scale8,
+                                                       int *__restrict__ bt_scale8)
 {
     const int64_t k = blockIdx.x;
     for (int p = threadIdx.x; p < kBlockBytes / 16; p += kBlock) {
@@ -294,7 +298,7 @@ __global__ __launch_bounds__(kBlock) void load8_kernel(int rows, int columns, co
         }
         *(u32x4 *)(val8 + k * kBlockBytes + block8_offset(r, c)) = w;
     }
-    if (threadIdx.x == 0) scale8[k] = scale[k];
+    if (threadIdx.x == 0) { scale8[k] = scale[k]; bt_scale8[bt_at[k]] = scale[k]; }
 }
 
 __global__ __launch_bounds__(kBlock) void store8_kernel(const uint8_t *__restrict__ val8, const int *__restrict__ scale8,
@@ -643,7 +647,7 @@ template <int PARTS> __device__ __forceinline__ void split1(float f, __bf16 *par
 
 struct TransposedArgs {
     int n, rows, columns, bcols, vtiles;
-    const int *ptr, *row, *id, *scale8;
+    const int *ptr, *row, *id, *scale;               // lists by block column, their blocks' scales
     const uint8_t *val8;
     int64_t lddy, lddx;
 };
@@ -697,15 +701,16 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         for (int j = 0; j < NU; j++) at[j] = (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * lddy + 8 * piece;
 
     Raw<DT, 8> yr[DIRECT ? 1 : NU];
-    int sa[R], id = 0, row = 0;                              // id, row: of the half block issued next, loaded a step before
+    int sa[R], id = 0, row = 0, scale = 0;                   // id, row, scale: of the half block issued next, loaded a step before
     auto look_up = [&](int k) {
         id = table(g.id, k >> 1);
         row = table(g.row, k >> 1);
+        scale = table(g.scale, k >> 1);
     };
     auto issue_block = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
         const uint8_t *half = g.val8 + (int64_t)id * kBlockBytes + (k & 1) * (kBlockBytes / 2);
-        sa[S] = table(g.scale8, id);
+        sa[S] = scale;
         // wave w brings strip w: 2 x 4 subtiles of 256 bytes
         const int from = wave * 2048 + q * 256 + ((i ^ (wave << 2)) << 4);
         load_to_lds(half, kBlockBytes / 2, from, &A[S][wave * 2048]);
@@ -832,9 +837,9 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
     const int wg = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
     const int which = NB == 2 ? wave >> 1 : 0;               // the wave's block, its columns and rows in it
-    const int id0 = NB == 2 ? g.list[2 * wg] : wg, id = NB == 2 ? g.list[2 * wg + which] : wg;
-    const int col = g.block_col[id < 0 ? id0 : id], c0 = (wave & 1) * 64, n0 = NB == 2 ? 0 : (wave >> 1) * 64;
-    const int row0 = g.block_row[id0] * kB;
+    const int id0 = table(g.list, NB * wg), id = table(g.list, NB * wg + which);
+    const int col = table(g.block_col, id < 0 ? id0 : id), c0 = (wave & 1) * 64, n0 = NB == 2 ? 0 : (wave >> 1) * 64;
+    const int row0 = table(g.block_row, id0) * kB;
     f32x4 acc[NU][4];
 #pragma unroll
     for (int u = 0; u < NU; u++)
@@ -1111,7 +1116,8 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
     bool ok = false;
     try {
         // the blocks once more, by block column; inside one in ascending block row
-        std::vector<int> row((size_t)nblocks), tptr((size_t)bcols + 1, 0), trow((size_t)nblocks), tid((size_t)nblocks);
+        std::vector<int> row((size_t)nblocks), tptr((size_t)bcols + 1, 0), trow((size_t)nblocks), tid((size_t)nblocks),
+            tat((size_t)nblocks);
         for (int r = 0; r < brows; r++)
             for (int k = block_ptr[r]; k < block_ptr[r + 1]; k++) {
                 row[(size_t)k] = r;
@@ -1125,15 +1131,25 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
             const int w = at[(size_t)block_col[k]]++;
             trow[(size_t)w] = row[(size_t)k];
             tid[(size_t)w] = k;
+            tat[(size_t)k] = w;
         }
-        // two neighbours of a block row each, for the gradient
-        std::vector<int> pair;
+        // For the gradient: the blocks, and two neighbours of a block row each, in an order in which those that run together
+        // share what they read -- 8 block rows and 16 block columns at a time.
+        std::vector<int> order((size_t)nblocks), pair;
+        std::vector<std::pair<int, int>> two;
+        for (int k = 0; k < nblocks; k++) order[(size_t)k] = k;
         for (int r = 0; r < brows; r++)
-            for (int k = block_ptr[r]; k < block_ptr[r + 1]; k += 2) {
-                pair.push_back(k);
-                pair.push_back(k + 1 < block_ptr[r + 1] ? k + 1 : -1);
-            }
-        m->npairs = (int)(pair.size() / 2);
+            for (int k = block_ptr[r]; k < block_ptr[r + 1]; k += 2) two.emplace_back(k, k + 1 < block_ptr[r + 1] ? k + 1 : -1);
+        auto before = [&](int a, int b) {
+            const int ra = row[(size_t)a], rb = row[(size_t)b], ca = block_col[a] / 16, cb = block_col[b] / 16;
+            if (ra / 8 != rb / 8) return ra / 8 < rb / 8;
+            if (ca != cb) return ca < cb;
+            return ra != rb ? ra < rb : a < b;
+        };
+        std::sort(order.begin(), order.end(), before);
+        std::sort(two.begin(), two.end(), [&](const std::pair<int, int> &a, const std::pair<int, int> &b) { return before(a.first, b.first); });
+        for (const auto &t : two) { pair.push_back(t.first); pair.push_back(t.second); }
+        m->npairs = (int)two.size();
         const std::vector<int> scale((size_t)nblocks, 127);
         auto up = [&](int **d, const int *h, size_t count) {
             if (dev_alloc(m, d, count)) return false;
@@ -1143,7 +1159,8 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
         ok = up(&m->d_block_ptr, block_ptr, (size_t)brows + 1) && up(&m->d_block_col, block_col, (size_t)nblocks) &&
              up(&m->d_block_row, row.data(), (size_t)nblocks) && up(&m->d_bt_ptr, tptr.data(), (size_t)bcols + 1) &&
              up(&m->d_bt_row, trow.data(), (size_t)nblocks) && up(&m->d_bt_id, tid.data(), (size_t)nblocks) &&
-             up(&m->d_pair, pair.data(), pair.size()) && up(&m->d_scale8, scale.data(), (size_t)nblocks) && dev_alloc(m, &m->d_val8, (size_t)nblocks * kBlockBytes) == 0;
+             up(&m->d_order, order.data(), order.size()) && up(&m->d_pair, pair.data(), pair.size()) && up(&m->d_bt_at, tat.data(), (size_t)nblocks) && up(&m->d_scale8, scale.data(), (size_t)nblocks) &&
+             up(&m->d_bt_scale8, scale.data(), (size_t)nblocks) && dev_alloc(m, &m->d_val8, (size_t)nblocks * kBlockBytes) == 0;
         if (ok && nblocks) {
             ok = hipMemset(m->d_val8, 0, (size_t)nblocks * kBlockBytes) == hipSuccess && hipDeviceSynchronize() == hipSuccess;
             if (!ok) set_error("clearing the blocks failed");
@@ -1164,7 +1181,7 @@ int spmv_hip_block8_set_values_dev(spmv_hip_matrix *m, const void *d_values, int
     with_elem(dtype, [&](auto t) {
         typedef decltype(t) T;
         hipLaunchKernelGGL((set_values_kernel<T>), dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream, m->rows, m->columns,
-                           m->d_block_row, m->d_block_col, (const T *)d_values, m->d_val8, m->d_scale8);
+                           m->d_block_row, m->d_block_col, (const T *)d_values, m->d_val8, m->d_bt_at, m->d_scale8, m->d_bt_scale8);
     });
     return launched("block8_set_values");
 }
@@ -1177,7 +1194,7 @@ int spmv_hip_block8_load_dev(spmv_hip_matrix *m, const uint8_t *d_values8, const
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
     hipLaunchKernelGGL(load8_kernel, dim3(m->nblocks), dim3(kBlock), 0, (hipStream_t)stream, m->rows, m->columns, m->d_block_row,
-                       m->d_block_col, d_values8, d_scale, m->d_val8, m->d_scale8);
+                       m->d_block_col, d_values8, d_scale, m->d_val8, m->d_bt_at, m->d_scale8, m->d_bt_scale8);
     return launched("block8_load");
 }
 
@@ -1290,7 +1307,7 @@ int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy
     if (!on.ok) return 1;
     TransposedArgs a{};
     a.n = n; a.rows = m->rows; a.columns = m->columns; a.bcols = m->bcols;
-    a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
+    a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale = m->d_bt_scale8;
     a.lddy = lddy; a.lddx = lddx;
     const int nu = vector_tiles(m, m->bcols, n, dy_dtype == SPMV_HIP_BF16 ? 8 : 4);
     a.vtiles = (n + 32 * nu - 1) / (32 * nu);
@@ -1337,8 +1354,9 @@ int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_
     a.block_row = m->d_block_row; a.block_col = m->d_block_col;
     a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.lddy = lddy;
     // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the registers
-    const bool pairs = dy_dtype == SPMV_HIP_BF16 && m->npairs >= m->cus;
-    a.list = pairs ? m->d_pair : nullptr;
+    // and not where many pairs lack their second block
+    const bool pairs = dy_dtype == SPMV_HIP_BF16 && m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
+    a.list = pairs ? m->d_pair : m->d_order;
     with_elem(dy_dtype, [&](auto t) {
         typedef decltype(t) T;
         with_elem(dtype, [&](auto o) {

@@ -133,8 +133,9 @@ struct spmv_hip_matrix {
     int nblocks = 0, brows = 0, bcols = 0;
     int *d_block_ptr = nullptr, *d_block_col = nullptr, *d_block_row = nullptr;
     int *d_bt_ptr = nullptr, *d_bt_row = nullptr, *d_bt_id = nullptr;
+    int *d_bt_at = nullptr, *d_bt_scale8 = nullptr; // a block's place in the lists by block column, the scale bytes in their order
     int npairs = 0;                 // two blocks of one block row each (the second -1 where the row runs out)
-    int *d_pair = nullptr;
+    int *d_pair = nullptr, *d_order = nullptr;      // pairs and single blocks in the gradient's order
     uint8_t *d_val8 = nullptr;      // [nblocks][16384] in the order of block8_offset
     int *d_scale8 = nullptr;        // [nblocks] scale byte, one per word (read by scalar loads)
 
