@@ -29,8 +29,26 @@ MAX_WIDE = 64                         # vectors a product rounds to 8 bits by it
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# torch's current stream on a device, as an address.  The public torch.cuda.current_stream(device).cuda_stream builds a
+# Stream object for it: 1.5 us, against 5 us for a whole call with few vectors.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+class _On:
+    """Makes `device` current for calls without a handle, which know no device of their own; free where it is already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def _wide(name: str, x: torch.Tensor, length: int | None = None) -> torch.Tensor:
@@ -71,6 +89,13 @@ class Packed8:
         self.values, self.scale, self.columns, self.dtype = values, scale, columns, dtype
         self.shape = tuple(shape) if shape is not None else (values.shape[0], columns)
 
+    @classmethod
+    def _made(cls, values, scale, columns, dtype, shape):
+        """Of tensors made here: nothing to check."""
+        q = object.__new__(cls)
+        q.values, q.scale, q.columns, q.dtype, q.shape = values, scale, columns, dtype, shape
+        return q
+
     @property
     def n(self) -> int:
         return self.values.shape[0]
@@ -80,11 +105,11 @@ class Packed8:
         dtype = dtype or self.dtype
         if dtype not in _DTYPE:
             raise TypeError("dtype must be float32, bfloat16 or float16")
-        x = torch.empty(self.shape, dtype=dtype, device=self.values.device)
-        with torch.cuda.device(x.device):
-            L.check(L.lib().spmv_hip_restore8_dev(self.n, self.columns, self.values.data_ptr(), self.values.shape[1],
-                                                  self.scale.data_ptr(), self.n, x.data_ptr(), _DTYPE[dtype], self.columns,
-                                                  _stream(x.device)))
+        device, (n, ld8) = self.values.device, self.values.shape
+        x = torch.empty(self.shape, dtype=dtype, device=device)
+        with _On(device):
+            L.check(L.lib().spmv_hip_restore8_dev(n, self.columns, self.values.data_ptr(), ld8, self.scale.data_ptr(), n,
+                                                  x.data_ptr(), _DTYPE[dtype], self.columns, _raw_stream(device.index)))
         return x
 
 
@@ -93,12 +118,13 @@ def quantize(x: torch.Tensor) -> Packed8:
     rows = _wide("x", x.detach() if isinstance(x, torch.Tensor) else x)
     n, columns = rows.shape
     groups = -(-columns // BLOCK)
-    values = torch.empty((n, groups * BLOCK), dtype=torch.uint8, device=rows.device)
-    scale = torch.empty((groups, n), dtype=torch.uint8, device=rows.device)
-    with torch.cuda.device(rows.device):
+    device = rows.device
+    values = torch.empty((n, groups * BLOCK), dtype=torch.uint8, device=device)
+    scale = torch.empty((groups, n), dtype=torch.uint8, device=device)
+    with _On(device):
         L.check(L.lib().spmv_hip_quantize8_dev(n, columns, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows), values.data_ptr(),
-                                               groups * BLOCK, scale.data_ptr(), n, _stream(rows.device)))
-    return Packed8(values, scale, columns, rows.dtype, x.shape)
+                                               groups * BLOCK, scale.data_ptr(), n, _raw_stream(device.index)))
+    return Packed8._made(values, scale, columns, rows.dtype, x.shape)
 
 
 class Block8(Matrix):
@@ -112,7 +138,8 @@ class Block8(Matrix):
             raise ValueError(f"block_ptr has shape {ptr.shape} for {rows} rows, block_col {col.shape}")
         super().__init__(L.lib().spmv_hip_create_block8(rows, columns, len(col), ptr.ctypes.data, col.ctypes.data))
         self.rows, self.columns, self.nblocks = rows, columns, len(col)
-        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = torch.cuda.current_device()
+        self.device = torch.device("cuda", self._index)
         self.values = None               # the tensor set_values last took: the leaf that linear() differentiates
         self._version = 0                # set_values / load calls so far
 
@@ -146,7 +173,7 @@ class Block8(Matrix):
     def set_values(self, values: torch.Tensor) -> None:
         """Rounds values [blocks, 128, 128] into the matrix.  linear() returns the gradient of this tensor."""
         self._blocks("values", values, _DTYPE)
-        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _stream(self.device)))
+        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _raw_stream(self._index)))
         self.values = values
         self._version += 1
 
@@ -156,7 +183,7 @@ class Block8(Matrix):
         if scale.dtype != torch.uint8 or tuple(scale.shape) != (self.nblocks,) or not scale.is_contiguous():
             raise ValueError(f"scale must be a contiguous uint8 tensor [{self.nblocks}]")
         self._here("scale", scale)
-        L.check(L.lib().spmv_hip_block8_load_dev(self._h, values8.data_ptr(), scale.data_ptr(), _stream(self.device)))
+        L.check(L.lib().spmv_hip_block8_load_dev(self._h, values8.data_ptr(), scale.data_ptr(), _raw_stream(self._index)))
         self.values = None
         self._version += 1
 
@@ -164,7 +191,7 @@ class Block8(Matrix):
         """(values8 uint8 [blocks, 128, 128], scale uint8 [blocks]): what load takes."""
         values8 = torch.empty((self.nblocks, BLOCK, BLOCK), dtype=torch.uint8, device=self.device)
         scale = torch.empty(self.nblocks, dtype=torch.uint8, device=self.device)
-        L.check(L.lib().spmv_hip_block8_store_dev(self._h, values8.data_ptr(), scale.data_ptr(), _stream(self.device)))
+        L.check(L.lib().spmv_hip_block8_store_dev(self._h, values8.data_ptr(), scale.data_ptr(), _raw_stream(self._index)))
         return values8, scale
 
     def product(self, x, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -177,7 +204,7 @@ class Block8(Matrix):
             if rows.shape[0] <= MAX_WIDE:
                 y = self._out(out, shape, dtype or rows.dtype, rows)
                 L.check(L.lib().spmv_hip_block8_mult_dev(self._h, rows.shape[0], rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
-                                                         None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self.device)))
+                                                         None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _raw_stream(self._index)))
                 return y
             dtype = dtype or rows.dtype
             x = quantize(rows)
@@ -188,7 +215,7 @@ class Block8(Matrix):
             shape = (*x.shape[:-1], self.rows)
         y = self._out(out, shape, dtype or x.dtype, x.values)
         L.check(L.lib().spmv_hip_block8_mult_dev(self._h, x.n, x.values.data_ptr(), L.E4M3, x.values.shape[1], x.scale.data_ptr(),
-                                                 x.n, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self.device)))
+                                                 x.n, y.data_ptr(), _DTYPE[y.dtype], self.rows, _raw_stream(self._index)))
         return y
 
     def product_t(self, dy: torch.Tensor, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -197,7 +224,7 @@ class Block8(Matrix):
         self._here("dy", d)
         dx = self._out(out, (*dy.shape[:-1], self.columns), dtype or d.dtype, d)
         L.check(L.lib().spmv_hip_block8_mult_t_dev(self._h, d.shape[0], d.data_ptr(), _DTYPE[d.dtype], _ld(d), dx.data_ptr(),
-                                                   _DTYPE[dx.dtype], self.columns, _stream(self.device)))
+                                                   _DTYPE[dx.dtype], self.columns, _raw_stream(self._index)))
         return dx
 
     def gradient(self, dy: torch.Tensor, x: Packed8, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
@@ -215,7 +242,7 @@ class Block8(Matrix):
         dv = self._out(out, (self.nblocks, BLOCK, BLOCK), out.dtype if out is not None else dtype, d)
         L.check(L.lib().spmv_hip_block8_gradient_dev(self._h, d.shape[0], d.data_ptr(), _DTYPE[d.dtype], _ld(d), x.values.data_ptr(),
                                                      x.values.shape[1], x.scale.data_ptr(), x.n, dv.data_ptr(), _DTYPE[dv.dtype],
-                                                     int(accumulate), _stream(self.device)))
+                                                     int(accumulate), _raw_stream(self._index)))
         return dv
 
     def linear(self, x: torch.Tensor) -> torch.Tensor:
@@ -249,5 +276,5 @@ class _Linear(torch.autograd.Function):
         dx = matrix.product_t(dy, ctx.x_dtype) if ctx.needs_input_grad[0] else None
         dv = None
         if ctx.needs_input_grad[1]:
-            dv = matrix.gradient(dy, Packed8(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), ctx.values_dtype)
+            dv = matrix.gradient(dy, Packed8._made(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), ctx.values_dtype)
         return dx, dv, None
