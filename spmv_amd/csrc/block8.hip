@@ -464,11 +464,14 @@ __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b)
     return (i32x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// 64 lanes x 16 bytes into LDS, lane l to lds + 16 l (lds is the wave's), from a 32-bit offset a lane into the `records`
-// bytes at base, zeros from past them.
-__device__ __forceinline__ void load_to_lds(const void *base, unsigned records, unsigned offset, uint8_t *lds)
+// `records` bytes at a wave-uniform address; loads past them bring zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *base, unsigned records)
 {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)records, 0x00027000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)records, 0x00027000);
+}
+// 64 lanes x 16 bytes into LDS, lane l to lds + 16 l (lds is the wave's), from its own offset into the buffer
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned offset, uint8_t *lds)
+{
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, (int)offset, 0, 0, 0);
 }
 
@@ -548,9 +551,10 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
     // piece j of a thread: 16 bytes of vector 32 j + t.  The 16-byte pieces of vector v are exchanged by v / NU, which
     // for 256 vectors differs between even and odd j.  Past the last vector zeros.
     const int t = wave * 8 + (lane >> 3);
-    const unsigned at = (unsigned)t * (unsigned)g.ldx8 + (((lane & 7) ^ ((t / NU) & 7)) << 4), flip = NU == 8 ? 64 : 0;
+    const unsigned at = (unsigned)t * (unsigned)g.ldx8 + (((lane & 7) ^ ((t / NU) & 7)) << 4);
     const uint8_t *xbase = g.x8 + (int64_t)t0 * g.ldx8;
     const unsigned ldx8 = (unsigned)g.ldx8, records = (unsigned)min(g.n - t0, TOK) * ldx8;
+    const __amdgpu_buffer_rsrc_t xs = buffer(xbase, records);
     const int back = max(v0 + NU - g.n, 0);                  // n > NU, so the load of scale bytes can move back from the end
 
     i32x8 a[R][4];
@@ -561,8 +565,13 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
         constexpr int S = decltype(slot)::value;
 #pragma unroll
         for (int j = 0; j < NU; j++) {
-            const unsigned skip = min((unsigned)j * 32 * ldx8 + c * kB, records);
-            load_to_lds(xbase + skip, records - skip, j & 1 ? at ^ flip : at, &X[S][(j * 32 + wave * 8) * kB]);
+            const unsigned skip = j * 32 * ldx8 + c * kB;
+            uint8_t *to = &X[S][(j * 32 + wave * 8) * kB];
+            if constexpr (NU < 8) load_to_lds(xs, at + skip, to);
+            else {                                           // 8 offsets more are too many registers: the buffer moves
+                const unsigned gone = min(skip, records);
+                load_to_lds(buffer(xbase + gone, records - gone), j & 1 ? at ^ 64 : at, to);
+            }
         }
         const uint8_t *half = g.val8 + (int64_t)b * kBlockBytes + wm * (kBlockBytes / 2);
 #pragma unroll
@@ -575,12 +584,19 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
     auto step = [&](auto slot, int b) {
         constexpr int S = decltype(slot)::value;
         stage_barrier<(R - 2) * (NU + 8)>();
-        issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
-        const uint64_t bytes = sx[S] >> (8 * min(back, 7));
         auto operand = [&](int u) {
             const uint8_t *row = &X[S][(wn * 16 * NU + NU * i + u) * kB];
             return join(*(const u32x4 *)(row + ((q ^ (i & 7)) << 4)), *(const u32x4 *)(row + (((q + 4) ^ (i & 7)) << 4)));
         };
+        // The first reads before the next stage's loads, which take a while to issue.  With few tiles all of them; with 8
+        // one tile ahead and no more: left alone, the compiler reads all of them first and runs out of registers.
+        constexpr int AHEAD = NU == 8 ? 1 : NU;
+        i32x8 w[NU];
+        if constexpr (NU == 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) w[u] = operand(u);
+        if constexpr (NU < 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
+        const uint64_t bytes = sx[S] >> (8 * min(back, 7));
         bf16x8 aw[4][EXACT ? 4 : 1];
         if constexpr (EXACT) {
             const float fa = scale_value(sa[S]);
@@ -589,30 +605,26 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
 #pragma unroll
                 for (int d = 0; d < 8; d++) unpack4((unsigned)a[S][s][d], fa, (__bf16 *)&aw[s][d >> 1] + 4 * (d & 1));
         }
-        i32x8 w = operand(0);
 #pragma unroll
         for (int u = 0; u < NU; u++) {
-            // one tile ahead and no more: left alone, the compiler reads all of them first and runs out of registers
-            i32x8 ahead = w;
-            if (u + 1 < NU) ahead = operand(u + 1);
+            if (u + AHEAD < NU) w[u + AHEAD] = operand(u + AHEAD);
             const int su = (int)(bytes >> (8 * u)) & 255;
             if constexpr (EXACT) {
                 const float fx = scale_value(su);
 #pragma unroll
                 for (int p = 0; p < 4; p++) {
                     bf16x8 xw;
-                    unpack4((unsigned)w[2 * p], fx, (__bf16 *)&xw);
-                    unpack4((unsigned)w[2 * p + 1], fx, (__bf16 *)&xw + 4);
+                    unpack4((unsigned)w[u][2 * p], fx, (__bf16 *)&xw);
+                    unpack4((unsigned)w[u][2 * p + 1], fx, (__bf16 *)&xw + 4);
 #pragma unroll
                     for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw[s][p], xw, acc[u][s], 0, 0, 0);
                 }
             } else {
 #pragma unroll
                 for (int s = 0; s < 4; s++)
-                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[S][s], w, acc[u][s], 0, 0, 0, sa[S], 0, su);
+                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[S][s], w[u], acc[u][s], 0, 0, 0, sa[S], 0, su);
             }
-            w = ahead;
-            __builtin_amdgcn_sched_barrier(0);
+            if (NU == 8) __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (first < last) {
@@ -638,10 +650,12 @@ template <> struct parts_of<float> { static constexpr int value = 3; };
 
 template <int PARTS> __device__ __forceinline__ void split1(float f, __bf16 *part, int stride)
 {
+    const bool finite = fabsf(f) < __builtin_inff();         // infinities and NaN: all in the first
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
         part[p * stride] = (__bf16)f;
         f -= (float)part[p * stride];
+        if (p == 0) f = finite ? f : 0.0f;
     }
 }
 
@@ -694,7 +708,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
     const DT *ybase = dy + (int64_t)t0 * g.lddy;
     const int row_of_lane = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((row_of_lane >> 1) & 7);
     const unsigned lddy = (unsigned)g.lddy, near = row_of_lane * lddy + 8 * piece;
-    const unsigned records = (unsigned)min(g.n - t0, TOK) * lddy * 2;        // bytes, DIRECT
+    const __amdgpu_buffer_rsrc_t ys = buffer(ybase, (unsigned)min(g.n - t0, TOK) * lddy * (unsigned)sizeof(DT));      // DIRECT
     unsigned at[DIRECT ? 1 : NU];
     if constexpr (!DIRECT)
 #pragma unroll
@@ -709,12 +723,12 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
     };
     auto issue_block = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
-        const uint8_t *half = g.val8 + (int64_t)id * kBlockBytes + (k & 1) * (kBlockBytes / 2);
+        const __amdgpu_buffer_rsrc_t half = buffer(g.val8 + (int64_t)id * kBlockBytes + (k & 1) * (kBlockBytes / 2), kBlockBytes / 2);
         sa[S] = scale;
         // wave w brings strip w: 2 x 4 subtiles of 256 bytes
         const int from = wave * 2048 + q * 256 + ((i ^ (wave << 2)) << 4);
-        load_to_lds(half, kBlockBytes / 2, from, &A[S][wave * 2048]);
-        load_to_lds(half, kBlockBytes / 2, from + 1024, &A[S][wave * 2048 + 1024]);
+        load_to_lds(half, from, &A[S][wave * 2048]);
+        load_to_lds(half, from + 1024, &A[S][wave * 2048 + 1024]);
     };
     auto issue = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
@@ -723,8 +737,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 #pragma unroll
         for (int j = 0; j < NU; j++)
             if constexpr (DIRECT) {
-                const unsigned skip = min((j * 32 * lddy + r) * 2, records);
-                load_to_lds((const uint8_t *)ybase + skip, records - skip, near * 2, &Y[S][0][(j * 32 + wave * 8) * 128]);
+                load_to_lds(ys, near * 2 + (j * 32 * lddy + r) * 2, &Y[S][0][(j * 32 + wave * 8) * 128]);
             } else {
                 __builtin_memcpy(yr[j].v, ybase + r + at[j], sizeof yr[j].v);
             }
@@ -736,45 +749,63 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 #pragma unroll
         for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[slot][p][(j * 32 + wave * 8) * 128 + lane * 16] = part[p];
     };
-    auto compute = [&](auto slot) {
+    // `between` runs after the first reads from LDS: the next stage's loads, which take a while to issue.  With few tiles all
+    // reads come first; with 8 those of the first half of the rows, then one tile ahead and no more.
+    auto compute = [&](auto slot, auto between) {
         constexpr int S = decltype(slot)::value;
-        const float fa = scale_value(sa[S]);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
+        constexpr bool ALL = NU < 8;
+        auto read_a = [&](int h, int s) {
             // row 32 h + 8 q + w, w = i >> 1, columns 8 (i & 1) .. + 7 of a subtile
             const int strip = (2 * q + (i >> 3)) & 3, quad = 2 * h + (q >> 1);
             const uint8_t *p = &A[S][strip * 2048 + wm * 1024 + ((quad ^ strip) << 6) + ((i >> 1) & 3) * 16 + (i & 1) * 8];
+            return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2 *)(p + s * 256));
+        };
+        auto read_b = [&](int h, int part, int u) {
+            const int t = wn * 16 * NU + 16 * u + i;
+            return *(const bf16x8 *)&Y[S][part][t * 128 + (((4 * h + q) ^ ((t >> 1) & 7)) << 4)];
+        };
+        i32x2 w[2][4];
+        bf16x8 b[2][PARTS][NU];
+#pragma unroll
+        for (int h = 0; h < (ALL ? 2 : 1); h++) {
+#pragma unroll
+            for (int s = 0; s < 4; s++) w[h][s] = read_a(h, s);
+#pragma unroll
+            for (int part = 0; part < PARTS; part++)
+#pragma unroll
+                for (int u = 0; u < (ALL ? NU : 1); u++) b[h][part][u] = read_b(h, part, u);
+        }
+        const float fa = scale_value(sa[S]);
+        between();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if constexpr (!ALL)
+                if (h == 1) {
+#pragma unroll
+                    for (int s = 0; s < 4; s++) w[1][s] = read_a(1, s);
+                    b[1][0][0] = read_b(1, 0, 0);
+                }
             bf16x8 a[4];
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2 *)(p + s * 256));
-                unpack4((unsigned)w[0], fa, (__bf16 *)&a[s]);
-                unpack4((unsigned)w[1], fa, (__bf16 *)&a[s] + 4);
+                unpack4((unsigned)w[h][s][0], fa, (__bf16 *)&a[s]);
+                unpack4((unsigned)w[h][s][1], fa, (__bf16 *)&a[s] + 4);
             }
-            auto operand = [&](int part, int u) {
-                const int t = wn * 16 * NU + 16 * u + i;
-                return *(const bf16x8 *)&Y[S][part][t * 128 + (((4 * h + q) ^ ((t >> 1) & 7)) << 4)];
-            };
 #pragma unroll
-            for (int part = 0; part < PARTS; part++) {
-                bf16x8 b = operand(part, 0);
+            for (int part = 0; part < PARTS; part++)
 #pragma unroll
                 for (int u = 0; u < NU; u++) {
-                    bf16x8 ahead = b;                        // one tile ahead and no more
-                    if (u + 1 < NU) ahead = operand(part, u + 1);
+                    if constexpr (!ALL) if (u + 1 < NU) b[h][part][u + 1] = read_b(h, part, u + 1);
 #pragma unroll
-                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
-                    b = ahead;
-                    if (u & 1) __builtin_amdgcn_sched_barrier(0);
+                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[h][part][u], acc[u][s], 0, 0, 0);
+                    if (!ALL && (u & 1)) __builtin_amdgcn_sched_barrier(0);
                 }
-            }
         }
     };
     auto step = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
         stage_barrier<DIRECT ? (R - 2) * (2 + NU) : 0>();
-        issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1));
-        compute(slot);
+        compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
         if constexpr (!DIRECT)
 #pragma unroll
             for (int j = 0; j < NU; j++) put((S + 1) % R, yr[j], j);
@@ -800,7 +831,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
             put(0, one, j);
         }
         stage_barrier<0>();
-        compute(ic<0>());
+        compute(ic<0>(), [] {});
         stage_barrier<0>();
     }
 #pragma unroll
@@ -910,8 +941,16 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
             for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][row * 64 + ((wave ^ ((row >> 1) & 3)) << 4)] = part[p];
         }
     };
-    auto compute = [&](auto slot, int buf) {
-        constexpr int S = decltype(slot)::value;
+    auto compute = [&](auto slot, int buf, auto between) {
+        constexpr int S = decltype(slot)::value, AHEAD = PARTS * NU <= 8 ? PARTS * NU : 4;
+        auto read_b = [&](int k) {
+            const int row = n0 + 16 * (k % NU) + i;
+            return *(const bf16x8 *)&Y[buf][k / NU][row * 64 + ((q ^ ((row >> 1) & 3)) << 4)];
+        };
+        bf16x8 b[PARTS * NU];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) b[k] = read_b(k);
+        between();                                           // the loads of a later stage, which take a while to issue
         bf16x8 a[4];
         {
             unsigned pair[8][2];                             // columns (0, 1) and (2, 3) of 8 vectors
@@ -931,14 +970,11 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
             }
         }
 #pragma unroll
-        for (int p = 0; p < PARTS; p++)
+        for (int k = 0; k < PARTS * NU; k++) {
+            if (k + AHEAD < PARTS * NU) b[k + AHEAD] = read_b(k + AHEAD);
 #pragma unroll
-            for (int u = 0; u < NU; u++) {
-                const int row = n0 + 16 * u + i;
-                const bf16x8 b = *(const bf16x8 *)&Y[buf][p][row * 64 + ((q ^ ((row >> 1) & 3)) << 4)];
-#pragma unroll
-                for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b, acc[u][s], 0, 0, 0);
-            }
+            for (int s = 0; s < 4; s++) acc[k % NU][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[k], acc[k % NU][s], 0, 0, 0);
+        }
     };
     const int whole = g.rows < 2 ? 0 : g.n / STEP;           // the rest one by one, a matrix of one row altogether
     if (whole) {
@@ -949,8 +985,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
         __syncthreads();
         ring<R>(0, whole, [&](auto slot, int k) {
             constexpr int S = decltype(slot)::value;
-            fetch(ic<(S + R - 1) % R>(), min(k + R - 1, whole - 1) * STEP);
-            compute(slot, k & 1);
+            compute(slot, k & 1, [&] { fetch(ic<(S + R - 1) % R>(), min(k + R - 1, whole - 1) * STEP); });
             put(ic<(S + 1) % R>(), (k & 1) ^ 1);             // after the last: once more the last, read by nobody
             __syncthreads();
         });
@@ -959,7 +994,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
         fetch_rest(t0);
         put(ic<0>(), 0);
         __syncthreads();
-        compute(ic<0>(), 0);
+        compute(ic<0>(), 0, [] {});
         __syncthreads();
     }
     if (id < 0) return;

@@ -336,6 +336,27 @@ def test_non_finite_vectors_stay_in_their_rows():
         assert torch.equal(c.A.gradient(wide[:n, :256], q), c.A.gradient(d, q))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 90])
+def test_infinities_in_dy_reach_what_they_multiply(dtype, n):
+    """inf * a is inf or, where a is 0, NaN: never NaN because dy was split into parts"""
+    c = Case(300, 256, 1.0, 9)
+    x, dy = _vectors(n, 256, dtype, 1), _vectors(n, 300, dtype, 2)
+    x[x == 0] = 1.0
+    dy[1, 7], dy[3, 299], dy[4, 130] = float("inf"), -float("inf"), float("nan")
+    xq, d = O.quantized(_np(x)), _np(dy)
+    with np.errstate(invalid="ignore"):
+        dx = np.zeros((n, 256))                              # block by block: what no stored block touches is not multiplied
+        for r in range(len(c.ptr) - 1):
+            for k in range(c.ptr[r], c.ptr[r + 1]):
+                rows, j = d[:, r * 128:(r + 1) * 128], c.col[k] * 128
+                dx[:, j:j + 128] += np.einsum("tr,rc->tc", rows, c.blocks[k][:rows.shape[1]])
+        for got, want in ((_np(c.A.product_t(dy, F32)), dx),
+                          (_np(c.A.gradient(dy, quantize(x))), O.sampled(np.einsum("tr,tc->rc", d, xq), c.ptr, c.col))):
+            assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+            assert np.array_equal(np.sign(got[np.isinf(got)]), np.sign(want[np.isinf(want)]))
+
+
 def test_general_entry_points_take_a_block8_handle():
     """mult, mult_dev, mult_mv, mult_mv_dev and bench of any handle (F32 vectors)"""
     c = Case(390, 390, 0.8, 10)
