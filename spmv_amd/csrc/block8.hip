@@ -450,6 +450,9 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
 
 template <int V> using ic = std::integral_constant<int, V>;
 
+// Keeps a scalar load where it is written: the compiler would move it down to its use in the next step, and wait there
+__device__ __forceinline__ void here(int &a) { asm volatile("" : "+s"(a)); }
+
 // Wait until at most N of the wave's loads are outstanding and its LDS reads are done, then meet the others.  What the
 // compiler does not see, it does not move: the asm statements order the memory accesses around them.
 template <int N> __device__ __forceinline__ void stage_barrier()
@@ -464,15 +467,28 @@ __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b)
     return (i32x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// `records` bytes at a wave-uniform address; loads past them bring zeros
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *base, unsigned records)
+// `records` bytes at a wave-uniform address (a raw buffer descriptor); loads past them bring zeros
+__device__ __forceinline__ u32x4 buffer(const void *base, unsigned records)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)records, 0x00027000);
+    const uint64_t at = (uint64_t)base;
+    return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, records, 0x00027000u};
 }
-// 64 lanes x 16 bytes into LDS, lane l to lds + 16 l (lds is the wave's), from its own offset into the buffer
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned offset, uint8_t *lds)
+// 64 lanes x 16 bytes into LDS, lane l to lds + 16 l (lds is the wave's), from its own offset into the buffer.
+// ASM: behind the builtin the compiler makes LDS reads that it cannot tell apart from these stores wait for all of them; in
+// assembly it does not see them, and the wait is stage_barrier's alone (transposed product of 8192 vectors, full 8192 x
+// 8192: 890 -> 824 us).  But neither does it move anything past the assembly (the product: 430 -> 490 us), so it is for
+// the kernel that needs it.  The load has no register results; m0 needs a cycle before it is used, and a descriptor that
+// a vector instruction made (readfirstlane) five.
+template <bool ASM> __device__ __forceinline__ void load_to_lds(u32x4 r, unsigned offset, uint8_t *lds)
 {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, (int)offset, 0, 0, 0);
+    const auto to = (__attribute__((address_space(3))) uint8_t *)lds;
+    if constexpr (ASM)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                     ::"v"(offset), "s"(r), "s"(__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)to)) : "memory", "m0");
+    else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)r[1] << 32 | r[0]), 0, (int)r[2], (int)r[3]),
+            (__attribute__((address_space(3))) void *)to, 16, (int)offset, 0, 0, 0);
 }
 
 // step(slot, k) for k = first .. last - 1, slot = (k - first) % R as a constant: whole rounds, then what is left (exits
@@ -554,7 +570,7 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
     const unsigned at = (unsigned)t * (unsigned)g.ldx8 + (((lane & 7) ^ ((t / NU) & 7)) << 4);
     const uint8_t *xbase = g.x8 + (int64_t)t0 * g.ldx8;
     const unsigned ldx8 = (unsigned)g.ldx8, records = (unsigned)min(g.n - t0, TOK) * ldx8;
-    const __amdgpu_buffer_rsrc_t xs = buffer(xbase, records);
+    const u32x4 xs = buffer(xbase, records);
     const int back = max(v0 + NU - g.n, 0);                  // n > NU, so the load of scale bytes can move back from the end
 
     i32x8 a[R][4];
@@ -567,10 +583,10 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
         for (int j = 0; j < NU; j++) {
             const unsigned skip = j * 32 * ldx8 + c * kB;
             uint8_t *to = &X[S][(j * 32 + wave * 8) * kB];
-            if constexpr (NU < 8) load_to_lds(xs, at + skip, to);
+            if constexpr (NU < 8) load_to_lds<false>(xs, at + skip, to);
             else {                                           // 8 offsets more are too many registers: the buffer moves
                 const unsigned gone = min(skip, records);
-                load_to_lds(buffer(xbase + gone, records - gone), j & 1 ? at ^ 64 : at, to);
+                load_to_lds<false>(buffer(xbase + gone, records - gone), j & 1 ? at ^ 64 : at, to);
             }
         }
         const uint8_t *half = g.val8 + (int64_t)b * kBlockBytes + wm * (kBlockBytes / 2);
@@ -583,6 +599,8 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
     };
     auto step = [&](auto slot, int b) {
         constexpr int S = decltype(slot)::value;
+        here(c);
+        here(scale);
         stage_barrier<(R - 2) * (NU + 8)>();
         auto operand = [&](int u) {
             const uint8_t *row = &X[S][(wn * 16 * NU + NU * i + u) * kB];
@@ -590,7 +608,7 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
         };
         // The first reads before the next stage's loads, which take a while to issue.  With few tiles all of them; with 8
         // one tile ahead and no more: left alone, the compiler reads all of them first and runs out of registers.
-        constexpr int AHEAD = NU == 8 ? 1 : NU;
+        constexpr int AHEAD = NU == 8 || EXACT ? 1 : NU;
         i32x8 w[NU];
         if constexpr (NU == 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
 #pragma unroll
@@ -708,7 +726,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
     const DT *ybase = dy + (int64_t)t0 * g.lddy;
     const int row_of_lane = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((row_of_lane >> 1) & 7);
     const unsigned lddy = (unsigned)g.lddy, near = row_of_lane * lddy + 8 * piece;
-    const __amdgpu_buffer_rsrc_t ys = buffer(ybase, (unsigned)min(g.n - t0, TOK) * lddy * (unsigned)sizeof(DT));      // DIRECT
+    const u32x4 ys = buffer(ybase, (unsigned)min(g.n - t0, TOK) * lddy * (unsigned)sizeof(DT));      // DIRECT
     unsigned at[DIRECT ? 1 : NU];
     if constexpr (!DIRECT)
 #pragma unroll
@@ -723,12 +741,12 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
     };
     auto issue_block = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
-        const __amdgpu_buffer_rsrc_t half = buffer(g.val8 + (int64_t)id * kBlockBytes + (k & 1) * (kBlockBytes / 2), kBlockBytes / 2);
+        const u32x4 half = buffer(g.val8 + (int64_t)id * kBlockBytes + (k & 1) * (kBlockBytes / 2), kBlockBytes / 2);
         sa[S] = scale;
         // wave w brings strip w: 2 x 4 subtiles of 256 bytes
         const int from = wave * 2048 + q * 256 + ((i ^ (wave << 2)) << 4);
-        load_to_lds(half, from, &A[S][wave * 2048]);
-        load_to_lds(half, from + 1024, &A[S][wave * 2048 + 1024]);
+        load_to_lds<DIRECT>(half, from, &A[S][wave * 2048]);
+        load_to_lds<DIRECT>(half, from + 1024, &A[S][wave * 2048 + 1024]);
     };
     auto issue = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
@@ -737,7 +755,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 #pragma unroll
         for (int j = 0; j < NU; j++)
             if constexpr (DIRECT) {
-                load_to_lds(ys, near * 2 + (j * 32 * lddy + r) * 2, &Y[S][0][(j * 32 + wave * 8) * 128]);
+                load_to_lds<true>(ys, near * 2 + (j * 32 * lddy + r) * 2, &Y[S][0][(j * 32 + wave * 8) * 128]);
             } else {
                 __builtin_memcpy(yr[j].v, ybase + r + at[j], sizeof yr[j].v);
             }
@@ -749,11 +767,12 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 #pragma unroll
         for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[slot][p][(j * 32 + wave * 8) * 128 + lane * 16] = part[p];
     };
-    // `between` runs after the first reads from LDS: the next stage's loads, which take a while to issue.  With few tiles all
-    // reads come first; with 8 those of the first half of the rows, then one tile ahead and no more.
+    // `between` runs after the first reads from LDS: the next stage's loads, which take a while to issue.  All reads of the block
+    // come before it -- the compiler cannot tell what a transposing read touches, and one behind the direct loads would wait
+    // for them -- and with few tiles those of dy; with many, one tile ahead and no more.
     auto compute = [&](auto slot, auto between) {
         constexpr int S = decltype(slot)::value;
-        constexpr bool ALL = NU < 8;
+        constexpr bool ALL = PARTS * NU <= 4;
         auto read_a = [&](int h, int s) {
             // row 32 h + 8 q + w, w = i >> 1, columns 8 (i & 1) .. + 7 of a subtile
             const int strip = (2 * q + (i >> 3)) & 3, quad = 2 * h + (q >> 1);
@@ -767,13 +786,14 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         i32x2 w[2][4];
         bf16x8 b[2][PARTS][NU];
 #pragma unroll
-        for (int h = 0; h < (ALL ? 2 : 1); h++) {
+        for (int h = 0; h < 2; h++) {
 #pragma unroll
             for (int s = 0; s < 4; s++) w[h][s] = read_a(h, s);
+            if (ALL || h == 0)
 #pragma unroll
-            for (int part = 0; part < PARTS; part++)
+                for (int part = 0; part < PARTS; part++)
 #pragma unroll
-                for (int u = 0; u < (ALL ? NU : 1); u++) b[h][part][u] = read_b(h, part, u);
+                    for (int u = 0; u < (ALL ? NU : 1); u++) b[h][part][u] = read_b(h, part, u);
         }
         const float fa = scale_value(sa[S]);
         between();
@@ -782,8 +802,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
             if constexpr (!ALL)
                 if (h == 1) {
 #pragma unroll
-                    for (int s = 0; s < 4; s++) w[1][s] = read_a(1, s);
-                    b[1][0][0] = read_b(1, 0, 0);
+                    for (int part = 0; part < PARTS; part++) b[1][part][0] = read_b(1, part, 0);
                 }
             bf16x8 a[4];
 #pragma unroll
@@ -798,12 +817,15 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
                     if constexpr (!ALL) if (u + 1 < NU) b[h][part][u + 1] = read_b(h, part, u + 1);
 #pragma unroll
                     for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[h][part][u], acc[u][s], 0, 0, 0);
-                    if (!ALL && (u & 1)) __builtin_amdgcn_sched_barrier(0);
+                    if (NU == 8 && (u & 1)) __builtin_amdgcn_sched_barrier(0);
                 }
         }
     };
     auto step = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
+        here(id);
+        here(row);
+        here(scale);
         stage_barrier<DIRECT ? (R - 2) * (2 + NU) : 0>();
         compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
         if constexpr (!DIRECT)
