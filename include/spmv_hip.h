@@ -382,7 +382,7 @@ int spmv_hip_dist_free(spmv_hip_dist *d);
  *
  * All calls are asynchronous on `stream`, allocate nothing and may be captured
  * into a graph; they keep nothing in the handle, so that products on one handle
- * may overlap.  n = 0 is allowed.  spmv_hip_mult, _mult_dev, _mult_mv, _mult_mv_dev
+ * may overlap.  Vectors of dy are less than 2^23 entries apart.  n = 0 is allowed.  spmv_hip_mult, _mult_dev, _mult_mv, _mult_mv_dev
  * and _bench take such a handle too (dtype F32): x is rounded to 8 bits on its way
  * in.  "variant", "block_map" and "hot_columns" do not apply. */
 
@@ -413,16 +413,20 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
 enum { SPMV_HIP_BLOCK8_MAX_WIDE = 64 };
 int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, int x_dtype, int64_t ldx,
                              const uint8_t *d_scale, int64_t lds, void *d_y, int y_dtype, int64_t ldy, void *stream);
-/* dx_v = A^T dy_v: the gradient of the product's input.  dy and dx in F32, BF16 or
- * F16; dy is used as it is, not rounded to 8 bits. */
-int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, void *d_dx,
-                               int dx_dtype, int64_t lddx, void *stream);
-/* The gradient of the stored blocks: d_dvalues[k][r][c] = sum over v of
- * dy_v[128 I_k + r] * x_v[128 J_k + c], x as its 8-bit checkpoint; zero beyond the
- * matrix's edge.  accumulate != 0 adds to what d_dvalues holds. */
-int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
-                                 const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dvalues,
-                                 int dtype, int accumulate, void *stream);
+/* The two gradients of the product, from dy (F32, BF16 or F16, used as it is, not
+ * rounded to 8 bits); either may be left out with NULL.
+ *   dx_v = A^T dy_v: the gradient of x, in F32, BF16 or F16
+ *   d_dvalues[k][r][c] = sum over v of dy_v[128 I_k + r] * x_v[128 J_k + c]: the
+ *     gradient of the stored blocks (I_k, J_k = block k's row and column), x as its
+ *     8-bit checkpoint (needed for this one only); zero beyond the matrix's edge.
+ *     accumulate != 0 adds to what d_dvalues holds.
+ * d_work: spmv_hip_block8_backward_work() bytes of device memory, 16-byte aligned,
+ * scratch for this call (NULL if that is 0: bf16 vectors at 16-byte aligned
+ * addresses, or bf16 and no dx).  with_dx: whether dx is asked for. */
+int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx);
+int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
+                                 const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dx, int dx_dtype,
+                                 int64_t lddx, void *d_dvalues, int dv_dtype, int accumulate, void *d_work, void *stream);
 
 /* free_X (csr.c:205-210, sellp.c:461-465; the reference leaks the others) */
 int spmv_hip_free(spmv_hip_matrix *m);

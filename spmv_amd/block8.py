@@ -220,18 +220,15 @@ class Block8(Matrix):
 
     def product_t(self, dy: torch.Tensor, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """dx[..., columns] = A^T dy for dy [..., rows]; dy is not rounded."""
-        d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
-        self._here("dy", d)
+        d = self._dy(dy)
         dx = self._out(out, (*dy.shape[:-1], self.columns), dtype or d.dtype, d)
-        L.check(L.lib().spmv_hip_block8_mult_t_dev(self._h, d.shape[0], d.data_ptr(), _DTYPE[d.dtype], _ld(d), dx.data_ptr(),
-                                                   _DTYPE[dx.dtype], self.columns, _raw_stream(self._index)))
+        self._backward(d, None, dx, None, False)
         return dx
 
     def gradient(self, dy: torch.Tensor, x: Packed8, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
                  accumulate: bool = False) -> torch.Tensor:
         """The gradient of the stored blocks [blocks, 128, 128] from dy [..., rows] and the 8-bit x of the product."""
-        d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
-        self._here("dy", d)
+        d = self._dy(dy)
         if not isinstance(x, Packed8):
             raise TypeError("x must be a Packed8 (quantize)")
         if x.columns != self.columns or x.n != d.shape[0]:
@@ -240,10 +237,27 @@ class Block8(Matrix):
         if accumulate and out is None:
             raise ValueError("accumulate adds to out, which is missing")
         dv = self._out(out, (self.nblocks, BLOCK, BLOCK), out.dtype if out is not None else dtype, d)
-        L.check(L.lib().spmv_hip_block8_gradient_dev(self._h, d.shape[0], d.data_ptr(), _DTYPE[d.dtype], _ld(d), x.values.data_ptr(),
-                                                     x.values.shape[1], x.scale.data_ptr(), x.n, dv.data_ptr(), _DTYPE[dv.dtype],
-                                                     int(accumulate), _raw_stream(self._index)))
+        self._backward(d, x, None, dv, accumulate)
         return dv
+
+    def _dy(self, dy) -> torch.Tensor:
+        d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
+        self._here("dy", d)
+        return d
+
+    def _backward(self, d, x, dx, dv, accumulate) -> None:
+        """dx and dv, either None, from checked operands."""
+        lib, n, ld = L.lib(), d.shape[0], _ld(d)
+        p, t, work = d.data_ptr(), _DTYPE[d.dtype], None
+        size = lib.spmv_hip_block8_backward_work(self._h, n, p, t, ld, dx is not None)
+        if size:
+            work = torch.empty(size, dtype=torch.uint8, device=self.device)
+        L.check(lib.spmv_hip_block8_backward_dev(
+            self._h, n, p, t, ld,
+            *((x.values.data_ptr(), x.values.shape[1], x.scale.data_ptr(), x.n) if dv is not None else (None, 0, None, 0)),
+            *((dx.data_ptr(), _DTYPE[dx.dtype], self.columns) if dx is not None else (None, 0, 0)),
+            *((dv.data_ptr(), _DTYPE[dv.dtype]) if dv is not None else (None, 0)), accumulate,
+            work.data_ptr() if work is not None else None, _raw_stream(self._index)))
 
     def linear(self, x: torch.Tensor) -> torch.Tensor:
         """y = A x, differentiable in x and in the tensor that set_values took.  Between the passes x is kept in 8 bits;
@@ -273,8 +287,10 @@ class _Linear(torch.autograd.Function):
         matrix = ctx.matrix
         if matrix._version != ctx.version:
             raise RuntimeError("the values of the 8-bit matrix were set again between forward and backward")
-        dx = matrix.product_t(dy, ctx.x_dtype) if ctx.needs_input_grad[0] else None
+        d = matrix._dy(dy)
+        dx = torch.empty(ctx.x_shape, dtype=ctx.x_dtype, device=d.device) if ctx.needs_input_grad[0] else None
         dv = None
         if ctx.needs_input_grad[1]:
-            dv = matrix.gradient(dy, Packed8._made(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), ctx.values_dtype)
+            dv = torch.empty((matrix.nblocks, BLOCK, BLOCK), dtype=ctx.values_dtype, device=d.device)
+        matrix._backward(d, Packed8._made(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), dx, dv, False)
         return dx, dv, None

@@ -660,49 +660,63 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
         if (v0 + u < g.n && r < g.rows) store_row<OT, 4>(y + (int64_t)(v0 + u) * g.ldy + r, g.rows - r, acc[u]);
 }
 
-// dy is used as it is: split into PARTS bf16 numbers that add up to it exactly (1 for bf16, 2 for fp16, 3 for fp32:
-// each holds 8 bits of the mantissa), one matrix instruction each
+// dy is used as it is: as PARTS bf16 numbers that add up to it exactly (1 for bf16, 2 for fp16, 3 for fp32: each holds 8
+// bits of the mantissa), one matrix instruction each
 template <typename DT> struct parts_of { static constexpr int value = 1; };
 template <> struct parts_of<_Float16> { static constexpr int value = 2; };
 template <> struct parts_of<float> { static constexpr int value = 3; };
 
-template <int PARTS> __device__ __forceinline__ void split1(float f, __bf16 *part, int stride)
+static int parts(int dtype) { return dtype == SPMV_HIP_BF16 ? 1 : dtype == SPMV_HIP_F16 ? 2 : 3; }
+
+// dy into its parts, `plane` entries apart, vectors `ld` apart (a multiple of 128), zero past `length`; 8 entries a
+// thread.  Before the products rather than in them: there the splitting stood between loads and matrix instructions of
+// every step (fp32, 333 vectors, 264 blocks: 41 us, now 4 + 14).
+template <typename T>
+__global__ __launch_bounds__(kBlock) void split_kernel(int n, int length, int ld, const T *__restrict__ dy, int64_t lddy,
+                                                       __bf16 *__restrict__ out, int64_t plane)
 {
-    const bool finite = fabsf(f) < __builtin_inff();         // infinities and NaN: all in the first
+    constexpr int PARTS = parts_of<T>::value;
+    const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+    if (at >= plane) return;
+    const int64_t v = at / ld;
+    const int c = (int)(at % ld);
+    Raw<T, 8> r;
+    r.load(dy + v * lddy + c, length - c);
+    bf16x8 part[PARTS];
+    if constexpr (PARTS == 1) __builtin_memcpy(&part[0], r.v, 16);
+    else
 #pragma unroll
-    for (int p = 0; p < PARTS; p++) {
-        part[p * stride] = (__bf16)f;
-        f -= (float)part[p * stride];
-        if (p == 0) f = finite ? f : 0.0f;
-    }
+        for (int e = 0; e < 8; e++) {
+            float f = (float)r.v[e];
+            const bool finite = fabsf(f) < __builtin_inff(); // infinities and NaN: all in the first
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) {
+                part[p][e] = (__bf16)f;
+                f = finite ? f - (float)part[p][e] : 0.0f;
+            }
+        }
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) *(bf16x8 *)(out + p * plane + at) = part[p];
 }
 
 struct TransposedArgs {
     int n, rows, columns, bcols, vtiles;
     const int *ptr, *row, *id, *scale;               // lists by block column, their blocks' scales
     const uint8_t *val8;
-    int64_t lddy, lddx;
+    const __bf16 *dy;
+    int64_t lddy, plane, lddx;     // plane: from one part of dy to the next
 };
-
-// 8 entries of dy as PARTS operands
-template <typename DT> __device__ __forceinline__ void operands8(const Raw<DT, 8> &r, bf16x8 *part)
-{
-    if constexpr (parts_of<DT>::value == 1) __builtin_memcpy(part, r.v, 16);
-    else
-#pragma unroll
-        for (int e = 0; e < 8; e++) split1<parts_of<DT>::value>((float)r.v[e], (__bf16 *)part + e, 8);
-}
 
 // dx = A^T dy, half a block (64 rows) a step, blocks and vectors through LDS.  ds_read_b64_tr_b8 hands every lane one
 // column of 8 rows of the block, widened to bf16 (exact) on the way to the matrix instruction.  8 rows of dy are 4 rows in
 // each of two strips of the block (block8_offset); in LDS the 4-row pieces of a 16 x 16 subtile are exchanged by XOR
-// with the strip, which puts the two on different banks.  DIRECT (bf16, rows of dy 16-byte aligned): dy goes to LDS by
-// direct loads, otherwise through registers, which take any alignment and split it.  The blocks of a last block row that is
-// not whole come last in every list: they are taken after the others, one by one, with the entries past the end masked.
-template <typename DT, bool DIRECT, int NU, typename OT>
-__global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g, const DT *__restrict__ dy, OT *__restrict__ dx)
+// with the strip, which puts the two on different banks.  The blocks of a last block row that is not whole come last in
+// every list: they are taken after the others, one by one, with the entries past the end masked (dy in parts is padded
+// and has no such rows).
+template <int PARTS, int NU, typename OT>
+__global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g, OT *__restrict__ dx)
 {
-    constexpr int PARTS = parts_of<DT>::value, R = !DIRECT || NU == 8 ? 2 : NU == 4 ? 3 : 4, TOK = 32 * NU;
+    constexpr int R = PARTS * NU >= 6 ? 2 : PARTS * NU == 4 ? 3 : 4, TOK = 32 * NU;
     __shared__ uint8_t Y[R][PARTS][TOK * 128];
     __shared__ uint8_t A[R][kBlockBytes / 2];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), i = lane & 15, q = lane >> 4;
@@ -712,7 +726,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
     const int t0 = vtile * TOK;
     const int begin = table(g.ptr, major), end = table(g.ptr, major + 1);
     int whole = end;
-    if (g.rows % kB)
+    if (PARTS == 1 && g.rows % kB)
         while (whole > begin && table(g.row, whole - 1) == g.rows / kB) whole--;
     const int first = 2 * begin, last = 2 * whole;
     f32x4 acc[NU][4];
@@ -723,16 +737,13 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 
     // piece j of a thread: 8 entries of vector 32 j + 8 wave + lane / 8, in place lane % 8 of its row in LDS; a
     // row's pieces are exchanged by XOR.  Past the last vector: the last, its result is not stored.
-    const DT *ybase = dy + (int64_t)t0 * g.lddy;
+    const __bf16 *ybase = g.dy + (int64_t)t0 * g.lddy;
     const int row_of_lane = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((row_of_lane >> 1) & 7);
     const unsigned lddy = (unsigned)g.lddy, near = row_of_lane * lddy + 8 * piece;
-    const u32x4 ys = buffer(ybase, (unsigned)min(g.n - t0, TOK) * lddy * (unsigned)sizeof(DT));      // DIRECT
-    unsigned at[DIRECT ? 1 : NU];
-    if constexpr (!DIRECT)
+    u32x4 ys[PARTS];
 #pragma unroll
-        for (int j = 0; j < NU; j++) at[j] = (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * lddy + 8 * piece;
+    for (int p = 0; p < PARTS; p++) ys[p] = buffer(ybase + p * g.plane, (unsigned)min(g.n - t0, TOK) * lddy * 2);
 
-    Raw<DT, 8> yr[DIRECT ? 1 : NU];
     int sa[R], id = 0, row = 0, scale = 0;                   // id, row, scale: of the half block issued next, loaded a step before
     auto look_up = [&](int k) {
         id = table(g.id, k >> 1);
@@ -745,27 +756,18 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         sa[S] = scale;
         // wave w brings strip w: 2 x 4 subtiles of 256 bytes
         const int from = wave * 2048 + q * 256 + ((i ^ (wave << 2)) << 4);
-        load_to_lds<DIRECT>(half, from, &A[S][wave * 2048]);
-        load_to_lds<DIRECT>(half, from + 1024, &A[S][wave * 2048 + 1024]);
+        load_to_lds<true>(half, from, &A[S][wave * 2048]);
+        load_to_lds<true>(half, from + 1024, &A[S][wave * 2048 + 1024]);
     };
     auto issue = [&](auto slot, int k) {
         constexpr int S = decltype(slot)::value;
         issue_block(slot, k);
         const unsigned r = row * kB + (k & 1) * 64;
 #pragma unroll
-        for (int j = 0; j < NU; j++)
-            if constexpr (DIRECT) {
-                load_to_lds<true>(ys, near * 2 + (j * 32 * lddy + r) * 2, &Y[S][0][(j * 32 + wave * 8) * 128]);
-            } else {
-                __builtin_memcpy(yr[j].v, ybase + r + at[j], sizeof yr[j].v);
-            }
-        look_up(min(k + 1, last - 1));
-    };
-    auto put = [&](int slot, const Raw<DT, 8> &r, int j) {
-        bf16x8 part[PARTS];
-        operands8(r, part);
+        for (int p = 0; p < PARTS; p++)
 #pragma unroll
-        for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[slot][p][(j * 32 + wave * 8) * 128 + lane * 16] = part[p];
+            for (int j = 0; j < NU; j++) load_to_lds<true>(ys[p], near * 2 + (j * 32 * lddy + r) * 2, &Y[S][p][(j * 32 + wave * 8) * 128]);
+        look_up(min(k + 1, last - 1));
     };
     // `between` runs after the first reads from LDS: the next stage's loads, which take a while to issue.  All reads of the block
     // come before it -- the compiler cannot tell what a transposing read touches, and one behind the direct loads would wait
@@ -826,18 +828,12 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         here(id);
         here(row);
         here(scale);
-        stage_barrier<DIRECT ? (R - 2) * (2 + NU) : 0>();
+        stage_barrier<(R - 2) * (2 + PARTS * NU)>();
         compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
-        if constexpr (!DIRECT)
-#pragma unroll
-            for (int j = 0; j < NU; j++) put((S + 1) % R, yr[j], j);
     };
     if (first < last) {
         look_up(first);
         issue(ic<0>(), first);
-        if constexpr (!DIRECT)
-#pragma unroll
-            for (int j = 0; j < NU; j++) put(0, yr[j], j);
         if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
         if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
         ring<R>(first, last, step);
@@ -848,9 +844,9 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         issue_block(ic<0>(), k);
         const int r = row * kB + (k & 1) * 64;
         for (int j = 0; j < NU; j++) {
-            Raw<DT, 8> one;
-            one.load(ybase + r + (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * (unsigned)g.lddy + 8 * piece, g.rows - (r + 8 * piece));
-            put(0, one, j);
+            Raw<__bf16, 8> one;
+            one.load(ybase + r + (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * lddy + 8 * piece, g.rows - (r + 8 * piece));
+            __builtin_memcpy(&Y[0][0][(j * 32 + wave * 8) * 128 + lane * 16], one.v, 16);
         }
         stage_barrier<0>();
         compute(ic<0>(), [] {});
@@ -869,11 +865,12 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 }
 
 struct GradientArgs {
-    int n, rows, columns, accumulate;
+    int n, rows, edge, columns, accumulate;      // rows of dy, and the matrix's; dy in parts is padded with zeros
     const int *list;               // NB blocks of one block row per workgroup, -1 = none
     const int *block_row, *block_col;
     const uint8_t *x8, *xscale;
-    int64_t ldx8, lds, lddy;
+    const __bf16 *dy;
+    int64_t ldx8, lds, lddy, plane;
 };
 
 // dA = dy^T x at the stored blocks, 32 vectors a step.  With NB = 2 a workgroup has two blocks of one block row, a wave
@@ -882,10 +879,10 @@ struct GradientArgs {
 // vectors).  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane: widened there with
 // the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane i's columns are
 // 4 i + s: its results are 16 neighbours.
-template <typename DT, int NB, typename OT>
-__global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, const DT *__restrict__ dy, OT *__restrict__ dv)
+template <int PARTS, int NB, typename OT>
+__global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT *__restrict__ dv)
 {
-    constexpr int PARTS = parts_of<DT>::value, STEP = 32, NU = 4 * NB, R = NB == 2 ? 2 : 4;
+    constexpr int STEP = 32, NU = 4 * NB, R = NB == 2 ? 2 : PARTS == 3 ? 3 : 4;
     __shared__ uint8_t Y[2][PARTS][kB * STEP * 2];           // [row][32 vectors], 16-byte pieces exchanged by XOR
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
     const int wg = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
@@ -899,7 +896,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
 #pragma unroll
         for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    Raw<DT, 2> yr[R][8];
+    unsigned yr[R][PARTS][8];                                // two rows of 8 vectors
     unsigned xr[R][8];
     uint64_t sx[R];
     // A lane's two rows of dy are r and r + 1, loaded from rp, which moves back where they run past the last row: then its
@@ -910,25 +907,32 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
     auto fetch = [&](auto slot, int t0) {                    // 32 whole vectors, two rows or more
         constexpr int S = decltype(slot)::value;
         const uint8_t *xp = g.x8 + (int64_t)t0 * g.ldx8 + col * kB + c0;
-        const DT *yp = dy + (int64_t)(t0 + 8 * wave) * g.lddy;
+        const __bf16 *yp = g.dy + (int64_t)(t0 + 8 * wave) * g.lddy;
 #pragma unroll
         for (int w = 0; w < 8; w++) xr[S][w] = *(const unsigned *)(xp + w * g.ldx8 + xat);
         __builtin_memcpy(&sx[S], g.xscale + (int64_t)col * g.lds + t0 + 8 * q, 8);
 #pragma unroll
-        for (int w = 0; w < 8; w++) __builtin_memcpy(yr[S][w].v, yp + w * g.lddy + (unsigned)rp, sizeof yr[S][w].v);
+        for (int p = 0; p < PARTS; p++)
+#pragma unroll
+            for (int w = 0; w < 8; w++) __builtin_memcpy(&yr[S][p][w], yp + p * g.plane + w * g.lddy + (unsigned)rp, 4);
     };
     // the vectors after the last whole 32; past the last dy is zero, and x the last one's, so that nothing new that is not
     // finite comes in
     auto fetch_rest = [&](int t0) {
         const uint8_t *xp = g.x8 + (int64_t)t0 * g.ldx8 + col * kB + c0 + 4 * i;
-        const DT *yp = dy + (int64_t)t0 * g.lddy + rp;
+        const __bf16 *yp = g.dy + (int64_t)t0 * g.lddy + rp;
         const uint8_t *sp = g.xscale + (int64_t)col * g.lds + t0;
         const int top = g.n - 1 - t0;
         sx[0] = 0;
 #pragma unroll
         for (int w = 0; w < 8; w++) {
             const int ty = 8 * wave + w, tx = 8 * q + w;
-            yr[0][w].load(yp + (int64_t)min(ty, top) * g.lddy, ty <= top ? min(g.rows, 2) : 0);
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) {
+                Raw<__bf16, 2> two;
+                two.load(yp + p * g.plane + (int64_t)min(ty, top) * g.lddy, ty <= top ? min(g.rows, 2) : 0);
+                __builtin_memcpy(&yr[0][p][w], two.v, 4);
+            }
             xr[0][w] = *(const unsigned *)(xp + (int64_t)min(tx, top) * g.ldx8);
             sx[0] |= (uint64_t)sp[min(tx, top)] << (8 * w);
         }
@@ -940,27 +944,14 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
         constexpr int S = decltype(slot)::value;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            bf16x8 part[PARTS];
-            if constexpr (PARTS == 1) {
-                unsigned v[4];
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    unsigned two[2];
-                    __builtin_memcpy(&two[0], yr[S][2 * w].v, 4);
-                    __builtin_memcpy(&two[1], yr[S][2 * w + 1].v, 4);
-                    v[w] = __builtin_amdgcn_perm(two[1], two[0], pick[k]);
-                }
-                __builtin_memcpy(&part[0], v, 16);
-            } else {
-#pragma unroll
-                for (int w = 0; w < 8; w++) {
-                    const float f = natural ? (float)yr[S][w].v[k] : shifted && k == 0 ? (float)yr[S][w].v[1] : 0.0f;
-                    split1<PARTS>(f, (__bf16 *)&part[0] + w, 8);
-                }
-            }
             const int row = 2 * lane + k;
 #pragma unroll
-            for (int p = 0; p < PARTS; p++) *(bf16x8 *)&Y[buf][p][row * 64 + ((wave ^ ((row >> 1) & 3)) << 4)] = part[p];
+            for (int p = 0; p < PARTS; p++) {
+                u32x4 v;
+#pragma unroll
+                for (int w = 0; w < 4; w++) v[w] = __builtin_amdgcn_perm(yr[S][p][2 * w + 1], yr[S][p][2 * w], pick[k]);
+                *(u32x4 *)&Y[buf][p][row * 64 + ((wave ^ ((row >> 1) & 3)) << 4)] = v;
+            }
         }
     };
     auto compute = [&](auto slot, int buf, auto between) {
@@ -1025,7 +1016,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, con
     for (int u = 0; u < NU; u++) {
         const int row = n0 + 16 * u + i;
         OT *o = dv + (int64_t)id * kBlockBytes + row * kB + c0 + 16 * q;
-        const int left = row0 + row < g.rows ? g.columns - (col * kB + c0 + 16 * q) : 0;
+        const int left = row0 + row < g.edge ? g.columns - (col * kB + c0 + 16 * q) : 0;
         f32x4 v[4];
 #pragma unroll
         for (int k = 0; k < 16; k++) {
@@ -1347,84 +1338,107 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     return launched(what);
 }
 
-int spmv_hip_block8_mult_t_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, void *d_dx,
-                               int dx_dtype, int64_t lddx, void *stream)
+// whether dy goes into the products as it lies: bf16, and for dx with 16-byte aligned vectors
+static bool as_it_lies(int n, const void *d_dy, int dtype, int64_t lddy, bool with_dx)
 {
-    const char *what = "block8_mult_t";
+    return dtype == SPMV_HIP_BF16 && (!with_dx || ((uintptr_t)d_dy % 16 == 0 && (n == 1 || lddy % 8 == 0)));
+}
+
+int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx)
+{
+    if (!m || m->format != SPMV_HIP_BLOCK8 || n <= 0 || !wide_dtype(dy_dtype) || as_it_lies(n, d_dy, dy_dtype, lddy, with_dx != 0)) return 0;
+    return (int64_t)parts(dy_dtype) * n * m->brows * kB * 2;
+}
+
+int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
+                                 const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dx, int dx_dtype,
+                                 int64_t lddx, void *d_dvalues, int dv_dtype, int accumulate, void *d_work, void *stream)
+{
+    const char *what = "block8_backward";
     if (check_block8(what, m)) return 1;
     if (!wide_dtype(dy_dtype)) return bad_dtype(what, dy_dtype);
-    if (!wide_dtype(dx_dtype)) return bad_dtype(what, dx_dtype);
-    if (check_vectors(what, n, d_dy, lddy, m->rows) || check_vectors(what, n, d_dx, lddx, m->columns)) return 1;
+    if (check_vectors(what, n, d_dy, lddy, m->rows)) return 1;
     if (n > 1 && lddy >= (int64_t)1 << 23) {                  // 256 of them stay inside 32-bit offsets
         set_error("%s: vectors %lld apart, at most 2^23 - 1", what, (long long)lddy);
         return 1;
     }
-    if (n == 0 || m->columns == 0) return 0;
+    if (d_dx) {
+        if (!wide_dtype(dx_dtype)) return bad_dtype(what, dx_dtype);
+        if (check_vectors(what, n, d_dx, lddx, m->columns)) return 1;
+    }
+    if (d_dvalues) {
+        if (!wide_dtype(dv_dtype)) return bad_dtype(what, dv_dtype);
+        if (check_eight(what, n, m->columns, d_x8, ldx8, d_scale, lds)) return 1;
+    }
+    const bool split = n > 0 && m->rows > 0 && !as_it_lies(n, d_dy, dy_dtype, lddy, d_dx != nullptr);
+    if (split && !d_work) {
+        set_error("%s: NULL workspace, %lld bytes needed", what, (long long)spmv_hip_block8_backward_work(m, n, d_dy, dy_dtype, lddy, d_dx != nullptr));
+        return 1;
+    }
+    if (split && (uintptr_t)d_work % 16) { set_error("%s: workspace is not 16-byte aligned", what); return 1; }
+    if (!d_dx && !d_dvalues) return 0;
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
-    TransposedArgs a{};
-    a.n = n; a.rows = m->rows; a.columns = m->columns; a.bcols = m->bcols;
-    a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale = m->d_bt_scale8;
-    a.lddy = lddy; a.lddx = lddx;
-    const int nu = vector_tiles(m, m->bcols, n, dy_dtype == SPMV_HIP_BF16 ? 8 : 4);
-    a.vtiles = (n + 32 * nu - 1) / (32 * nu);
-    const bool direct = dy_dtype == SPMV_HIP_BF16 && (uintptr_t)d_dy % 16 == 0 && lddy % 8 == 0;
-    if (check_tiles(what, m->bcols, a.vtiles)) return 1;
-    with_elem(dy_dtype, [&](auto t) {
-        typedef decltype(t) T;
+    const hipStream_t st = (hipStream_t)stream;
+    const __bf16 *dy = (const __bf16 *)d_dy;
+    int rows = m->rows;
+    int64_t plane = 0;
+    if (split) {
+        rows = m->brows * kB;
+        plane = (int64_t)n * rows;
+        if (plane / 8 > (int64_t)0x7fffffff * kBlock || rows >= 1 << 23) { set_error("%s: %d vectors of %d are more than one launch takes", what, n, m->rows); return 1; }
+        with_elem(dy_dtype, [&](auto t) {
+            typedef decltype(t) T;
+            hipLaunchKernelGGL(split_kernel<T>, dim3((unsigned)((plane / 8 + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, n, m->rows, rows,
+                               (const T *)d_dy, lddy, (__bf16 *)d_work, plane);
+        });
+        dy = (const __bf16 *)d_work;
+        lddy = rows;
+    }
+    const int count = parts(dy_dtype);
+    auto with_parts = [&](auto f) {
+        if (count == 1) f(ic<1>());
+        else if (count == 2) f(ic<2>());
+        else f(ic<3>());
+    };
+    if (d_dx && n > 0 && m->columns > 0) {
+        TransposedArgs a{};
+        a.n = n; a.rows = rows; a.columns = m->columns; a.bcols = m->bcols;
+        a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale = m->d_bt_scale8;
+        a.dy = dy; a.lddy = lddy; a.plane = plane; a.lddx = lddx;
+        const int nu = vector_tiles(m, m->bcols, n, count == 1 ? 8 : 4);
+        a.vtiles = (n + 32 * nu - 1) / (32 * nu);
+        if (check_tiles(what, m->bcols, a.vtiles)) return 1;
         with_elem(dx_dtype, [&](auto o) {
             typedef decltype(o) O;
-            auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles), dim3(kBlock), 0, (hipStream_t)stream, a, (const T *)d_dy, (O *)d_dx);
-            };
-            if constexpr (std::is_same<T, __bf16>::value) {
-                if (direct) {
-                    if (nu == 8) go(transposed_kernel<T, true, 8, O>);
-                    else if (nu == 4) go(transposed_kernel<T, true, 4, O>);
-                    else go(transposed_kernel<T, true, 2, O>);
-                    return;
-                }
-                if (nu == 8) { go(transposed_kernel<T, false, 8, O>); return; }
-            }
-            if (nu == 4) go(transposed_kernel<T, false, 4, O>);
-            else go(transposed_kernel<T, false, 2, O>);
+            with_parts([&](auto p) {
+                constexpr int P = decltype(p)::value;
+                auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles), dim3(kBlock), 0, st, a, (O *)d_dx); };
+                if constexpr (P == 1) if (nu == 8) { go(transposed_kernel<P, 8, O>); return; }
+                if (nu == 4) go(transposed_kernel<P, 4, O>);
+                else go(transposed_kernel<P, 2, O>);
+            });
         });
-    });
-    return launched(what);
-}
-
-int spmv_hip_block8_gradient_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
-                                 const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dvalues,
-                                 int dtype, int accumulate, void *stream)
-{
-    const char *what = "block8_gradient";
-    if (check_block8(what, m)) return 1;
-    if (!wide_dtype(dy_dtype)) return bad_dtype(what, dy_dtype);
-    if (!wide_dtype(dtype)) return bad_dtype(what, dtype);
-    if (check_vectors(what, n, d_dy, lddy, m->rows) || check_eight(what, n, m->columns, d_x8, ldx8, d_scale, lds)) return 1;
-    if (m->nblocks == 0) return 0;
-    if (!d_dvalues) { set_error("%s: NULL gradient", what); return 1; }
-    DeviceGuard on(m->device);
-    if (!on.ok) return 1;
-    GradientArgs a{};
-    a.n = n; a.rows = m->rows; a.columns = m->columns; a.accumulate = accumulate;
-    a.block_row = m->d_block_row; a.block_col = m->d_block_col;
-    a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.lddy = lddy;
-    // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the registers
-    // and not where many pairs lack their second block
-    const bool pairs = dy_dtype == SPMV_HIP_BF16 && m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
-    a.list = pairs ? m->d_pair : m->d_order;
-    with_elem(dy_dtype, [&](auto t) {
-        typedef decltype(t) T;
-        with_elem(dtype, [&](auto o) {
+    }
+    if (d_dvalues && m->nblocks > 0) {
+        GradientArgs a{};
+        a.n = n; a.rows = rows; a.edge = m->rows; a.columns = m->columns; a.accumulate = accumulate;
+        a.block_row = m->d_block_row; a.block_col = m->d_block_col;
+        a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.dy = dy; a.lddy = lddy; a.plane = plane;
+        // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
+        // registers; and not where many pairs lack their second block
+        const bool pairs = count == 1 && m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
+        a.list = pairs ? m->d_pair : m->d_order;
+        with_elem(dv_dtype, [&](auto o) {
             typedef decltype(o) O;
-            auto go = [&](auto kernel, int count) {
-                hipLaunchKernelGGL(kernel, dim3(count), dim3(kBlock), 0, (hipStream_t)stream, a, (const T *)d_dy, (O *)d_dvalues);
-            };
-            if constexpr (std::is_same<T, __bf16>::value) if (pairs) { go(gradient_kernel<T, 2, O>, m->npairs); return; }
-            go(gradient_kernel<T, 1, O>, m->nblocks);
+            with_parts([&](auto p) {
+                constexpr int P = decltype(p)::value;
+                auto go = [&](auto kernel, int wgs) { hipLaunchKernelGGL(kernel, dim3(wgs), dim3(kBlock), 0, st, a, (O *)d_dvalues); };
+                if constexpr (P == 1) if (pairs) { go(gradient_kernel<P, 2, O>, m->npairs); return; }
+                go(gradient_kernel<P, 1, O>, m->nblocks);
+            });
         });
-    });
+    }
     return launched(what);
 }
 

@@ -83,10 +83,11 @@ def test_vector_calls_refuse_bad_arguments():
     _fails(r(ldx=3), "shorter than their length")
     _fails(r(ld8=255), "multiple of 128")
     assert q(n=0) == 0 and r(n=0) == 0 and q(cols=0) == 0    # nothing to do
-    for name, args in (("mult", (None, 1, p, S.F32, 9, None, 0, p, S.F32, 9, None)), ("mult_t", (None, 1, p, S.F32, 9, p, S.F32, 9, None)),
-                       ("gradient", (None, 1, p, S.F32, 9, p, 128, p, 1, p, S.F32, 0, None)), ("set_values", (None, p, S.F32, None)),
+    for name, args in (("mult", (None, 1, p, S.F32, 9, None, 0, p, S.F32, 9, None)), ("backward", (None, 1, p, S.F32, 9, p, 128, p, 1, p, S.F32, 9, p, S.F32, 0, p, None)),
+                       ("set_values", (None, p, S.F32, None)),
                        ("load", (None, p, p, None)), ("store", (None, p, p, None))):
         _fails(getattr(L, f"spmv_hip_block8_{name}_dev")(*args), "NULL handle")
+    assert L.spmv_hip_block8_backward_work(None, 1, p, S.F32, 9, 1) == 0
 
 
 def test_python_layer_refuses_what_is_not_on_a_gpu():

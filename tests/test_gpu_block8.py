@@ -156,13 +156,17 @@ def test_abi_strides_leave_the_gaps_alone():
         assert torch.all(y[:, 260:] == -5.0) and torch.all(y[k:] == -5.0)
     dy = _vectors(n, 277, F16, 2)
     dx = torch.full((n, 301), -5.0, device=DEV)
-    S.check(L.spmv_hip_block8_mult_t_dev(c.A._h, n, dy.data_ptr(), S.F16, 277, dx.data_ptr(), S.F32, 301, st))
+    assert L.spmv_hip_block8_backward_work(c.A._h, n, dy.data_ptr(), S.F16, 277, 1) == 2 * n * 384 * 2
+    work = torch.zeros(2 * n * 384 * 2 + 16, dtype=torch.uint8, device=DEV)
+    args = (c.A._h, n, dy.data_ptr(), S.F16, 277)
+    S.check(L.spmv_hip_block8_backward_dev(*args, None, 0, None, 0, dx.data_ptr(), S.F32, 301, None, 0, 0, work.data_ptr(), st))
     d = _np(dy)[:, :260]
     _close(dx[:, :columns], _mat(d, c.dense), 260, _mat(np.abs(d), c.dense_abs))
     assert torch.all(dx[:, columns:] == -5.0)
     dv = torch.full((c.A.nblocks + 1, 128, 128), -5.0, device=DEV)
-    S.check(L.spmv_hip_block8_gradient_dev(c.A._h, n, dy.data_ptr(), S.F16, 277, x8.data_ptr(), ld8, sc.data_ptr(), lds,
-                                           dv.data_ptr(), S.F32, 0, st))
+    S.check(L.spmv_hip_block8_backward_dev(*args, x8.data_ptr(), ld8, sc.data_ptr(), lds, None, 0, 0, dv.data_ptr(), S.F32, 0,
+                                           work.data_ptr(), st))
+    assert torch.all(work[-16:] == 0)
     _close(dv[:-1], O.sampled(_mat(d.T, xq), c.ptr, c.col), n, O.sampled(_mat(np.abs(d).T, np.abs(xq)), c.ptr, c.col))
     assert torch.all(dv[-1] == -5.0)
 
@@ -581,10 +585,21 @@ def test_refusals():
     fails(L.spmv_hip_block8_mult_dev(h, 1, p, S.E4M3, 300, p, 1, p, S.F32, 200, None), "multiple of 128")
     fails(L.spmv_hip_block8_mult_dev(h, 2, p, S.F32, 300, None, 0, p, S.F32, 199, None), "shorter than their length")
     fails(L.spmv_hip_block8_mult_dev(h, -1, p, S.F32, 300, None, 0, p, S.F32, 200, None), "negative vector count")
-    fails(L.spmv_hip_block8_mult_t_dev(h, 2, p, S.F32, 199, p, S.F32, 300, None), "shorter than their length")
-    fails(L.spmv_hip_block8_mult_t_dev(h, 2, None, S.F32, 200, p, S.F32, 300, None), "NULL vector block")
-    fails(L.spmv_hip_block8_gradient_dev(h, 2, p, S.F32, 200, p, 384, p, 1, p, S.F32, 0, None), "1 scales per group")
-    fails(L.spmv_hip_block8_gradient_dev(h, 2, p, S.F32, 200, p, 384, p, 2, None, S.F32, 0, None), "NULL gradient")
+    back = lambda n=2, dy=p, dt=S.F32, ld=200, x8=p, ld8=384, sc=p, lds=2, dx=p, xt=S.F32, ldx=300, dv=p, vt=S.F32, work=p: \
+        L.spmv_hip_block8_backward_dev(h, n, dy, dt, ld, x8, ld8, sc, lds, dx, xt, ldx, dv, vt, 0, work, None)
+    fails(back(ld=199), "shorter than their length")
+    fails(back(ldx=299), "shorter than their length")
+    fails(back(ld=1 << 23), "at most 2^23 - 1")
+    fails(back(dy=None), "NULL vector block")
+    fails(back(dt=S.E4M3), "must be F32, BF16 or F16")
+    fails(back(xt=S.F64), "must be F32, BF16 or F16")
+    fails(back(vt=9), "must be F32, BF16 or F16")
+    fails(back(n=-1), "negative vector count")
+    fails(back(lds=1), "1 scales per group")
+    fails(back(x8=None), "NULL 8-bit")
+    fails(back(work=None), f"NULL workspace, {3 * 2 * 256 * 2} bytes needed")
+    fails(back(work=p + 8), "workspace is not 16-byte aligned")
+    assert back(dx=None, dv=None) == 0                       # neither asked for: nothing to do
     m = S.Matrix.csr(2, 2, S.make_coo([0, 1], [0, 1], [1.0, 2.0]))
     fails(L.spmv_hip_block8_mult_dev(m._h, 1, p, S.F32, 2, None, 0, p, S.F32, 2, None), "needs a handle of 8-bit blocks")
     m.free()
