@@ -421,9 +421,12 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
  *     8-bit checkpoint (needed for this one only); zero beyond the matrix's edge.
  *     accumulate != 0 adds to what d_dvalues holds.
  * d_work: spmv_hip_block8_backward_work() bytes of device memory, 16-byte aligned,
- * scratch for this call (NULL if that is 0: bf16 vectors at 16-byte aligned
- * addresses, or bf16 and no dx).  with_dx: whether dx is asked for. */
-int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx);
+ * scratch for this call, NULL if that is 0.  It holds dy in bf16 parts, where dy is
+ * not bf16 or, for dx, its vectors are not 16-byte aligned, and the slices of sums
+ * that are cut because there are too few of them to fill the device.  with_dx,
+ * with_dvalues: which of the two the call will ask for. */
+int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx,
+                                      int with_dvalues);
 int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
                                  const uint8_t *d_x8, int64_t ldx8, const uint8_t *d_scale, int64_t lds, void *d_dx, int dx_dtype,
                                  int64_t lddx, void *d_dvalues, int dv_dtype, int accumulate, void *d_work, void *stream);

@@ -70,7 +70,7 @@ SIGNATURES = {
     "spmv_hip_quantize8_dev": (_i, [_i, _i, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp]),
     "spmv_hip_restore8_dev": (_i, [_i, _i, _vp, _i64, _vp, _i64, _vp, _i, _i64, _vp]),
     "spmv_hip_block8_mult_dev": (_i, [_vp, _i, _vp, _i, _i64, _vp, _i64, _vp, _i, _i64, _vp]),
-    "spmv_hip_block8_backward_work": (_i64, [_vp, _i, _vp, _i, _i64, _i]),
+    "spmv_hip_block8_backward_work": (_i64, [_vp, _i, _vp, _i, _i64, _i, _i]),
     "spmv_hip_block8_backward_dev": (_i, [_vp, _i, _vp, _i, _i64, _vp, _i64, _vp, _i64, _vp, _i, _i64, _vp, _i, _i, _vp, _vp]),
     "spmv_hip_set_row_map": (_i, [_vp, _vp]),
     "spmv_hip_free": (_i, [_vp]),

@@ -249,7 +249,7 @@ class Block8(Matrix):
         """dx and dv, either None, from checked operands."""
         lib, n, ld = L.lib(), d.shape[0], _ld(d)
         p, t, work = d.data_ptr(), _DTYPE[d.dtype], None
-        size = lib.spmv_hip_block8_backward_work(self._h, n, p, t, ld, dx is not None)
+        size = lib.spmv_hip_block8_backward_work(self._h, n, p, t, ld, dx is not None, dv is not None)
         if size:
             work = torch.empty(size, dtype=torch.uint8, device=self.device)
         L.check(lib.spmv_hip_block8_backward_dev(

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <new>
+#include <cstdlib>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -670,7 +671,7 @@ static int parts(int dtype) { return dtype == SPMV_HIP_BF16 ? 1 : dtype == SPMV_
 
 // dy into its parts, `plane` entries apart, vectors `ld` apart (a multiple of 128), zero past `length`; 8 entries a
 // thread.  Before the products rather than in them: there the splitting stood between loads and matrix instructions of
-// every step (fp32, 333 vectors, 264 blocks: 41 us, now 4 + 14).
+// every step (fp32, 333 vectors, 264 blocks: 41 us, now 6 + 26).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void split_kernel(int n, int length, int ld, const T *__restrict__ dy, int64_t lddy,
                                                        __bf16 *__restrict__ out, int64_t plane)
@@ -704,7 +705,7 @@ struct TransposedArgs {
     const int *ptr, *row, *id, *scale;               // lists by block column, their blocks' scales
     const uint8_t *val8;
     const __bf16 *dy;
-    int64_t lddy, plane, lddx;     // plane: from one part of dy to the next
+    int64_t lddy, plane, lddx, slice;    // plane: from one part of dy to the next; slice: of dx, where the sum is cut
 };
 
 // dx = A^T dy, half a block (64 rows) a step, blocks and vectors through LDS.  ds_read_b64_tr_b8 hands every lane one
@@ -728,7 +729,14 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
     int whole = end;
     if (PARTS == 1 && g.rows % kB)
         while (whole > begin && table(g.row, whole - 1) == g.rows / kB) whole--;
-    const int first = 2 * begin, last = 2 * whole;
+    int first = 2 * begin, last = 2 * whole, edge = last;    // half blocks of this slice; those with masked entries
+    if (gridDim.y > 1) {
+        const int per = (last - first + (int)gridDim.y - 1) / (int)gridDim.y;
+        first = min(first + (int)blockIdx.y * per, last);
+        last = min(first + per, last);
+        if (blockIdx.y + 1 < gridDim.y) edge = 2 * end;
+        dx += blockIdx.y * g.slice;
+    }
     f32x4 acc[NU][4];
 #pragma unroll
     for (int u = 0; u < NU; u++)
@@ -839,7 +847,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         ring<R>(first, last, step);
     }
     stage_barrier<0>();                                      // no load to LDS outlives the workgroup, or meets the next
-    for (int k = last; k < 2 * end; k++) {
+    for (int k = edge; k < 2 * end; k++) {
         look_up(k);
         issue_block(ic<0>(), k);
         const int r = row * kB + (k & 1) * 64;
@@ -870,20 +878,21 @@ struct GradientArgs {
     const int *block_row, *block_col;
     const uint8_t *x8, *xscale;
     const __bf16 *dy;
-    int64_t ldx8, lds, lddy, plane;
+    int64_t ldx8, lds, lddy, plane, slice;       // slice: of dv, where the sum is cut
 };
 
 // dA = dy^T x at the stored blocks, 32 vectors a step.  With NB = 2 a workgroup has two blocks of one block row, a wave
 // 128 rows x 64 columns; with NB = 1 one block, a wave 64 x 64.  Both operands lie vector by vector, along the sum,
-// and have to be turned.  dy, which all waves share, is turned on its way into LDS (a thread has 2 rows of 8
-// vectors).  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane: widened there with
-// the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane i's columns are
-// 4 i + s: its results are 16 neighbours.
+// and have to be turned.  dy, which all waves share, comes into LDS by direct loads and is turned by ds_read_b64_tr_b16 (a
+// lane gets one row of 4 vectors); a vector's 16-byte pieces are exchanged by XOR so that the 8 vectors of a read cycle
+// lie on different banks.  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane:
+// widened there with the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane
+// i's columns are 4 i + s: its results are 16 neighbours.
 template <int PARTS, int NB, typename OT>
 __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT *__restrict__ dv)
 {
-    constexpr int STEP = 32, NU = 4 * NB, R = NB == 2 ? 2 : PARTS == 3 ? 3 : 4;
-    __shared__ uint8_t Y[2][PARTS][kB * STEP * 2];           // [row][32 vectors], 16-byte pieces exchanged by XOR
+    constexpr int STEP = 32, NU = 4 * NB, R = NB == 2 ? (PARTS == 1 ? 3 : 2) : PARTS == 3 ? 3 : 4;
+    __shared__ uint8_t Y[R][PARTS][STEP * kB * 2];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
     const int wg = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
     const int which = NB == 2 ? wave >> 1 : 0;               // the wave's block, its columns and rows in it
@@ -896,74 +905,64 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
 #pragma unroll
         for (int s = 0; s < 4; s++) acc[u][s] = f32x4{0, 0, 0, 0};
 
-    unsigned yr[R][PARTS][8];                                // two rows of 8 vectors
     unsigned xr[R][8];
     uint64_t sx[R];
-    // A lane's two rows of dy are r and r + 1, loaded from rp, which moves back where they run past the last row: then its
-    // first row is the second loaded, or both are past the end.
-    const int r = row0 + 2 * lane, rp = min(r, max(g.rows - 2, 0));
-    const bool natural = r == rp, shifted = r == rp + 1 && r < g.rows;
     const unsigned xat = 8 * (unsigned)q * (unsigned)g.ldx8 + 4 * i;
-    auto fetch = [&](auto slot, int t0) {                    // 32 whole vectors, two rows or more
+    // a thread's pieces of dy: 8 rows from `prow` on, of vectors 8 wave + q and 4 further
+    const int prow = row0 + 8 * (i ^ (q << 1 | (wave & 1) << 3));
+    const unsigned lddy = (unsigned)g.lddy, near = ((8 * wave + q) * lddy + prow) * 2;
+    auto issue = [&](auto slot, int k) {                     // 32 whole vectors
         constexpr int S = decltype(slot)::value;
+        const int t0 = k * STEP;
         const uint8_t *xp = g.x8 + (int64_t)t0 * g.ldx8 + col * kB + c0;
-        const __bf16 *yp = g.dy + (int64_t)(t0 + 8 * wave) * g.lddy;
 #pragma unroll
         for (int w = 0; w < 8; w++) xr[S][w] = *(const unsigned *)(xp + w * g.ldx8 + xat);
         __builtin_memcpy(&sx[S], g.xscale + (int64_t)col * g.lds + t0 + 8 * q, 8);
 #pragma unroll
-        for (int p = 0; p < PARTS; p++)
+        for (int p = 0; p < PARTS; p++) {
+            const u32x4 y = buffer(g.dy + p * g.plane + (int64_t)t0 * g.lddy, ((STEP - 1) * lddy + g.rows) * 2);
 #pragma unroll
-            for (int w = 0; w < 8; w++) __builtin_memcpy(&yr[S][p][w], yp + p * g.plane + w * g.lddy + (unsigned)rp, 4);
+            for (int j = 0; j < 2; j++) load_to_lds<true>(y, near + j * 8 * lddy, &Y[S][p][(8 * wave + 4 * j) * 256]);
+        }
     };
     // the vectors after the last whole 32; past the last dy is zero, and x the last one's, so that nothing new that is not
     // finite comes in
-    auto fetch_rest = [&](int t0) {
+    auto bring_rest = [&](int t0) {
         const uint8_t *xp = g.x8 + (int64_t)t0 * g.ldx8 + col * kB + c0 + 4 * i;
-        const __bf16 *yp = g.dy + (int64_t)t0 * g.lddy + rp;
         const uint8_t *sp = g.xscale + (int64_t)col * g.lds + t0;
         const int top = g.n - 1 - t0;
         sx[0] = 0;
 #pragma unroll
         for (int w = 0; w < 8; w++) {
-            const int ty = 8 * wave + w, tx = 8 * q + w;
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) {
-                Raw<__bf16, 2> two;
-                two.load(yp + p * g.plane + (int64_t)min(ty, top) * g.lddy, ty <= top ? min(g.rows, 2) : 0);
-                __builtin_memcpy(&yr[0][p][w], two.v, 4);
-            }
-            xr[0][w] = *(const unsigned *)(xp + (int64_t)min(tx, top) * g.ldx8);
-            sx[0] |= (uint64_t)sp[min(tx, top)] << (8 * w);
+            const int tx = min(8 * q + w, top);
+            xr[0][w] = *(const unsigned *)(xp + (int64_t)tx * g.ldx8);
+            sx[0] |= (uint64_t)sp[tx] << (8 * w);
         }
-    };
-    // bytes of two vectors' words that make a row's pair: the first or the second half of each, or zeros
-    const unsigned lo = 0x05040100u, hi = 0x07060302u, none = 0x0c0c0c0cu;
-    const unsigned pick[2] = {natural ? lo : shifted ? hi : none, natural ? hi : none};
-    auto put = [&](auto slot, int buf) {
-        constexpr int S = decltype(slot)::value;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int row = 2 * lane + k;
+        for (int p = 0; p < PARTS; p++)
 #pragma unroll
-            for (int p = 0; p < PARTS; p++) {
-                u32x4 v;
-#pragma unroll
-                for (int w = 0; w < 4; w++) v[w] = __builtin_amdgcn_perm(yr[S][p][2 * w + 1], yr[S][p][2 * w], pick[k]);
-                *(u32x4 *)&Y[buf][p][row * 64 + ((wave ^ ((row >> 1) & 3)) << 4)] = v;
+            for (int j = 0; j < 2; j++) {
+                const int ty = 8 * wave + 4 * j + q;
+                Raw<__bf16, 8> one;
+                one.load(g.dy + p * g.plane + (int64_t)(t0 + min(ty, top)) * g.lddy + prow, ty <= top ? g.rows - prow : 0);
+                __builtin_memcpy(&Y[0][p][(8 * wave + 4 * j) * 256 + lane * 16], one.v, 16);
             }
-        }
     };
-    auto compute = [&](auto slot, int buf, auto between) {
+    auto compute = [&](auto slot, auto between) {
         constexpr int S = decltype(slot)::value, AHEAD = PARTS * NU <= 8 ? PARTS * NU : 4;
         auto read_b = [&](int k) {
-            const int row = n0 + 16 * (k % NU) + i;
-            return *(const bf16x8 *)&Y[buf][k / NU][row * 64 + ((q ^ ((row >> 1) & 3)) << 4)];
+            typedef short i16x4 __attribute__((ext_vector_type(4)));
+            // lane i: 4 rows of vector 8 q + i / 4, then of the one 4 further; it gets row i of those vectors
+            const int v = 8 * q + (i >> 2), piece = n0 / 8 + 2 * (k % NU) + ((i >> 1) & 1);
+            const uint8_t *at = &Y[S][k / NU][v * 256 + ((piece ^ ((v & 3) << 1 | (q & 1) << 3)) << 4) + (i & 1) * 8];
+            union { i16x4 h[2]; bf16x8 v; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)at);
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)(at + 4 * 256));
+            return u.v;
         };
         bf16x8 b[PARTS * NU];
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) b[k] = read_b(k);
-        between();                                           // the loads of a later stage, which take a while to issue
         bf16x8 a[4];
         {
             unsigned pair[8][2];                             // columns (0, 1) and (2, 3) of 8 vectors
@@ -982,6 +981,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
                 __builtin_memcpy(&a[s], v, 16);
             }
         }
+        between();                                           // the loads of a later stage, which take a while to issue
 #pragma unroll
         for (int k = 0; k < PARTS * NU; k++) {
             if (k + AHEAD < PARTS * NU) b[k + AHEAD] = read_b(k + AHEAD);
@@ -989,26 +989,30 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
             for (int s = 0; s < 4; s++) acc[k % NU][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[k], acc[k % NU][s], 0, 0, 0);
         }
     };
-    const int whole = g.rows < 2 ? 0 : g.n / STEP;           // the rest one by one, a matrix of one row altogether
-    if (whole) {
-        fetch(ic<0>(), 0);
-        if constexpr (R > 2) fetch(ic<1>(), min(1, whole - 1) * STEP);
-        if constexpr (R > 3) fetch(ic<2>(), min(2, whole - 1) * STEP);
-        put(ic<0>(), 0);
-        __syncthreads();
-        ring<R>(0, whole, [&](auto slot, int k) {
+    const int whole = g.n / STEP;
+    int first = 0, last = whole, rest = whole * STEP;
+    if (gridDim.y > 1) {                                     // this slice of the sum
+        const int per = (whole + (int)gridDim.y - 1) / (int)gridDim.y;
+        first = min((int)blockIdx.y * per, whole);
+        last = min(first + per, whole);
+        if (blockIdx.y + 1 < gridDim.y) rest = g.n;
+        dv += blockIdx.y * g.slice;
+    }
+    if (first < last) {
+        issue(ic<0>(), first);
+        if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
+        if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
+        ring<R>(first, last, [&](auto slot, int k) {
             constexpr int S = decltype(slot)::value;
-            compute(slot, k & 1, [&] { fetch(ic<(S + R - 1) % R>(), min(k + R - 1, whole - 1) * STEP); });
-            put(ic<(S + 1) % R>(), (k & 1) ^ 1);             // after the last: once more the last, read by nobody
-            __syncthreads();
+            stage_barrier<(R - 2) * (9 + 2 * PARTS)>();
+            compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
         });
     }
-    for (int t0 = whole * STEP; t0 < g.n; t0 += STEP) {
-        fetch_rest(t0);
-        put(ic<0>(), 0);
-        __syncthreads();
-        compute(ic<0>(), 0, [] {});
-        __syncthreads();
+    stage_barrier<0>();                                      // no load to LDS outlives the workgroup, or meets the next
+    if (rest < g.n) {
+        bring_rest(rest);
+        stage_barrier<0>();
+        compute(ic<0>(), [] {});
     }
     if (id < 0) return;
     // a lane has columns 16 q .. 16 q + 15 of its wave's 64, row 16 u + i; result r of tile s is column 16 q + 4 r + s
@@ -1026,6 +1030,28 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
         }
         store_row<OT, 4>(o, 16, v);
     }
+}
+
+// out (+)= the slices of a cut sum, added in their order; rows of `ldin` entries (a multiple of 4), 4 a thread
+template <typename OT>
+__global__ __launch_bounds__(kBlock) void join_kernel(int64_t count, int columns, int slices, const float *__restrict__ in, int64_t ldin,
+                                                      int64_t slice, OT *__restrict__ out, int64_t ldout, int accumulate)
+{
+    const int64_t at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 4;
+    if (at >= count) return;
+    const int64_t r = at / ldin;
+    const int c = (int)(at % ldin), left = columns - c;
+    if (left <= 0) return;
+    OT *o = out + r * ldout + c;
+    f32x4 sum = *(const f32x4 *)(in + at);
+    for (int z = 1; z < slices; z++) sum += *(const f32x4 *)(in + z * slice + at);
+    if (accumulate) {
+        Raw<OT, 4> old;
+        old.load(o, left);
+#pragma unroll
+        for (int k = 0; k < 4; k++) sum[k] += (float)old.v[k];
+    }
+    store_row<OT, 1>(o, left, &sum);
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------
@@ -1131,6 +1157,55 @@ static int check_tiles(const char *what, int majors, int vtiles)
     if ((int64_t)majors * vtiles <= 0x7fffffff) return 0;
     set_error("%s: %d x %d tiles are more than one launch takes", what, majors, vtiles);
     return 1;
+}
+
+// How a backward call runs; `work` in bytes: the parts of dy, then the slices of a cut sum
+struct BackwardPlan {
+    bool split;                    // dy goes into its parts first
+    bool pairs;                    // two blocks of a block row a workgroup
+    int tiles, dx_slices, dv_slices;
+    int64_t dx_slice, dv_slice, parts_bytes, work;
+};
+
+// Slices of a sum of `steps` steps whose `tiles` workgroups leave much of the GPU idle: as many as make `wgs` workgroups,
+// `least` steps each or more
+static int slices(int64_t tiles, int64_t wgs, int64_t steps, int least)
+{
+    return (int)std::max<int64_t>(1, std::min(wgs / tiles, steps / least));
+}
+
+static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d_dy, int dtype, int64_t lddy, bool with_dx, bool with_dv)
+{
+    BackwardPlan p{};
+    p.dx_slices = p.dv_slices = 1;
+    if (n <= 0) return p;
+    // dy goes into the products as it lies: bf16 with 16-byte aligned vectors
+    p.split = m->rows > 0 && (dtype != SPMV_HIP_BF16 || (uintptr_t)d_dy % 16 || (n > 1 && lddy % 8));
+    const int count = parts(dtype);
+    if (p.split) p.parts_bytes = (int64_t)count * n * m->brows * kB * 2;
+    if (with_dx && m->bcols) {
+        p.tiles = vector_tiles(m, m->bcols, n, count == 1 ? 8 : 4);
+        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), m->cus, 2 * (int64_t)m->nblocks / m->bcols, 4);
+        p.dx_slice = (int64_t)n * m->bcols * kB;
+    }
+    if (with_dv && m->nblocks) {
+        // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
+        // registers; and not where many pairs lack their second block
+        p.pairs = m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
+        static const int B = getenv("SB") ? atoi(getenv("SB")) : 2;
+        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, B * m->cus, n / 32, 8);
+        p.dv_slice = (int64_t)m->nblocks * kBlockBytes;
+    }
+    p.work = p.parts_bytes + 4 * std::max(p.dx_slices > 1 ? p.dx_slices * p.dx_slice : 0, p.dv_slices > 1 ? p.dv_slices * p.dv_slice : 0);
+    return p;
+}
+
+template <typename O>
+static void launch_join(int64_t rows, int64_t ldin, int columns, int slices, const float *in, O *out, int64_t ldout, int accumulate, hipStream_t st)
+{
+    const int64_t count = rows * ldin;
+    hipLaunchKernelGGL(join_kernel<O>, dim3((unsigned)((count / 4 + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, count, columns, slices, in, ldin,
+                       count, out, ldout, accumulate);
 }
 
 } // namespace spmv
@@ -1338,16 +1413,10 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     return launched(what);
 }
 
-// whether dy goes into the products as it lies: bf16, and for dx with 16-byte aligned vectors
-static bool as_it_lies(int n, const void *d_dy, int dtype, int64_t lddy, bool with_dx)
+int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx, int with_dvalues)
 {
-    return dtype == SPMV_HIP_BF16 && (!with_dx || ((uintptr_t)d_dy % 16 == 0 && (n == 1 || lddy % 8 == 0)));
-}
-
-int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx)
-{
-    if (!m || m->format != SPMV_HIP_BLOCK8 || n <= 0 || !wide_dtype(dy_dtype) || as_it_lies(n, d_dy, dy_dtype, lddy, with_dx != 0)) return 0;
-    return (int64_t)parts(dy_dtype) * n * m->brows * kB * 2;
+    if (!m || m->format != SPMV_HIP_BLOCK8 || !wide_dtype(dy_dtype)) return 0;
+    return backward_plan(m, n, d_dy, dy_dtype, lddy, with_dx != 0, with_dvalues != 0).work;
 }
 
 int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,
@@ -1370,12 +1439,12 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
         if (!wide_dtype(dv_dtype)) return bad_dtype(what, dv_dtype);
         if (check_eight(what, n, m->columns, d_x8, ldx8, d_scale, lds)) return 1;
     }
-    const bool split = n > 0 && m->rows > 0 && !as_it_lies(n, d_dy, dy_dtype, lddy, d_dx != nullptr);
-    if (split && !d_work) {
-        set_error("%s: NULL workspace, %lld bytes needed", what, (long long)spmv_hip_block8_backward_work(m, n, d_dy, dy_dtype, lddy, d_dx != nullptr));
+    const BackwardPlan plan = backward_plan(m, n, d_dy, dy_dtype, lddy, d_dx != nullptr, d_dvalues != nullptr);
+    if (plan.work && !d_work) {
+        set_error("%s: NULL workspace, %lld bytes needed", what, (long long)plan.work);
         return 1;
     }
-    if (split && (uintptr_t)d_work % 16) { set_error("%s: workspace is not 16-byte aligned", what); return 1; }
+    if (plan.work && (uintptr_t)d_work % 16) { set_error("%s: workspace is not 16-byte aligned", what); return 1; }
     if (!d_dx && !d_dvalues) return 0;
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
@@ -1383,7 +1452,7 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
     const __bf16 *dy = (const __bf16 *)d_dy;
     int rows = m->rows;
     int64_t plane = 0;
-    if (split) {
+    if (plan.split) {
         rows = m->brows * kB;
         plane = (int64_t)n * rows;
         if (plane / 8 > (int64_t)0x7fffffff * kBlock || rows >= 1 << 23) { set_error("%s: %d vectors of %d are more than one launch takes", what, n, m->rows); return 1; }
@@ -1395,6 +1464,7 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
         dy = (const __bf16 *)d_work;
         lddy = rows;
     }
+    float *cut = (float *)((char *)d_work + plan.parts_bytes);  // slices of dx, then of dvalues
     const int count = parts(dy_dtype);
     auto with_parts = [&](auto f) {
         if (count == 1) f(ic<1>());
@@ -1405,38 +1475,49 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
         TransposedArgs a{};
         a.n = n; a.rows = rows; a.columns = m->columns; a.bcols = m->bcols;
         a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale = m->d_bt_scale8;
-        a.dy = dy; a.lddy = lddy; a.plane = plane; a.lddx = lddx;
-        const int nu = vector_tiles(m, m->bcols, n, count == 1 ? 8 : 4);
+        a.dy = dy; a.lddy = lddy; a.plane = plane; a.slice = plan.dx_slice;
+        const int nu = plan.tiles;
         a.vtiles = (n + 32 * nu - 1) / (32 * nu);
         if (check_tiles(what, m->bcols, a.vtiles)) return 1;
-        with_elem(dx_dtype, [&](auto o) {
-            typedef decltype(o) O;
+        auto into = [&](auto *to, int64_t ld) {
+            typedef std::remove_pointer_t<decltype(to)> O;
+            a.lddx = ld;
             with_parts([&](auto p) {
                 constexpr int P = decltype(p)::value;
-                auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles), dim3(kBlock), 0, st, a, (O *)d_dx); };
+                auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles, plan.dx_slices), dim3(kBlock), 0, st, a, to); };
                 if constexpr (P == 1) if (nu == 8) { go(transposed_kernel<P, 8, O>); return; }
                 if (nu == 4) go(transposed_kernel<P, 4, O>);
                 else go(transposed_kernel<P, 2, O>);
             });
+        };
+        with_elem(dx_dtype, [&](auto o) {
+            typedef decltype(o) O;
+            if (plan.dx_slices == 1) { into((O *)d_dx, lddx); return; }
+            into(cut, m->bcols * (int64_t)kB);
+            launch_join(n, m->bcols * (int64_t)kB, m->columns, plan.dx_slices, cut, (O *)d_dx, lddx, 0, st);
         });
     }
     if (d_dvalues && m->nblocks > 0) {
         GradientArgs a{};
-        a.n = n; a.rows = rows; a.edge = m->rows; a.columns = m->columns; a.accumulate = accumulate;
+        a.n = n; a.rows = rows; a.edge = m->rows; a.columns = m->columns;
         a.block_row = m->d_block_row; a.block_col = m->d_block_col;
-        a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.dy = dy; a.lddy = lddy; a.plane = plane;
-        // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
-        // registers; and not where many pairs lack their second block
-        const bool pairs = count == 1 && m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
-        a.list = pairs ? m->d_pair : m->d_order;
-        with_elem(dv_dtype, [&](auto o) {
-            typedef decltype(o) O;
+        a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.dy = dy; a.lddy = lddy; a.plane = plane; a.slice = plan.dv_slice;
+        a.list = plan.pairs ? m->d_pair : m->d_order;
+        auto into = [&](auto *to, int add) {
+            typedef std::remove_pointer_t<decltype(to)> O;
+            a.accumulate = add;
             with_parts([&](auto p) {
                 constexpr int P = decltype(p)::value;
-                auto go = [&](auto kernel, int wgs) { hipLaunchKernelGGL(kernel, dim3(wgs), dim3(kBlock), 0, st, a, (O *)d_dvalues); };
-                if constexpr (P == 1) if (pairs) { go(gradient_kernel<P, 2, O>, m->npairs); return; }
+                auto go = [&](auto kernel, int wgs) { hipLaunchKernelGGL(kernel, dim3(wgs, plan.dv_slices), dim3(kBlock), 0, st, a, to); };
+                if (plan.pairs) { go(gradient_kernel<P, 2, O>, m->npairs); return; }
                 go(gradient_kernel<P, 1, O>, m->nblocks);
             });
+        };
+        with_elem(dv_dtype, [&](auto o) {
+            typedef decltype(o) O;
+            if (plan.dv_slices == 1) { into((O *)d_dvalues, accumulate); return; }
+            into(cut, 0);
+            launch_join(m->nblocks, (int64_t)kBlockBytes, kBlockBytes, plan.dv_slices, cut, (O *)d_dvalues, (int64_t)kBlockBytes, accumulate, st);
         });
     }
     return launched(what);

@@ -87,7 +87,7 @@ def test_vector_calls_refuse_bad_arguments():
                        ("set_values", (None, p, S.F32, None)),
                        ("load", (None, p, p, None)), ("store", (None, p, p, None))):
         _fails(getattr(L, f"spmv_hip_block8_{name}_dev")(*args), "NULL handle")
-    assert L.spmv_hip_block8_backward_work(None, 1, p, S.F32, 9, 1) == 0
+    assert L.spmv_hip_block8_backward_work(None, 1, p, S.F32, 9, 1, 1) == 0
 
 
 def test_python_layer_refuses_what_is_not_on_a_gpu():

@@ -156,8 +156,9 @@ def test_abi_strides_leave_the_gaps_alone():
         assert torch.all(y[:, 260:] == -5.0) and torch.all(y[k:] == -5.0)
     dy = _vectors(n, 277, F16, 2)
     dx = torch.full((n, 301), -5.0, device=DEV)
-    assert L.spmv_hip_block8_backward_work(c.A._h, n, dy.data_ptr(), S.F16, 277, 1) == 2 * n * 384 * 2
-    work = torch.zeros(2 * n * 384 * 2 + 16, dtype=torch.uint8, device=DEV)
+    size = L.spmv_hip_block8_backward_work(c.A._h, n, dy.data_ptr(), S.F16, 277, 1, 1)
+    assert size >= 2 * n * 384 * 2
+    work = torch.zeros(size + 16, dtype=torch.uint8, device=DEV)
     args = (c.A._h, n, dy.data_ptr(), S.F16, 277)
     S.check(L.spmv_hip_block8_backward_dev(*args, None, 0, None, 0, dx.data_ptr(), S.F32, 301, None, 0, 0, work.data_ptr(), st))
     d = _np(dy)[:, :260]
