@@ -887,7 +887,7 @@ struct GradientArgs {
 // lane gets one row of 4 vectors); a vector's 16-byte pieces are exchanged by XOR so that the 8 vectors of a read cycle
 // lie on different banks.  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane:
 // widened there with the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane
-// i's columns are 4 i + s: its results are 16 neighbours.
+// i's columns are 4 i + s.
 template <int PARTS, int NB, typename OT>
 __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT *__restrict__ dv)
 {
@@ -986,7 +986,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
         for (int k = 0; k < PARTS * NU; k++) {
             if (k + AHEAD < PARTS * NU) b[k + AHEAD] = read_b(k + AHEAD);
 #pragma unroll
-            for (int s = 0; s < 4; s++) acc[k % NU][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[k], acc[k % NU][s], 0, 0, 0);
+            for (int s = 0; s < 4; s++) acc[k % NU][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[k], a[s], acc[k % NU][s], 0, 0, 0);
         }
     };
     const int whole = g.n / STEP;
@@ -1015,21 +1015,28 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
         compute(ic<0>(), [] {});
     }
     if (id < 0) return;
-    // a lane has columns 16 q .. 16 q + 15 of its wave's 64, row 16 u + i; result r of tile s is column 16 q + 4 r + s
+    // result r of tile (u, s) is row 16 u + 4 q + r, column 4 i + s: 16 lanes write 64 neighbours of a row.  (The other way
+    // round a lane had 16 neighbours, and a store 64 pieces of 16 bytes: MEASURE.)
+    const int c = c0 + 4 * i, left = g.columns - (col * kB + c);
+    OT *o = dv + (int64_t)id * kBlockBytes + (n0 + 4 * q) * kB + c;
 #pragma unroll
-    for (int u = 0; u < NU; u++) {
-        const int row = n0 + 16 * u + i;
-        OT *o = dv + (int64_t)id * kBlockBytes + row * kB + c0 + 16 * q;
-        const int left = row0 + row < g.edge ? g.columns - (col * kB + c0 + 16 * q) : 0;
-        f32x4 v[4];
+    for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int k = 0; k < 16; k++) {
+        for (int r = 0; r < 4; r++) {
+            const int row = 16 * u + r;
             // beyond the edge x is zero, but for 8-bit vectors that were not made by quantize8
-            v[k >> 2][k & 3] = k < left ? acc[u][k & 3][k >> 2] : 0.0f;
-            if (g.accumulate) v[k >> 2][k & 3] += (float)o[k];
+            const int here = row0 + n0 + 4 * q + row < g.edge ? left : 0;
+            f32x4 v;
+#pragma unroll
+            for (int s = 0; s < 4; s++) v[s] = s < here ? acc[u][s][r] : 0.0f;
+            if (g.accumulate) {
+                Raw<OT, 4> old;
+                old.load(o + row * kB, 4);
+#pragma unroll
+                for (int s = 0; s < 4; s++) v[s] += (float)old.v[s];
+            }
+            store_row<OT, 1>(o + row * kB, 4, &v);
         }
-        store_row<OT, 4>(o, 16, v);
-    }
 }
 
 // out (+)= the slices of a cut sum, added in their order; rows of `ldin` entries (a multiple of 4), 4 a thread
