@@ -6,7 +6,6 @@
 
 #include <algorithm>
 #include <new>
-#include <cstdlib>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -25,11 +24,11 @@ constexpr int kBlockBytes = kB * kB;
 
 // Place of (row, column) inside a block's 16 KB: 16 x 16 subtiles of 256 bytes, so that one 16-byte load per lane
 // is a contiguous 1 KB piece of a matrix-instruction operand (16 rows of one strip, 64 columns).  A strip holds the rows
-// {16 q + 4 s + r} of one 64-row half (s = strip in the half, q, r = 0..3): the accumulator keeps rows 4 q .. 4 q + 3 of
-// a tile in lane group q, which makes 4 tiles' results in a lane 16 consecutive rows of y.
+// {4 i + s} of one 64-row half (s = strip in the half, i = 0..15): with the rows along the lanes of a result, 4 strips'
+// results in a lane are 4 consecutive rows of y, and those of 16 lanes 64.
 __host__ __device__ __forceinline__ int block8_offset(int row, int col)
 {
-    const int strip = (row >> 6) * 4 + ((row >> 2) & 3), i = ((row >> 4) & 3) * 4 + (row & 3);
+    const int strip = (row >> 6) * 4 + (row & 3), i = (row >> 2) & 15;
     return ((strip * 8 + (col >> 4)) * 16 + i) * 16 + (col & 15);
 }
 
@@ -429,11 +428,11 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         f32x4 s = part[0][t][l];
 #pragma unroll
         for (int w = 1; w < W; w++) s += part[w][t][l];
-        const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + 4 * (strip & 3);
+        const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + (strip & 3);
         if (v >= n) continue;
         for (int k = 0; k < 4; k++) {
-            if (r0 + k >= rows) break;
-            const int64_t at = (int64_t)v * ldy + r0 + k;
+            if (r0 + 4 * k >= rows) break;
+            const int64_t at = (int64_t)v * ldy + r0 + 4 * k;
             if (y_dtype == SPMV_HIP_F32) ((float *)y)[at] = s[k];
             else if (y_dtype == SPMV_HIP_BF16) ((__bf16 *)y)[at] = (__bf16)s[k];
             else ((_Float16 *)y)[at] = (_Float16)s[k];
@@ -636,12 +635,12 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
                     unpack4((unsigned)w[u][2 * p], fx, (__bf16 *)&xw);
                     unpack4((unsigned)w[u][2 * p + 1], fx, (__bf16 *)&xw + 4);
 #pragma unroll
-                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(aw[s][p], xw, acc[u][s], 0, 0, 0);
+                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xw, aw[s][p], acc[u][s], 0, 0, 0);
                 }
             } else {
 #pragma unroll
                 for (int s = 0; s < 4; s++)
-                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[S][s], w[u], acc[u][s], 0, 0, 0, sa[S], 0, su);
+                    acc[u][s] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u], a[S][s], acc[u][s], 0, 0, 0, su, 0, sa[S]);
             }
             if (NU == 8) __builtin_amdgcn_sched_barrier(0);
         }
@@ -654,11 +653,17 @@ __global__ __launch_bounds__(kBlock, 2) void product_kernel(ProductArgs g, OT *_
         ring<R>(first, last, step);
     }
     stage_barrier<0>();                                      // no load to LDS outlives the workgroup
-    // a lane has rows 16 q .. 16 q + 15 of its wave's 64 for NU vectors
-    const int r = major * kB + wm * 64 + 16 * q;
+    // result k of tile (u, s) is vector NU (4 q + k) + u, row 4 i + s of the wave's 64: 16 lanes write 64 neighbours.  (The
+    // other way round a lane had 16 neighbours, and a store 64 pieces of 16 bytes: MEASURE.)
+    const int r = major * kB + wm * 64 + 4 * i, v1 = t0 + wn * 16 * NU + NU * 4 * q;
 #pragma unroll
-    for (int u = 0; u < NU; u++)
-        if (v0 + u < g.n && r < g.rows) store_row<OT, 4>(y + (int64_t)(v0 + u) * g.ldy + r, g.rows - r, acc[u]);
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const f32x4 f = {acc[u][0][k], acc[u][1][k], acc[u][2][k], acc[u][3][k]};
+            const int v = v1 + NU * k + u;
+            if (v < g.n && r < g.rows) store_row<OT, 1>(y + (int64_t)v * g.ldy + r, g.rows - r, &f);
+        }
 }
 
 // dy is used as it is: as PARTS bf16 numbers that add up to it exactly (1 for bf16, 2 for fp16, 3 for fp32: each holds 8
@@ -709,9 +714,9 @@ struct TransposedArgs {
 };
 
 // dx = A^T dy, half a block (64 rows) a step, blocks and vectors through LDS.  ds_read_b64_tr_b8 hands every lane one
-// column of 8 rows of the block, widened to bf16 (exact) on the way to the matrix instruction.  8 rows of dy are 4 rows in
-// each of two strips of the block (block8_offset); in LDS the 4-row pieces of a 16 x 16 subtile are exchanged by XOR
-// with the strip, which puts the two on different banks.  The blocks of a last block row that is not whole come last in
+// column of 8 rows of the block, widened to bf16 (exact) on the way to the matrix instruction.  8 rows of dy are 2 rows in
+// each of four strips of the block (block8_offset); in LDS the 4-row pieces of a 16 x 16 subtile are exchanged by XOR
+// with the strip, which puts the four on different banks.  The blocks of a last block row that is not whole come last in
 // every list: they are taken after the others, one by one, with the entries past the end masked (dy in parts is padded
 // and has no such rows).
 template <int PARTS, int NU, typename OT>
@@ -785,8 +790,8 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         constexpr bool ALL = PARTS * NU <= 4;
         auto read_a = [&](int h, int s) {
             // row 32 h + 8 q + w, w = i >> 1, columns 8 (i & 1) .. + 7 of a subtile
-            const int strip = (2 * q + (i >> 3)) & 3, quad = 2 * h + (q >> 1);
-            const uint8_t *p = &A[S][strip * 2048 + wm * 1024 + ((quad ^ strip) << 6) + ((i >> 1) & 3) * 16 + (i & 1) * 8];
+            const int strip = (i >> 1) & 3, in = 8 * h + 2 * q + (i >> 3);
+            const uint8_t *p = &A[S][strip * 2048 + wm * 1024 + ((in ^ (strip << 2)) << 4) + (i & 1) * 8];
             return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2 *)(p + s * 256));
         };
         auto read_b = [&](int h, int part, int u) {
@@ -1152,11 +1157,11 @@ static dim3 group_grid(int n, int groups, int r)
     return dim3((unsigned)((n + per - 1) / per), (groups + kQuantGroups - 1) / kQuantGroups);
 }
 
-// Tiles of 16 vectors a wave takes: `most` where that still gives every CU a workgroup, else half, down to 2
-static int vector_tiles(const spmv_hip_matrix *m, int majors, int n, int most)
+// Tiles of 16 vectors a wave takes: `most` where that still makes `least` workgroups, else half, down to 2
+static int vector_tiles(int majors, int n, int most, int least)
 {
     int nu = most;
-    while (nu > 2 && (int64_t)majors * ((n + 32 * nu - 1) / (32 * nu)) < m->cus) nu /= 2;
+    while (nu > 2 && (int64_t)majors * ((n + 32 * nu - 1) / (32 * nu)) < least) nu /= 2;
     return nu;
 }
 static int check_tiles(const char *what, int majors, int vtiles)
@@ -1191,7 +1196,9 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
     const int count = parts(dtype);
     if (p.split) p.parts_bytes = (int64_t)count * n * m->brows * kB * 2;
     if (with_dx && m->bcols) {
-        p.tiles = vector_tiles(m, m->bcols, n, count == 1 ? 8 : 4);
+        // dy in parts: 2, so that two workgroups fit a CU (fp32, 3000 vectors, 440 blocks: 157 us, 189 with 4).  bf16: more
+        // only with 1 1/2 workgroups a CU left (777 vectors: 30 us, 42 with 4; 3000: 66 us with 8, 77 with 2)
+        p.tiles = count > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2);
         p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), m->cus, 2 * (int64_t)m->nblocks / m->bcols, 4);
         p.dx_slice = (int64_t)n * m->bcols * kB;
     }
@@ -1199,8 +1206,8 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
         // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
         // registers; and not where many pairs lack their second block
         p.pairs = m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
-        static const int B = getenv("SB") ? atoi(getenv("SB")) : 2;
-        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, B * m->cus, n / 32, 8);
+        const int tiles = p.pairs ? m->npairs : m->nblocks;
+        p.dv_slices = slices(tiles, 2 * m->cus, n / 32, 16 + tiles / 8);
         p.dv_slice = (int64_t)m->nblocks * kBlockBytes;
     }
     p.work = p.parts_bytes + 4 * std::max(p.dx_slices > 1 ? p.dx_slices * p.dx_slice : 0, p.dv_slices > 1 ? p.dv_slices * p.dv_slice : 0);
@@ -1404,7 +1411,7 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     a.n = n; a.rows = m->rows; a.brows = m->brows;
     a.ptr = m->d_block_ptr; a.col = m->d_block_col; a.val8 = m->d_val8; a.scale8 = m->d_scale8;
     a.x8 = (const uint8_t *)d_x; a.xscale = d_scale; a.ldx8 = ldx; a.lds = lds; a.ldy = ldy;
-    const int nu = vector_tiles(m, m->brows, n, y_dtype == SPMV_HIP_BF16 ? 8 : 4);
+    const int nu = vector_tiles(m->brows, n, y_dtype == SPMV_HIP_BF16 ? 8 : 4, m->cus);
     a.vtiles = (n + 32 * nu - 1) / (32 * nu);
     if (check_tiles(what, m->brows, a.vtiles)) return 1;
     with_elem(y_dtype, [&](auto t) {
@@ -1492,9 +1499,11 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
             with_parts([&](auto p) {
                 constexpr int P = decltype(p)::value;
                 auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles, plan.dx_slices), dim3(kBlock), 0, st, a, to); };
-                if constexpr (P == 1) if (nu == 8) { go(transposed_kernel<P, 8, O>); return; }
-                if (nu == 4) go(transposed_kernel<P, 4, O>);
-                else go(transposed_kernel<P, 2, O>);
+                if constexpr (P == 1) {
+                    if (nu == 8) { go(transposed_kernel<P, 8, O>); return; }
+                    if (nu == 4) { go(transposed_kernel<P, 4, O>); return; }
+                }
+                go(transposed_kernel<P, 2, O>);
             });
         };
         with_elem(dx_dtype, [&](auto o) {
