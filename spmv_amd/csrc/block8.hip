@@ -154,8 +154,9 @@ __global__ __launch_bounds__(kBlock) void quantize8_kernel(int n, int groups, in
     constexpr int U = R < 4 ? R : 4, TV = R * kQuantWaves;
     __shared__ uint8_t bytes[kQuantGroups][TV];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, gq = lane >> 4;
-    const int g0 = blockIdx.y * kQuantGroups, c = (g0 + gq) * kB + (lane & 15) * 8;
-    const int64_t v0 = (int64_t)blockIdx.x * TV;
+    const unsigned gtiles = (groups + kQuantGroups - 1) / kQuantGroups;
+    const int g0 = blockIdx.x % gtiles * kQuantGroups, c = (g0 + gq) * kB + (lane & 15) * 8;
+    const int64_t v0 = (int64_t)(blockIdx.x / gtiles) * TV;
     for (int r = 0; r < R; r += U) {
         Raw<T, 8> a[U];
 #pragma unroll
@@ -196,9 +197,10 @@ __global__ __launch_bounds__(kBlock) void restore8_kernel(int n, int groups, int
 {
     constexpr int U = R < 4 ? R : 4;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int g = blockIdx.y * kQuantGroups + (lane >> 4), c = g * kB + (lane & 15) * 8;
+    const unsigned gtiles = (groups + kQuantGroups - 1) / kQuantGroups;
+    const int g = blockIdx.x % gtiles * kQuantGroups + (lane >> 4), c = g * kB + (lane & 15) * 8;
     if (g >= groups) return;
-    const int64_t v0 = ((int64_t)blockIdx.x * kQuantWaves + wave) * R;
+    const int64_t v0 = ((int64_t)(blockIdx.x / gtiles) * kQuantWaves + wave) * R;
     const float top = largest_finite<T>();
     for (int r = 0; r < R; r += U) {
         uint2 w[U];
@@ -1154,7 +1156,7 @@ static bool many_groups(int n, int groups) { return (int64_t)(n / 64) * ((groups
 static dim3 group_grid(int n, int groups, int r)
 {
     const int64_t per = (int64_t)kQuantWaves * r;
-    return dim3((unsigned)((n + per - 1) / per), (groups + kQuantGroups - 1) / kQuantGroups);
+    return dim3((unsigned)((n + per - 1) / per * ((groups + kQuantGroups - 1) / kQuantGroups)));
 }
 
 // Tiles of 16 vectors a wave takes: `most` where that still makes `least` workgroups, else half, down to 2
