@@ -16,6 +16,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned piece __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes of a vector, wherever they lie
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -141,41 +142,46 @@ template <typename T, int K> __device__ __forceinline__ float finite_top(const R
 
 // ---- to 8 bits and back ---------------------------------------------------------------------------------------
 
-// Bound by memory.  A wave takes 4 neighbouring groups of R vectors in turn (16 lanes a group, 8 entries a lane), four loads
-// in flight; the scale bytes meet in LDS, because those of one group lie vector by vector.  R = 16 where that leaves
-// 2048 workgroups, else 1: few vectors are all latency.
+// Bound by memory.  A wave takes 4 neighbouring groups of R vectors, 16 lanes a group, a lane one 16-byte piece (of fp32 two, 64
+// entries apart): whole lines at every load and store.  Neighbouring workgroups take neighbouring columns.  16384 x 8192 of
+// bf16: to 8 bits 69 us (5.8 TB/s; 100 us with a wave on 16 vectors and neighbouring workgroups on neighbouring vectors),
+// back 57 us (117 us).
 constexpr int kQuantGroups = 4, kQuantWaves = kBlock / kWave;
 
+// The scale bytes meet in LDS, because those of one group lie vector by vector.
 template <typename T, int R>
 __global__ __launch_bounds__(kBlock) void quantize8_kernel(int n, int groups, int columns, const T *__restrict__ x, int64_t ldx,
                                                            uint8_t *__restrict__ x8, int64_t ldx8, uint8_t *__restrict__ scale,
                                                            int64_t lds)
 {
-    constexpr int U = R < 4 ? R : 4, TV = R * kQuantWaves;
+    constexpr int K = 16 / sizeof(T), H = 8 / K, TV = R * kQuantWaves;
     __shared__ uint8_t bytes[kQuantGroups][TV];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, gq = lane >> 4;
     const unsigned gtiles = (groups + kQuantGroups - 1) / kQuantGroups;
-    const int g0 = blockIdx.x % gtiles * kQuantGroups, c = (g0 + gq) * kB + (lane & 15) * 8;
+    const int g0 = blockIdx.x % gtiles * kQuantGroups, c = (g0 + gq) * kB + (lane & 15) * K;
     const int64_t v0 = (int64_t)(blockIdx.x / gtiles) * TV;
-    for (int r = 0; r < R; r += U) {
-        Raw<T, 8> a[U];
+    Raw<T, K> a[R][H];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t v = v0 + wave * R + r + u;
-            a[u].load(x + (v < n ? v : n - 1) * ldx + c, columns - c);
-        }
+    for (int r = 0; r < R; r++) {
+        const int64_t v = v0 + wave * R + r;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t v = v0 + wave * R + r + u;
-            float top = finite_top(a[u]);
+        for (int h = 0; h < H; h++) a[r][h].load(x + (v < n ? v : n - 1) * ldx + c + h * 16 * K, columns - c - h * 16 * K);
+    }
 #pragma unroll
-            for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-            const int b = scale_byte(top);
+    for (int r = 0; r < R; r++) {
+        const int64_t v = v0 + wave * R + r;
+        float top = finite_top(a[r][0]);
+        if constexpr (H == 2) top = fmaxf(top, finite_top(a[r][1]));
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        const int b = scale_byte(top);
+#pragma unroll
+        for (int h = 0; h < H; h++) {
             unsigned w[2];
-            a[u].pack(scale_value(b), w);
-            if (v < n && g0 + gq < groups) *(uint2 *)(x8 + v * ldx8 + c) = uint2{w[0], w[1]};
-            if ((lane & 15) == 0) bytes[gq][wave * R + r + u] = (uint8_t)b;
+            a[r][h].pack(scale_value(b), w);
+            if (v < n && g0 + gq < groups) __builtin_memcpy(__builtin_assume_aligned(x8 + v * ldx8 + c + h * 16 * K, K), w, K);
         }
+        if ((lane & 15) == 0) bytes[gq][wave * R + r] = (uint8_t)b;
     }
     __syncthreads();
     for (int t = threadIdx.x; t < kQuantGroups * TV; t += kBlock) {
@@ -190,44 +196,52 @@ template <> __device__ __forceinline__ float largest_finite<float>() { return 3.
 template <> __device__ __forceinline__ float largest_finite<__bf16>() { return 3.38953139e38f; }
 template <> __device__ __forceinline__ float largest_finite<_Float16>() { return 65504.0f; }
 
-template <typename T, int R>
+// ONCE: the result goes past the caches
+template <typename T, int R, bool ONCE>
 __global__ __launch_bounds__(kBlock) void restore8_kernel(int n, int groups, int columns, const uint8_t *__restrict__ x8,
                                                           int64_t ldx8, const uint8_t *__restrict__ scale, int64_t lds,
                                                           T *__restrict__ x, int64_t ldx)
 {
-    constexpr int U = R < 4 ? R : 4;
+    constexpr int K = 16 / sizeof(T), H = 8 / K;             // entries of a 16-byte store; stores a vector takes
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const unsigned gtiles = (groups + kQuantGroups - 1) / kQuantGroups;
-    const int g = blockIdx.x % gtiles * kQuantGroups + (lane >> 4), c = g * kB + (lane & 15) * 8;
+    const int g = blockIdx.x % gtiles * kQuantGroups + (lane >> 4), c0 = g * kB + (lane & 15) * K;
     if (g >= groups) return;
     const int64_t v0 = ((int64_t)(blockIdx.x / gtiles) * kQuantWaves + wave) * R;
     const float top = largest_finite<T>();
-    for (int r = 0; r < R; r += U) {
-        uint2 w[U];
-        int b[U];
+    unsigned w[R][2];
+    int b[R];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t v = v0 + r + u < n ? v0 + r + u : n - 1;
-            w[u] = *(const uint2 *)(x8 + v * ldx8 + c);
-            b[u] = scale[(int64_t)g * lds + v];
-        }
+    for (int u = 0; u < R; u++) {
+        const int64_t v = v0 + u < n ? v0 + u : n - 1;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const float s = scale_value(b[u]);
-            T y[8];
+        for (int h = 0; h < H; h++) __builtin_memcpy(&w[u][h], __builtin_assume_aligned(x8 + v * ldx8 + c0 + h * 16 * K, K), K);
+        b[u] = scale[(int64_t)g * lds + v];
+    }
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
+    for (int u = 0; u < R; u++) {
+        if (v0 + u >= n) continue;
+        const float s = scale_value(b[u]);
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            T y[K];
+#pragma unroll
+            for (int k = 0; k < K; k++) {
                 typedef float f32x2 __attribute__((ext_vector_type(2)));
-                const f32x2 p = (k & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(k < 4 ? w[u].x : w[u].y, true)
-                                        : __builtin_amdgcn_cvt_pk_f32_fp8(k < 4 ? w[u].x : w[u].y, false);
+                const unsigned d = w[u][h + k / 4];
+                const f32x2 p = (k & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(d, true) : __builtin_amdgcn_cvt_pk_f32_fp8(d, false);
                 const float f = p[k & 1] * s;
                 y[k] = (T)(f > top ? top : f < -top ? -top : f);             // NaN stays
             }
-            if (v0 + r + u >= n) continue;
-            T *o = x + (v0 + r + u) * ldx + c;
-            if (columns - c >= 8) __builtin_memcpy(o, y, sizeof y);
-            else
-                for (int k = 0; k < 8; k++)
+            const int c = c0 + h * 16 * K;
+            T *o = x + (v0 + u) * ldx + c;
+            if (columns - c >= K) {
+                        piece v;
+                __builtin_memcpy(&v, y, 16);
+                if (ONCE) __builtin_nontemporal_store(v, (piece *)o);
+                else *(piece *)o = v;
+            } else
+                for (int k = 0; k < K; k++)
                     if (k < columns - c) o[k] = y[k];
         }
     }
@@ -1152,7 +1166,7 @@ static int check_block8(const char *what, const spmv_hip_matrix *m)
     return 0;
 }
 // launch shape of quantize8 / restore8; R vectors a wave
-static bool many_groups(int n, int groups) { return (int64_t)(n / 64) * ((groups + kQuantGroups - 1) / kQuantGroups) >= 2048; }
+static bool many_groups(int n, int groups) { return (int64_t)(n / 16) * ((groups + kQuantGroups - 1) / kQuantGroups) >= 512; }
 static dim3 group_grid(int n, int groups, int r)
 {
     const int64_t per = (int64_t)kQuantWaves * r;
@@ -1361,7 +1375,7 @@ int spmv_hip_quantize8_dev(int n, int columns, const void *d_x, int dtype, int64
         auto go = [&](auto kernel, int r) {
             hipLaunchKernelGGL(kernel, group_grid(n, groups, r), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, (const T *)d_x, ldx, d_x8, ldx8, d_scale, lds);
         };
-        if (many_groups(n, groups)) go(quantize8_kernel<T, 16>, 16);
+        if (many_groups(n, groups)) go(quantize8_kernel<T, 4>, 4);
         else go(quantize8_kernel<T, 1>, 1);
     });
     return launched("quantize8");
@@ -1380,8 +1394,10 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
         auto go = [&](auto kernel, int r) {
             hipLaunchKernelGGL(kernel, group_grid(n, groups, r), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, d_x8, ldx8, d_scale, lds, (T *)d_x, ldx);
         };
-        if (many_groups(n, groups)) go(restore8_kernel<T, 16>, 16);
-        else go(restore8_kernel<T, 1>, 1);
+        // Past the caches where the 256 MB of the last one would not hold both sides (16384 x 8192 of bf16: 57 us, 67 through
+        // them), but not below (30000 x 1000 of fp32: 36 us, 24 through them)
+        if ((int64_t)n * columns * (int64_t)(sizeof(T) + 1) > (int64_t)192 << 20) go(restore8_kernel<T, 2, true>, 2);
+        else go(restore8_kernel<T, 2, false>, 2);
     });
     return launched("restore8");
 }
