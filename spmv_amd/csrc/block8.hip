@@ -1002,9 +1002,12 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
                 __builtin_memcpy(&a[s], v, 16);
             }
         }
-        between();                                           // the loads of a later stage, which take a while to issue
+        // the loads of a later stage, which take a while to issue; with three parts halfway, or registers spill (2048 vectors,
+        // 2048 blocks: 312 us, 400 before the products)
+        constexpr int THEN = PARTS == 3 ? PARTS * NU / 2 : 0;
 #pragma unroll
         for (int k = 0; k < PARTS * NU; k++) {
+            if (k == THEN) between();
             if (k + AHEAD < PARTS * NU) b[k + AHEAD] = read_b(k + AHEAD);
 #pragma unroll
             for (int s = 0; s < 4; s++) acc[k % NU][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[k], a[s], acc[k % NU][s], 0, 0, 0);
@@ -1215,7 +1218,7 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
         // dy in parts: 2, so that two workgroups fit a CU (fp32, 3000 vectors, 440 blocks: 157 us, 189 with 4).  bf16: more
         // only with 1 1/2 workgroups a CU left (777 vectors: 30 us, 42 with 4; 3000: 66 us with 8, 77 with 2)
         p.tiles = count > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2);
-        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), m->cus, 2 * (int64_t)m->nblocks / m->bcols, 4);
+        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), m->cus * (count > 1 ? 2 : 1), 2 * (int64_t)m->nblocks / m->bcols, 4);
         p.dx_slice = (int64_t)n * m->bcols * kB;
     }
     if (with_dv && m->nblocks) {
