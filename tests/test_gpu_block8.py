@@ -270,6 +270,113 @@ def test_gradient(rows, columns, keep, dy_dtype, dv_dtype):
             _close(out, want + _np(base), n * 3 + 1, magnitude + np.abs(_np(base)))
 
 
+# ---- the larger tiles, pairs of blocks and cut sums -------------------------------------------------------------------
+
+def _close_64(got, want, terms, magnitude, extra=0.0):
+    """_close with 64-bit tensors on the GPU"""
+    eps = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * 2 * eps
+    err = (got.double() - want).abs()
+    tol = (terms * 2.0 ** -23 + extra) * magnitude * (1 + eps) + eps * want.abs() + tiny
+    assert got.shape == want.shape and bool((err <= tol).all()), float((err / tol.clamp(min=1e-300)).max())
+
+
+def _on_gpu(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+
+
+# rows, columns, share of blocks, vectors: 33 block rows (or columns) x 4, 8 or 16 tiles of vectors a workgroup, and 18
+# blocks a row for the 16 waves of few vectors
+@pytest.mark.parametrize("rows,columns,keep,counts", [(700, 2300, 1.0, [1, 13, 31, 64]), (4200, 500, 0.7, [1000, 2050]), (4100, 150, 1.0, [700])])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product_larger(rows, columns, keep, counts, dtype):
+    c = Case(rows, columns, keep, rows + columns)
+    a, mag = _on_gpu(c.dense.T), _on_gpu(c.dense_abs.T)
+    for n in counts:
+        x = _vectors(n, columns, dtype, n)
+        xq = _on_gpu(O.quantized(_np(x)))
+        extra = EIGHT if dtype == BF16 and n > 64 else 0.0
+        _close_64(c.A.product(x), torch.mm(xq, a), columns, torch.mm(xq.abs(), mag), extra)
+
+
+@pytest.mark.parametrize("rows,columns,keep,counts", [(500, 4200, 0.7, [700, 1500, 2900]), (5200, 200, 0.8, [1, 5, 40, 130]), (3001, 130, 1.0, [3, 65, 700]),
+                                                      (9000, 64, 0.5, [2, 20])])
+@pytest.mark.parametrize("dy_dtype,dx_dtype", [(F32, F32), (BF16, BF16), (F16, F16), (BF16, F32), (F32, BF16)])
+def test_product_t_larger_and_cut(rows, columns, keep, counts, dy_dtype, dx_dtype):
+    c = Case(rows, columns, keep, rows + columns)
+    a, mag = _on_gpu(c.dense), _on_gpu(c.dense_abs)
+    for n in counts:
+        # beyond a row's end lies what must not be read, or not be used
+        wide = torch.full((n, rows + 24), float("nan"), dtype=dy_dtype, device=DEV)
+        for dy in (_vectors(n, rows, dy_dtype, n), wide[:, :rows]):
+            dy.copy_(_vectors(n, rows, dy_dtype, n))
+            got = c.A.product_t(dy, dx_dtype)
+            _close_64(got, torch.mm(dy.double(), a), rows * (3 if dy_dtype == F32 else 2), torch.mm(dy.double().abs(), mag))
+            assert torch.equal(c.A.product_t(dy, dx_dtype), got)
+
+
+@pytest.mark.parametrize("rows,columns,keep,counts", [(4200, 4200, 0.5, [1, 33, 70, 200]), (130, 300, 1.0, [512, 1000, 2111]), (100, 1, 1.0, [4000]),
+                                                      (2001, 1500, 0.6, [1999])])
+@pytest.mark.parametrize("dy_dtype,dv_dtype", [(F32, F32), (BF16, F32), (F16, F16), (BF16, BF16)])
+def test_gradient_larger_and_cut(rows, columns, keep, counts, dy_dtype, dv_dtype):
+    c = Case(rows, columns, keep, rows + columns)
+    for n in counts:
+        x = _vectors(n, columns, dy_dtype, n)
+        q = quantize(x)
+        xq = _on_gpu(O.quantized(_np(x)))
+        wide = torch.full((n, rows + 24), float("nan"), dtype=dy_dtype, device=DEV)
+        for dy in (_vectors(n, rows, dy_dtype, n), wide[:, :rows]):
+            dy.copy_(_vectors(n, rows, dy_dtype, n + 1, 0.5))
+            d = dy.double()
+            want = _on_gpu(O.sampled(torch.mm(d.t().contiguous(), xq).cpu().numpy(), c.ptr, c.col))
+            magnitude = _on_gpu(O.sampled(torch.mm(d.abs().t().contiguous(), xq.abs()).cpu().numpy(), c.ptr, c.col))
+            dv = c.A.gradient(dy, q, dv_dtype)
+            _close_64(dv, want, n * (3 if dy_dtype == F32 else 2), magnitude)
+            assert torch.equal(c.A.gradient(dy, q, dv_dtype), dv)
+        base = torch.randn(dv.shape, device=DEV).to(dv_dtype)
+        out = base.clone()
+        c.A.gradient(dy, q, out=out, accumulate=True)
+        _close_64(out, want + base.double(), n * 3 + 1, magnitude + base.double().abs())
+
+
+def test_a_cut_gradient_replays_and_does_not_share_its_workspace():
+    """Two captured graphs and an eager call, all of cut sums on one handle, replayed in turn."""
+    c = Case(1500, 250, 0.9, 21)
+    runs = []
+    for k, n in enumerate((900, 4)):
+        x, dy = _vectors(n, 250, F16, k), _vectors(n, 1500, F16, 10 + k)
+        q = quantize(x)
+        f = lambda q=q, dy=dy: (c.A.product_t(dy), c.A.gradient(dy, q))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            f()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f()
+        runs.append((graph, out, f, dy))
+    for k in range(4):
+        for graph, out, f, dy in runs:
+            dy.copy_(_vectors(dy.shape[0], 1500, F16, 30 + k))
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, out, f, dy in runs:
+            assert all(torch.equal(a, b) for a, b in zip(out, f())), k
+
+
+@pytest.mark.parametrize("dtype,n", [(F32, 5500), (BF16, 9000)])
+def test_results_larger_than_the_last_cache(dtype, n):
+    """restore past the caches against restore through them, of the same vectors in two halves"""
+    columns = 7700
+    q = quantize(torch.randn(n, columns, device=DEV).to(dtype))
+    back = q.restore()
+    half = n // 2
+    for rows in (slice(0, half), slice(half, n)):
+        part = Packed8(q.values[rows], q.scale[:, rows].contiguous(), columns, dtype)
+        assert torch.equal(part.restore(), back[rows])
+
+
 def test_two_blocks_at_one_place_add_up_and_get_a_gradient_each():
     ptr, col = np.array([0, 3], np.int32), np.array([1, 0, 1], np.int32)
     A = Block8(100, 200, ptr, col)
