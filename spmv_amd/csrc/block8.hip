@@ -1481,6 +1481,7 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
     }
     if (plan.work && (uintptr_t)d_work % 16) { set_error("%s: workspace is not 16-byte aligned", what); return 1; }
     if (!d_dx && !d_dvalues) return 0;
+    if (n == 1) lddy = m->rows;                               // bounds the loads; the caller's says nothing
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
     const hipStream_t st = (hipStream_t)stream;

@@ -172,6 +172,28 @@ def test_abi_strides_leave_the_gaps_alone():
     assert torch.all(dv[-1] == -5.0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_abi_one_vector_needs_no_distance(dtype):
+    """n = 1: whatever stands for the distance to the next vector"""
+    c = Case(600, 300, 0.9, 6)
+    x, dy = _vectors(1, 300, dtype, 1), _vectors(1, 600, dtype, 2)
+    q, L, st = quantize(x), S.lib(), torch.cuda.current_stream().cuda_stream
+    code = {F32: S.F32, BF16: S.BF16, F16: S.F16}[dtype]
+    want_dx, want_dv = c.A.product_t(dy), c.A.gradient(dy, q)
+    for ld in (0, 600, 1 << 40):
+        dx, dv = torch.full_like(want_dx, -5.0), torch.full_like(want_dv, -5.0)
+        work = torch.empty(L.spmv_hip_block8_backward_work(c.A._h, 1, dy.data_ptr(), code, ld, 1, 1) + 16, dtype=torch.uint8, device=DEV)
+        S.check(L.spmv_hip_block8_backward_dev(c.A._h, 1, dy.data_ptr(), code, ld, q.values.data_ptr(), 384, q.scale.data_ptr(), 1, dx.data_ptr(),
+                                               code, ld, dv.data_ptr(), S.F32, 0, work.data_ptr(), st))
+        assert torch.equal(dx, want_dx) and torch.equal(dv, want_dv)
+        y = torch.full((1, 600), -5.0, dtype=dtype, device=DEV)
+        S.check(L.spmv_hip_block8_mult_dev(c.A._h, 1, x.data_ptr(), code, ld, None, 0, y.data_ptr(), code, ld, st))
+        assert torch.equal(y, c.A.product(x))
+        x8, sc = torch.zeros_like(q.values), torch.zeros_like(q.scale)
+        S.check(L.spmv_hip_quantize8_dev(1, 300, x.data_ptr(), code, ld, x8.data_ptr(), 384, sc.data_ptr(), 1, st))
+        assert torch.equal(x8, q.values) and torch.equal(sc, q.scale)
+
+
 # ---- the matrix -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -634,6 +656,38 @@ def test_captured_step_replays_with_new_inputs():
         x.copy_(_vectors(n, 520, BF16, 20 + k))
         dy.copy_(_vectors(n, 390, BF16, 30 + k))
         few.copy_(_vectors(3, 520, BF16, 40 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), k
+
+
+def test_captured_training_step_through_linear():
+    """set_values, linear and its backward pass in one graph; nothing of an eager pass alive meanwhile"""
+    c = Case(390, 520, 0.7, 19)
+    n = 100
+    w = c.values.to(DEV).requires_grad_()
+    x, dy = _vectors(n, 520, BF16, 1).requires_grad_(), _vectors(n, 390, BF16, 2)
+
+    def step():
+        c.A.set_values(w)
+        y = c.A.linear(x)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            w.copy_(torch.randn(w.shape) * 2.0 ** (k - 2))
+            x.copy_(_vectors(n, 520, BF16, 20 + k))
+        dy.copy_(_vectors(n, 390, BF16, 30 + k))
         graph.replay()
         torch.cuda.synchronize()
         got = [t.clone() for t in out]
