@@ -399,6 +399,23 @@ def test_results_larger_than_the_last_cache(dtype, n):
         assert torch.equal(part.restore(), back[rows])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_vectors_and_many_blocks(dtype):
+    """from some size on x is rounded before the product: the same bits as inside it"""
+    c = Case(4000, 3900, 1.0, 22)
+    a, mag = _on_gpu(c.dense.T), _on_gpu(c.dense_abs.T)
+    code = {F32: S.F32, BF16: S.BF16, F16: S.F16}[dtype]
+    for n in (1, 8, 16, 17, 33, 64):
+        x = _vectors(n, 3900, dtype, n)
+        y = c.A.product(x)
+        inside = torch.empty_like(y)
+        S.check(S.lib().spmv_hip_block8_mult_dev(c.A._h, n, x.data_ptr(), code, 3900, None, 0, inside.data_ptr(), code, 4000,
+                                                 torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(y, inside)
+        xq = _on_gpu(O.quantized(_np(x)))
+        _close_64(y, torch.mm(xq, a), 3900, torch.mm(xq.abs(), mag))
+
+
 def test_two_blocks_at_one_place_add_up_and_get_a_gradient_each():
     ptr, col = np.array([0, 3], np.int32), np.array([1, 0, 1], np.int32)
     A = Block8(100, 200, ptr, col)
