@@ -113,9 +113,7 @@ class Packed8:
         return x
 
 
-def quantize(x: torch.Tensor) -> Packed8:
-    """x [..., columns] to 8 bits."""
-    rows = _wide("x", x.detach() if isinstance(x, torch.Tensor) else x)
+def _rounded(rows: torch.Tensor, shape) -> Packed8:
     n, columns = rows.shape
     groups = -(-columns // BLOCK)
     device = rows.device
@@ -124,7 +122,12 @@ def quantize(x: torch.Tensor) -> Packed8:
     with _On(device):
         L.check(L.lib().spmv_hip_quantize8_dev(n, columns, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows), values.data_ptr(),
                                                groups * BLOCK, scale.data_ptr(), n, _raw_stream(device.index)))
-    return Packed8._made(values, scale, columns, rows.dtype, x.shape)
+    return Packed8._made(values, scale, columns, rows.dtype, shape)
+
+
+def quantize(x: torch.Tensor) -> Packed8:
+    """x [..., columns] to 8 bits."""
+    return _rounded(_wide("x", x.detach() if isinstance(x, torch.Tensor) else x), x.shape)
 
 
 class Block8(Matrix):
@@ -201,15 +204,16 @@ class Block8(Matrix):
             rows = _wide("x", x.detach() if isinstance(x, torch.Tensor) else x, self.columns)
             self._here("x", rows)
             shape = (*x.shape[:-1], self.rows)
-            # Rounded inside the product, by every strip of rows again, where that costs less than a call to quantize (bytes
-            # of x times blocks; fp32, 16 vectors: 1024 blocks 15 us inside, 17 before; 1920 blocks 31 and 17 us).
-            if rows.shape[0] <= MAX_WIDE and rows.shape[0] * rows.element_size() * self.nblocks < 66000:
+            # Rounded inside the product, by every workgroup again, where that costs less than a call to quantize (bf16,
+            # 1920 blocks: 16 vectors 11 us inside, 17 before; 32 vectors 26 and 17 us; 4096 blocks, 16 vectors 17 and 17 us)
+            n = rows.shape[0]
+            if n <= MAX_WIDE and self.nblocks * (-(-n // 16) * rows.element_size()) < (8500 if n <= 16 else 7500):
                 y = self._out(out, shape, dtype or rows.dtype, rows)
-                L.check(L.lib().spmv_hip_block8_mult_dev(self._h, rows.shape[0], rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
+                L.check(L.lib().spmv_hip_block8_mult_dev(self._h, n, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
                                                          None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _raw_stream(self._index)))
                 return y
             dtype = dtype or rows.dtype
-            x = quantize(rows)
+            x = _rounded(rows, rows.shape)
         else:
             if x.columns != self.columns:
                 raise ValueError(f"x has {x.columns} columns, the matrix {self.columns}")
@@ -274,9 +278,9 @@ class Block8(Matrix):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, values, matrix):
-        _wide("x", x, matrix.columns)
-        matrix._here("x", x)
-        q = quantize(x)
+        rows = _wide("x", x, matrix.columns)
+        matrix._here("x", rows)
+        q = _rounded(rows, x.shape)
         ctx.save_for_backward(q.values, q.scale)
         ctx.matrix, ctx.version, ctx.x_shape, ctx.x_dtype = matrix, matrix._version, x.shape, x.dtype
         ctx.values_dtype = values.dtype if values is not None else None

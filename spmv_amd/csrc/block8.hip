@@ -51,6 +51,8 @@ __device__ __forceinline__ void unpack4(unsigned w, float scale, __bf16 *out)
     out[0] = lo[0]; out[1] = lo[1]; out[2] = hi[0]; out[3] = hi[1];
 }
 
+template <int V> using ic = std::integral_constant<int, V>;
+
 template <int DT> struct elem;
 template <> struct elem<SPMV_HIP_F32> { typedef float type; };
 template <> struct elem<SPMV_HIP_BF16> { typedef __bf16 type; };
@@ -337,12 +339,13 @@ __device__ __forceinline__ int table(const int *p, int k)
 
 // ---- few vectors ----------------------------------------------------------------------------------------------
 
-// One workgroup per strip of 16 rows; its W waves take the strip's blocks in turn and add their results in LDS.
-// Bound by reading the matrix once, and for small matrices by latency: a wave's next block is on its way while
-// it works on one.  NT tiles of 16 vectors.  XT: uint8_t (x in 8 bits) or a wide type, rounded to 8 bits
+// One workgroup per S strips of 16 rows; its W waves take the strips' blocks in turn and add their results in LDS.
+// Bound by reading the matrix once (8192 x 8192, up to 16 vectors in 8 bits: 12.5 us, 5.4 TB/s), for small matrices by
+// latency -- a wave's next block is on its way while it works on one -- and with more vectors by widening x, which every
+// strip's workgroup does again: two strips share it.  NT tiles of 16 vectors.  XT: uint8_t (x in 8 bits) or a wide type, rounded to 8 bits
 // here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.  Operands are widened
 // to bf16 (exact), sums are 32 bits.
-template <typename XT, int NT, int W>
+template <typename XT, int NT, int W, int S>
 __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, int columns, const int *__restrict__ block_ptr,
                                                                const int *__restrict__ block_col, const uint8_t *__restrict__ val8,
                                                                const int *__restrict__ scale8, const XT *__restrict__ x,
@@ -351,11 +354,13 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
 {
     constexpr bool kEight = std::is_same<XT, uint8_t>::value;
     __shared__ f32x4 part[W][NT][kWave];
-    const int brow = blockIdx.x >> 3, strip = blockIdx.x & 7;
+    const int brow = blockIdx.x / (8 / S), strip0 = blockIdx.x % (8 / S) * S;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), i = lane & 15, q = lane >> 4;
-    f32x4 acc[NT];
+    f32x4 acc[S][NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
+    for (int k = 0; k < S; k++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[k][t] = f32x4{0, 0, 0, 0};
     // vectors past the last read the last: a column of the result that is not stored
     int64_t vec[NT];
 #pragma unroll
@@ -367,7 +372,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         int scale;
     };
     struct Stage {
-        u32x4 a[2];
+        u32x4 a[S][2];
         int scale, group;
         Vector x[AHEAD ? NT : 1];
     };
@@ -387,9 +392,9 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
     };
     auto load = [&](int b) {
         Stage s;
-        const uint8_t *block = val8 + (int64_t)b * kBlockBytes + (strip * 2 * kWave + lane) * 16;
-        s.a[0] = *(const u32x4 *)block;
-        s.a[1] = *(const u32x4 *)(block + kWave * 16);
+        const uint8_t *block = val8 + (int64_t)b * kBlockBytes + (strip0 * 2 * kWave + lane) * 16;
+#pragma unroll
+        for (int k = 0; k < 2 * S; k++) s.a[k >> 1][k & 1] = *(const u32x4 *)(block + k * kWave * 16);
         s.scale = table(scale8, b);
         s.group = table(block_col, b);
         if constexpr (AHEAD)
@@ -399,9 +404,9 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
     };
     auto use = [&](const Stage &s) {
         const float sa = scale_value(s.scale);
-        bf16x8 a[4];
+        bf16x8 a[S][4];
 #pragma unroll
-        for (int d = 0; d < 8; d++) unpack4(s.a[d >> 2][d & 3], sa, (__bf16 *)&a[d >> 1] + 4 * (d & 1));
+        for (int d = 0; d < 8 * S; d++) unpack4(s.a[d >> 3][d >> 2 & 1][d & 3], sa, (__bf16 *)&a[d >> 3][d >> 1 & 3] + 4 * (d & 1));
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const Vector v = AHEAD ? s.x[AHEAD ? t : 0] : load_x(t, s.group);
@@ -423,7 +428,8 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
                 bf16x8 b;
                 unpack4(w8[2 * p], sx, (__bf16 *)&b);
                 unpack4(w8[2 * p + 1], sx, (__bf16 *)&b + 4);
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], b, acc[t], 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < S; k++) acc[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k][p], b, acc[k][t], 0, 0, 0);
             }
         }
     };
@@ -437,21 +443,26 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; t++) part[wave][t][lane] = acc[t];
-    __syncthreads();
-    for (int id = threadIdx.x; id < NT * kWave; id += W * kWave) {
-        const int t = id / kWave, l = id & (kWave - 1), v = t * 16 + (l & 15);
-        f32x4 s = part[0][t][l];
+    for (int k = 0; k < S; k++) {
+        const int strip = strip0 + k;
+        if (k) __syncthreads();
 #pragma unroll
-        for (int w = 1; w < W; w++) s += part[w][t][l];
-        const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + (strip & 3);
-        if (v >= n) continue;
-        for (int k = 0; k < 4; k++) {
-            if (r0 + 4 * k >= rows) break;
-            const int64_t at = (int64_t)v * ldy + r0 + 4 * k;
-            if (y_dtype == SPMV_HIP_F32) ((float *)y)[at] = s[k];
-            else if (y_dtype == SPMV_HIP_BF16) ((__bf16 *)y)[at] = (__bf16)s[k];
-            else ((_Float16 *)y)[at] = (_Float16)s[k];
+        for (int t = 0; t < NT; t++) part[wave][t][lane] = acc[k][t];
+        __syncthreads();
+        for (int id = threadIdx.x; id < NT * kWave; id += W * kWave) {
+            const int t = id / kWave, l = id & (kWave - 1), v = t * 16 + (l & 15);
+            f32x4 s = part[0][t][l];
+#pragma unroll
+            for (int w = 1; w < W; w++) s += part[w][t][l];
+            const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + (strip & 3);
+            if (v >= n) continue;
+            for (int e = 0; e < 4; e++) {
+                if (r0 + 4 * e >= rows) break;
+                const int64_t at = (int64_t)v * ldy + r0 + 4 * e;
+                if (y_dtype == SPMV_HIP_F32) ((float *)y)[at] = s[e];
+                else if (y_dtype == SPMV_HIP_BF16) ((__bf16 *)y)[at] = (__bf16)s[e];
+                else ((_Float16 *)y)[at] = (_Float16)s[e];
+            }
         }
     }
 }
@@ -464,7 +475,6 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
 // loads are issued R - 1 steps ahead: one step where two workgroups of 256 vectors share a CU and cover each other's waits,
 // three where there are few workgroups and a step is short.
 
-template <int V> using ic = std::integral_constant<int, V>;
 
 // Keeps a scalar load where it is written: the compiler would move it down to its use in the next step, and wait there
 __device__ __forceinline__ void here(int &a) { asm volatile("" : "+s"(a)); }
@@ -1100,22 +1110,25 @@ static int groups_of(int length) { return length / kB + (length % kB != 0); }
 static int launch_few(const spmv_hip_matrix *m, int n, const void *x, int x_dtype, int64_t ldx, const uint8_t *xscale,
                       int64_t lds, void *y, int y_dtype, int64_t ldy, hipStream_t st)
 {
-    // 16 waves a strip where every one of them gets a block, else 4
-    const bool many_waves = m->nblocks >= 16 * (int64_t)m->brows;
+    // 16 waves a workgroup where every one of them gets a block, else 4; two strips a workgroup where that leaves workgroups
+    // for two CUs in three (8 bits, 64 vectors: 8192 x 8192 37.7 us with one, 22.3 with two; 4096 x 4096 11.1 and 12.4)
+    const bool many_waves = m->nblocks >= 16 * (int64_t)m->brows, pairs = m->brows * (int64_t)6 >= m->cus;
     auto go = [&](auto t) {
         typedef decltype(t) XT;
-        auto launch = [&](auto kernel, int waves) {
-            hipLaunchKernelGGL(kernel, dim3(m->brows * 8), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
+        auto launch = [&](auto kernel, int waves, int strips) {
+            hipLaunchKernelGGL(kernel, dim3(m->brows * (8 / strips)), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
                                m->d_block_col, m->d_val8, m->d_scale8, (const XT *)x, ldx, xscale, lds, y, y_dtype, ldy);
         };
-        auto tiles = [&](auto w) {
-            constexpr int W = decltype(w)::value;
-            if (n <= 16) launch(few_vectors_kernel<XT, 1, W>, W);
-            else if (n <= 32) launch(few_vectors_kernel<XT, 2, W>, W);
-            else launch(few_vectors_kernel<XT, 4, W>, W);
+        auto tiles = [&](auto w, auto two) {
+            constexpr int W = decltype(w)::value, S = decltype(two)::value;
+            if (n <= 16) launch(few_vectors_kernel<XT, 1, W, S>, W, S);
+            else if (n <= 32) launch(few_vectors_kernel<XT, 2, W, S>, W, S);
+            else launch(few_vectors_kernel<XT, 4, W, S>, W, S);
         };
-        if (many_waves) tiles(std::integral_constant<int, 16>());
-        else tiles(std::integral_constant<int, 4>());
+        if (many_waves && pairs) tiles(ic<16>(), ic<2>());
+        else if (many_waves) tiles(ic<16>(), ic<1>());
+        else if (pairs) tiles(ic<4>(), ic<2>());
+        else tiles(ic<4>(), ic<1>());
     };
     if (x_dtype == SPMV_HIP_E4M3) go(uint8_t());
     else with_elem(x_dtype, go);
