@@ -1211,11 +1211,19 @@ struct BackwardPlan {
     int64_t dx_slice, dv_slice, parts_bytes, work;
 };
 
-// Slices of a sum of `steps` steps whose `tiles` workgroups leave much of the GPU idle: as many as make `wgs` workgroups,
-// `least` steps each or more
-static int slices(int64_t tiles, int64_t wgs, int64_t steps, int least)
+// Slices to cut sums of `steps` steps into, whose `tiles` workgroups leave CUs idle: as many as take the least time by
+// what was measured -- `step` us a step, 1.4 times that where two workgroups share a CU; the slices, `bytes` each, written and
+// read again at 4 TB/s, and 6 us for the launch that adds them.  (dx of 96 tiles x 80 steps of fp32: 106 us in one piece, 47
+// cut; of 132 tiles x 16 steps of fp16: 17 us in one, 22 in three.)
+static int slices(int64_t tiles, int64_t steps, int cus, float step, int64_t bytes)
 {
-    return (int)std::max<int64_t>(1, std::min(wgs / tiles, steps / least));
+    int best = 1;
+    float least = steps * step;
+    for (int64_t k = 2; k * tiles <= 2 * cus && k <= steps; k += k / 2) {
+        const float us = (steps + k - 1) / k * step * (k * tiles > cus ? 1.4f : 1.0f) + 6.0f + k * bytes * 0.5e-6f;
+        if (us < least) { least = us; best = (int)k; }
+    }
+    return best;
 }
 
 static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d_dy, int dtype, int64_t lddy, bool with_dx, bool with_dv)
@@ -1231,16 +1239,16 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
         // dy in parts: 2, so that two workgroups fit a CU (fp32, 3000 vectors, 440 blocks: 157 us, 189 with 4).  bf16: more
         // only with 1 1/2 workgroups a CU left (777 vectors: 30 us, 42 with 4; 3000: 66 us with 8, 77 with 2)
         p.tiles = count > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2);
-        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), m->cus * (count > 1 ? 2 : 1), 2 * (int64_t)m->nblocks / m->bcols, 4);
         p.dx_slice = (int64_t)n * m->bcols * kB;
+        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), 2 * (int64_t)m->nblocks / m->bcols, m->cus,
+                             0.1f + 0.25f * count, p.dx_slice * 4);
     }
     if (with_dv && m->nblocks) {
         // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
         // registers; and not where many pairs lack their second block
         p.pairs = m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
-        const int tiles = p.pairs ? m->npairs : m->nblocks;
-        p.dv_slices = slices(tiles, 2 * m->cus, n / 32, 16 + tiles / 8);
         p.dv_slice = (int64_t)m->nblocks * kBlockBytes;
+        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, n / 32, m->cus, 0.1f + 0.2f * count, p.dv_slice * 4);
     }
     p.work = p.parts_bytes + 4 * std::max(p.dx_slices > 1 ? p.dx_slices * p.dx_slice : 0, p.dv_slices > 1 ? p.dv_slices * p.dv_slice : 0);
     return p;
