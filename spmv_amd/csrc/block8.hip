@@ -14,6 +14,7 @@ namespace spmv {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned piece __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes of a vector, wherever they lie
@@ -42,6 +43,13 @@ __device__ __forceinline__ int scale_byte(float amax)
     if (amax == 0.0f) return 127;
     const int e = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 8;      // exponent byte of the scale
     return e < 1 ? 1 : e;
+}
+__device__ __forceinline__ void unpack4(unsigned w, float scale, _Float16 *out)      // exact where fp16 holds the results
+{
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false);
+    const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true);
+    out[0] = lo[0]; out[1] = lo[1]; out[2] = hi[0]; out[3] = hi[1];
 }
 // four e4m3 bytes times a power of two -> four bf16, exact
 __device__ __forceinline__ void unpack4(unsigned w, float scale, __bf16 *out)
@@ -719,23 +727,29 @@ __global__ __launch_bounds__(kBlock) void split_kernel(int n, int length, int ld
     else
 #pragma unroll
         for (int e = 0; e < 8; e++) {
+            // each part the upper half of what is left, cut off, not rounded: the largest numbers would round to infinity
             float f = (float)r.v[e];
             const bool finite = fabsf(f) < __builtin_inff(); // infinities and NaN: all in the first
 #pragma unroll
             for (int p = 0; p < PARTS; p++) {
-                part[p][e] = (__bf16)f;
-                f = finite ? f - (float)part[p][e] : 0.0f;
+                const float top = finite ? __uint_as_float(__float_as_uint(f) & 0xffff0000u) : f;
+                part[p][e] = (__bf16)top;
+                f = finite ? f - top : 0.0f;
             }
         }
 #pragma unroll
     for (int p = 0; p < PARTS; p++) *(bf16x8 *)(out + p * plane + at) = part[p];
 }
 
+template <typename E> using x8 = E __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
 struct TransposedArgs {
     int n, rows, columns, bcols, vtiles;
     const int *ptr, *row, *id, *scale;               // lists by block column, their blocks' scales
     const uint8_t *val8;
-    const __bf16 *dy;
+    const void *dy;
     int64_t lddy, plane, lddx, slice;    // plane: from one part of dy to the next; slice: of dx, where the sum is cut
 };
 
@@ -745,9 +759,11 @@ struct TransposedArgs {
 // with the strip, which puts the four on different banks.  The blocks of a last block row that is not whole come last in
 // every list: they are taken after the others, one by one, with the entries past the end masked (dy in parts is padded
 // and has no such rows).
-template <int PARTS, int NU, typename OT>
+template <typename E, int PARTS, int NU, typename OT>
 __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g, OT *__restrict__ dx)
 {
+    constexpr bool HALF = std::is_same<E, _Float16>::value;
+    typedef x8<E> e8;
     constexpr int R = PARTS * NU >= 6 ? 2 : PARTS * NU == 4 ? 3 : 4, TOK = 32 * NU;
     __shared__ uint8_t Y[R][PARTS][TOK * 128];
     __shared__ uint8_t A[R][kBlockBytes / 2];
@@ -776,7 +792,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
 
     // piece j of a thread: 8 entries of vector 32 j + 8 wave + lane / 8, in place lane % 8 of its row in LDS; a
     // row's pieces are exchanged by XOR.  Past the last vector: the last, its result is not stored.
-    const __bf16 *ybase = g.dy + (int64_t)t0 * g.lddy;
+    const E *ybase = (const E *)g.dy + (int64_t)t0 * g.lddy;
     const int row_of_lane = wave * 8 + (lane >> 3), piece = (lane & 7) ^ ((row_of_lane >> 1) & 7);
     const unsigned lddy = (unsigned)g.lddy, near = row_of_lane * lddy + 8 * piece;
     u32x4 ys[PARTS];
@@ -822,10 +838,10 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         };
         auto read_b = [&](int h, int part, int u) {
             const int t = wn * 16 * NU + 16 * u + i;
-            return *(const bf16x8 *)&Y[S][part][t * 128 + (((4 * h + q) ^ ((t >> 1) & 7)) << 4)];
+            return *(const e8 *)&Y[S][part][t * 128 + (((4 * h + q) ^ ((t >> 1) & 7)) << 4)];
         };
         i32x2 w[2][4];
-        bf16x8 b[2][PARTS][NU];
+        e8 b[2][PARTS][NU];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
 #pragma unroll
@@ -838,28 +854,53 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         }
         const float fa = scale_value(sa[S]);
         between();
+        e8 a[2][4];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            if constexpr (!ALL)
+            if constexpr (!ALL && !HALF)
                 if (h == 1) {
 #pragma unroll
                     for (int part = 0; part < PARTS; part++) b[1][part][0] = read_b(1, part, 0);
                 }
-            bf16x8 a[4];
+            if constexpr (HALF) {
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                unpack4((unsigned)w[h][s][0], fa, (__bf16 *)&a[s]);
-                unpack4((unsigned)w[h][s][1], fa, (__bf16 *)&a[s] + 4);
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int d = 0; d < 2; d++) unpack4((unsigned)w[h][s][d], 1.0f, (E *)&a[h][s] + 4 * d);
+                continue;
             }
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int d = 0; d < 2; d++) unpack4((unsigned)w[h][s][d], fa, (E *)&a[h][s] + 4 * d);
 #pragma unroll
             for (int part = 0; part < PARTS; part++)
 #pragma unroll
                 for (int u = 0; u < NU; u++) {
                     if constexpr (!ALL) if (u + 1 < NU) b[h][part][u + 1] = read_b(h, part, u + 1);
 #pragma unroll
-                    for (int s = 0; s < 4; s++) acc[u][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], b[h][part][u], acc[u][s], 0, 0, 0);
+                    for (int s = 0; s < 4; s++) acc[u][s] = mfma(a[h][s], b[h][part][u], acc[u][s]);
                     if (NU == 8 && (u & 1)) __builtin_amdgcn_sched_barrier(0);
                 }
+        }
+        if constexpr (HALF) {
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                if (!ALL && u) {
+                    b[0][0][u] = read_b(0, 0, u);
+                    b[1][0][u] = read_b(1, 0, u);
+                } else if (!ALL) b[1][0][0] = read_b(1, 0, 0);
+                f32x4 t[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) t[s] = mfma(a[0][s], b[0][0][u], f32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int s = 0; s < 4; s++) t[s] = mfma(a[1][s], b[1][0][u], t[s]);
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[u][s][r] = __builtin_fmaf(t[s][r], fa, acc[u][s][r]);
+                if (NU == 8) __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     auto step = [&](auto slot, int k) {
@@ -883,7 +924,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         issue_block(ic<0>(), k);
         const int r = row * kB + (k & 1) * 64;
         for (int j = 0; j < NU; j++) {
-            Raw<__bf16, 8> one;
+            Raw<E, 8> one;
             one.load(ybase + r + (unsigned)min(j * 32 + row_of_lane, g.n - 1 - t0) * lddy + 8 * piece, g.rows - (r + 8 * piece));
             __builtin_memcpy(&Y[0][0][(j * 32 + wave * 8) * 128 + lane * 16], one.v, 16);
         }
@@ -1203,24 +1244,24 @@ static int check_tiles(const char *what, int majors, int vtiles)
     return 1;
 }
 
-// How a backward call runs; `work` in bytes: the parts of dy, then the slices of a cut sum
+// How a backward call runs; `work` in bytes: the parts of dy, its copy for dx, then the slices of a cut sum
 struct BackwardPlan {
-    bool split;                    // dy goes into its parts first
+    int dx_parts, dv_parts;        // bf16 numbers an entry of dy is taken as
     bool pairs;                    // two blocks of a block row a workgroup
     int tiles, dx_slices, dv_slices;
-    int64_t dx_slice, dv_slice, parts_bytes, work;
+    int64_t dx_slice, dv_slice, parts_bytes, copy_bytes, work;
 };
 
 // Slices to cut sums of `steps` steps into, whose `tiles` workgroups leave CUs idle: as many as take the least time by
 // what was measured -- `step` us a step, 1.4 times that where two workgroups share a CU; the slices, `bytes` each, written and
-// read again at 4 TB/s, and 6 us for the launch that adds them.  (dx of 96 tiles x 80 steps of fp32: 106 us in one piece, 47
+// read again at 4 TB/s, and 5 us for the launch that adds them.  (dx of 96 tiles x 80 steps of fp32: 106 us in one piece, 47
 // cut; of 132 tiles x 16 steps of fp16: 17 us in one, 22 in three.)
 static int slices(int64_t tiles, int64_t steps, int cus, float step, int64_t bytes)
 {
     int best = 1;
     float least = steps * step;
     for (int64_t k = 2; k * tiles <= 2 * cus && k <= steps; k += k / 2) {
-        const float us = (steps + k - 1) / k * step * (k * tiles > cus ? 1.4f : 1.0f) + 6.0f + k * bytes * 0.5e-6f;
+        const float us = (steps + k - 1) / k * step * (k * tiles > cus ? 1.4f : 1.0f) + 5.0f + k * bytes * 0.5e-6f;
         if (us < least) { least = us; best = (int)k; }
     }
     return best;
@@ -1231,26 +1272,32 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
     BackwardPlan p{};
     p.dx_slices = p.dv_slices = 1;
     if (n <= 0) return p;
-    // dy goes into the products as it lies: bf16 with 16-byte aligned vectors
-    p.split = m->rows > 0 && (dtype != SPMV_HIP_BF16 || (uintptr_t)d_dy % 16 || (n > 1 && lddy % 8));
-    const int count = parts(dtype);
-    if (p.split) p.parts_bytes = (int64_t)count * n * m->brows * kB * 2;
+    // Into the products dy goes in bf16 parts (fp32: 3; fp16: 2, for dvalues), or as it lies (bf16; fp16, for dx), from 16-byte
+    // aligned vectors: others are copied first.
+    const bool lies = (uintptr_t)d_dy % 16 == 0 && (n == 1 || lddy % 8 == 0);
+    p.dv_parts = parts(dtype);
+    p.dx_parts = dtype == SPMV_HIP_F32 ? 3 : 1;
+    if (m->rows > 0) {
+        const int64_t plane = (int64_t)n * m->brows * kB * 2;
+        if (dtype == SPMV_HIP_F32 ? with_dx || with_dv : dtype == SPMV_HIP_F16 ? with_dv : !lies) p.parts_bytes = p.dv_parts * plane;
+        if (dtype == SPMV_HIP_F16 && with_dx && !lies) p.copy_bytes = plane;
+    }
     if (with_dx && m->bcols) {
         // dy in parts: 2, so that two workgroups fit a CU (fp32, 3000 vectors, 440 blocks: 157 us, 189 with 4).  bf16: more
         // only with 1 1/2 workgroups a CU left (777 vectors: 30 us, 42 with 4; 3000: 66 us with 8, 77 with 2)
-        p.tiles = count > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2);
+        p.tiles = p.dx_parts > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2);
         p.dx_slice = (int64_t)n * m->bcols * kB;
-        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), 2 * (int64_t)m->nblocks / m->bcols, m->cus,
-                             0.1f + 0.25f * count, p.dx_slice * 4);
+        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), 2 * (int64_t)m->longest, m->cus,
+                             0.15f + 0.25f * p.dx_parts, p.dx_slice * 4);
     }
     if (with_dv && m->nblocks) {
         // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
         // registers; and not where many pairs lack their second block
         p.pairs = m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
         p.dv_slice = (int64_t)m->nblocks * kBlockBytes;
-        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, n / 32, m->cus, 0.1f + 0.2f * count, p.dv_slice * 4);
+        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, n / 32, m->cus, 0.1f + 0.2f * p.dv_parts, p.dv_slice * 4);
     }
-    p.work = p.parts_bytes + 4 * std::max(p.dx_slices > 1 ? p.dx_slices * p.dx_slice : 0, p.dv_slices > 1 ? p.dv_slices * p.dv_slice : 0);
+    p.work = p.parts_bytes + p.copy_bytes + 4 * std::max(p.dx_slices > 1 ? p.dx_slices * p.dx_slice : 0, p.dv_slices > 1 ? p.dv_slices * p.dv_slice : 0);
     return p;
 }
 
@@ -1302,7 +1349,10 @@ spmv_hip_matrix *spmv_hip_create_block8(int rows, int columns, int nblocks, cons
                 m->nnz += (int64_t)(rows - r * kB < kB ? rows - r * kB : kB) *
                           (columns - block_col[k] * kB < kB ? columns - block_col[k] * kB : kB);
             }
-        for (int c = 0; c < bcols; c++) tptr[(size_t)c + 1] += tptr[(size_t)c];
+        for (int c = 0; c < bcols; c++) {
+            m->longest = std::max(m->longest, tptr[(size_t)c + 1]);
+            tptr[(size_t)c + 1] += tptr[(size_t)c];
+        }
         std::vector<int> at(tptr.begin(), tptr.end());
         for (int k = 0; k < nblocks; k++) {
             const int w = at[(size_t)block_col[k]]++;
@@ -1506,48 +1556,60 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
     const hipStream_t st = (hipStream_t)stream;
-    const __bf16 *dy = (const __bf16 *)d_dy;
-    int rows = m->rows;
-    int64_t plane = 0;
-    if (plan.split) {
-        rows = m->brows * kB;
-        plane = (int64_t)n * rows;
-        if (plane / 8 > (int64_t)0x7fffffff * kBlock || rows >= 1 << 23) { set_error("%s: %d vectors of %d are more than one launch takes", what, n, m->rows); return 1; }
-        with_elem(dy_dtype, [&](auto t) {
-            typedef decltype(t) T;
-            hipLaunchKernelGGL(split_kernel<T>, dim3((unsigned)((plane / 8 + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, n, m->rows, rows,
-                               (const T *)d_dy, lddy, (__bf16 *)d_work, plane);
-        });
-        dy = (const __bf16 *)d_work;
-        lddy = rows;
+    // dy and the distance of its vectors for either product; bf16 parts are padded with zeros to whole blocks
+    const void *dx_dy = d_dy, *dv_dy = d_dy;
+    int64_t dx_ld = lddy, dv_ld = lddy, plane = 0;
+    int dx_rows = m->rows, dv_rows = m->rows;
+    if (plan.parts_bytes || plan.copy_bytes) {
+        const int padded = m->brows * kB;
+        plane = (int64_t)n * padded;
+        if (plane / 8 > (int64_t)0x7fffffff * kBlock || padded >= 1 << 23) { set_error("%s: %d vectors of %d are more than one launch takes", what, n, m->rows); return 1; }
+        auto go = [&](auto kernel, auto *from, void *to) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((plane / 8 + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, n, m->rows, padded, from, lddy, (__bf16 *)to, plane);
+        };
+        if (plan.parts_bytes) {
+            with_elem(dy_dtype, [&](auto t) {
+                typedef decltype(t) T;
+                go(split_kernel<T>, (const T *)d_dy, d_work);
+            });
+            dv_dy = d_work;
+            dv_ld = dv_rows = padded;
+            if (dy_dtype != SPMV_HIP_F16) { dx_dy = d_work; dx_ld = dx_rows = padded; }
+        }
+        if (plan.copy_bytes) {                                // 16 bits as they are
+            void *to = (char *)d_work + plan.parts_bytes;
+            go(split_kernel<__bf16>, (const __bf16 *)d_dy, to);
+            dx_dy = to;
+            dx_ld = dx_rows = padded;
+        }
     }
-    float *cut = (float *)((char *)d_work + plan.parts_bytes);  // slices of dx, then of dvalues
-    const int count = parts(dy_dtype);
+    float *cut = (float *)((char *)d_work + plan.parts_bytes + plan.copy_bytes);     // slices of dx, then of dvalues
     auto with_parts = [&](auto f) {
-        if (count == 1) f(ic<1>());
-        else if (count == 2) f(ic<2>());
+        if (plan.dv_parts == 1) f(ic<1>());
+        else if (plan.dv_parts == 2) f(ic<2>());
         else f(ic<3>());
     };
     if (d_dx && n > 0 && m->columns > 0) {
         TransposedArgs a{};
-        a.n = n; a.rows = rows; a.columns = m->columns; a.bcols = m->bcols;
+        a.n = n; a.rows = dx_rows; a.columns = m->columns; a.bcols = m->bcols;
         a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale = m->d_bt_scale8;
-        a.dy = dy; a.lddy = lddy; a.plane = plane; a.slice = plan.dx_slice;
+        a.dy = dx_dy; a.lddy = dx_ld; a.plane = plane; a.slice = plan.dx_slice;
         const int nu = plan.tiles;
         a.vtiles = (n + 32 * nu - 1) / (32 * nu);
         if (check_tiles(what, m->bcols, a.vtiles)) return 1;
         auto into = [&](auto *to, int64_t ld) {
             typedef std::remove_pointer_t<decltype(to)> O;
             a.lddx = ld;
-            with_parts([&](auto p) {
-                constexpr int P = decltype(p)::value;
-                auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles, plan.dx_slices), dim3(kBlock), 0, st, a, to); };
-                if constexpr (P == 1) {
-                    if (nu == 8) { go(transposed_kernel<P, 8, O>); return; }
-                    if (nu == 4) { go(transposed_kernel<P, 4, O>); return; }
-                }
-                go(transposed_kernel<P, 2, O>);
-            });
+            auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles, plan.dx_slices), dim3(kBlock), 0, st, a, to); };
+            auto tiles = [&](auto e) {
+                typedef decltype(e) E;
+                if (nu == 8) go(transposed_kernel<E, 1, 8, O>);
+                else if (nu == 4) go(transposed_kernel<E, 1, 4, O>);
+                else go(transposed_kernel<E, 1, 2, O>);
+            };
+            if (dy_dtype == SPMV_HIP_F32) go(transposed_kernel<__bf16, 3, 2, O>);
+            else if (dy_dtype == SPMV_HIP_F16) tiles(_Float16());
+            else tiles(__bf16());
         };
         with_elem(dx_dtype, [&](auto o) {
             typedef decltype(o) O;
@@ -1558,9 +1620,9 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
     }
     if (d_dvalues && m->nblocks > 0) {
         GradientArgs a{};
-        a.n = n; a.rows = rows; a.edge = m->rows; a.columns = m->columns;
+        a.n = n; a.rows = dv_rows; a.edge = m->rows; a.columns = m->columns;
         a.block_row = m->d_block_row; a.block_col = m->d_block_col;
-        a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.dy = dy; a.lddy = lddy; a.plane = plane; a.slice = plan.dv_slice;
+        a.x8 = d_x8; a.xscale = d_scale; a.ldx8 = ldx8; a.lds = lds; a.dy = (const __bf16 *)dv_dy; a.lddy = dv_ld; a.plane = plane; a.slice = plan.dv_slice;
         a.list = plan.pairs ? m->d_pair : m->d_order;
         auto into = [&](auto *to, int add) {
             typedef std::remove_pointer_t<decltype(to)> O;

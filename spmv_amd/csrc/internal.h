@@ -130,7 +130,7 @@ struct spmv_hip_matrix {
 
     // 8-bit blocks (BLOCK8): the blocks by block row (block_ptr, block_col) and by block column (bt_ptr over block
     // columns, bt_row = block row, bt_id = block)
-    int nblocks = 0, brows = 0, bcols = 0;
+    int nblocks = 0, brows = 0, bcols = 0, longest = 0;     // longest: blocks of the fullest block column
     int *d_block_ptr = nullptr, *d_block_col = nullptr, *d_block_row = nullptr;
     int *d_bt_ptr = nullptr, *d_bt_row = nullptr, *d_bt_id = nullptr;
     int *d_bt_at = nullptr, *d_bt_scale8 = nullptr; // a block's place in the lists by block column, the scale bytes in their order

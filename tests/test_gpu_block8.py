@@ -273,6 +273,24 @@ def test_product_t(rows, columns, keep, dy_dtype, dx_dtype):
         _close(c.A.product_t(dy, dx_dtype), _mat(d, c.dense), rows * (3 if dy_dtype == F32 else 2), _mat(np.abs(d), c.dense_abs))
 
 
+@pytest.mark.parametrize("dy_dtype", TYPES)
+@pytest.mark.parametrize("n", [3, 80])
+def test_product_t_small_entries_and_far_scales(dy_dtype, n):
+    """dy among its type's subnormals (fp16; 2^-100 for the others), blocks of one column 2^-60 to 2^60 apart"""
+    rows, columns = 520, 140
+    ptr, col = O.pattern(rows, columns, 1.0, 3)
+    values = torch.randn(len(col), 128, 128) * torch.exp2(torch.tensor([[-60.0, 60.0, -3.0, 0.0, 20.0][k % 5] for k in range(len(col))]))[:, None, None]
+    A = Block8(rows, columns, ptr, col)
+    A.set_values(values.to(DEV))
+    blocks, _ = O.quantized_blocks(_np(values), ptr, col, rows, columns)
+    a, mag = O.dense(blocks, ptr, col, rows, columns), O.dense(np.abs(blocks), ptr, col, rows, columns)
+    dy = (torch.randn(n, rows) * (2.0 ** -17 if dy_dtype == F16 else 2.0 ** -40)).to(dy_dtype)
+    dy[:, 1::7] = (torch.randn(n, len(range(1, rows, 7))) * (2.0 ** -23 if dy_dtype == F16 else 2.0 ** -60)).to(dy_dtype)
+    d = _np(dy)
+    assert dy_dtype != F16 or (np.abs(d[d != 0]) < 2.0 ** -14).mean() > 0.9
+    _close(A.product_t(dy.to(DEV), F32), _mat(d, a), rows * (3 if dy_dtype == F32 else 2), _mat(np.abs(d), mag))
+
+
 @pytest.mark.parametrize("rows,columns,keep", SHAPES)
 @pytest.mark.parametrize("dy_dtype,dv_dtype", [(F32, F32), (BF16, F32), (F16, F32), (BF16, BF16), (F16, F16)])
 def test_gradient(rows, columns, keep, dy_dtype, dv_dtype):
@@ -506,6 +524,28 @@ def test_infinities_in_dy_reach_what_they_multiply(dtype, n):
                           (_np(c.A.gradient(dy, quantize(x))), O.sampled(np.einsum("tr,tc->rc", d, xq), c.ptr, c.col))):
             assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
             assert np.array_equal(np.sign(got[np.isinf(got)]), np.sign(want[np.isinf(want)]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 90])
+def test_the_largest_numbers_in_dy(dtype, n):
+    """finite results of the largest finite dy: no part of it may overflow on the way"""
+    rows, columns = 260, 140
+    ptr, col = O.pattern(rows, columns, 1.0, 3)
+    values = torch.randn(len(col), 128, 128) * 2.0 ** -20
+    A = Block8(rows, columns, ptr, col)
+    A.set_values(values.to(DEV))
+    blocks, _ = O.quantized_blocks(_np(values), ptr, col, rows, columns)
+    a, mag = O.dense(blocks, ptr, col, rows, columns), O.dense(np.abs(blocks), ptr, col, rows, columns)
+    top = torch.finfo(dtype).max
+    dy = torch.randn(n, rows).to(dtype)
+    dy[0, 3], dy[1, 200], dy[n - 1, 259] = top, -top, top
+    x = _vectors(n, columns, dtype, 4) * 2.0 ** -20
+    q, d = quantize(x), _np(dy)
+    xq = O.quantized(_np(x))
+    _close(A.product_t(dy.to(DEV), F32), _mat(d, a), 3 * rows, _mat(np.abs(d), mag))
+    want, magnitude = O.sampled(_mat(d.T, xq), ptr, col), O.sampled(_mat(np.abs(d).T, np.abs(xq)), ptr, col)
+    _close(A.gradient(dy.to(DEV), q), want, 3 * n, magnitude)
 
 
 def test_general_entry_points_take_a_block8_handle():
