@@ -541,6 +541,32 @@ template <int R, typename F> __device__ __forceinline__ void ring(int first, int
     if constexpr (R > 3) if (k + 2 < last) step(ic<2>(), k + 2);
 }
 
+// G = 2 groups of four waves share a tile whose workgroup has a CU to itself, each with half of the sum and its own stages: one
+// group's loads and LDS reads run beside the other's matrix instructions.  Every barrier is the whole workgroup's, so
+// both pass as many; `rounds`, the steps of the first, is the larger number.
+template <int G> __device__ __forceinline__ int half_of(int group, int *first, int *last)
+{
+    if (G == 1) return *last - *first;
+    const int rounds = (*last - *first + 1) / 2;
+    if (group) *first += rounds;
+    else *last = *first + rounds;
+    return rounds;
+}
+// adds the second group's sums to the first's, through LDS that nothing else uses any more; true in the first
+template <int G, int NU> __device__ __forceinline__ bool joined(int group, int tid, f32x4 *lds, f32x4 (&acc)[NU][4])
+{
+    if constexpr (G > 1) {
+        if (group)
+#pragma unroll
+            for (int k = 0; k < 4 * NU; k++) lds[k * kBlock + tid] = acc[k >> 2][k & 3];
+        __syncthreads();
+        if (group) return false;
+#pragma unroll
+        for (int k = 0; k < 4 * NU; k++) acc[k >> 2][k & 3] += lds[k * kBlock + tid];
+    }
+    return true;
+}
+
 // logical tile of a workgroup: every XCD walks its own eighth of the tiles, in it 8 block rows (columns) side by side
 // and then the next vectors, so that the blocks and the vectors of the workgroups that run together stay in its L2
 __device__ __forceinline__ void tile_of_block(unsigned bid, int majors, int vtiles, int *major, int *vtile)
@@ -759,15 +785,18 @@ struct TransposedArgs {
 // with the strip, which puts the four on different banks.  The blocks of a last block row that is not whole come last in
 // every list: they are taken after the others, one by one, with the entries past the end masked (dy in parts is padded
 // and has no such rows).
-template <typename E, int PARTS, int NU, typename OT>
-__global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g, OT *__restrict__ dx)
+template <typename E, int PARTS, int NU, int G, typename OT>
+__global__ __launch_bounds__(G *kBlock, 2) void transposed_kernel(TransposedArgs g, OT *__restrict__ dx)
 {
     constexpr bool HALF = std::is_same<E, _Float16>::value;
     typedef x8<E> e8;
     constexpr int R = PARTS * NU >= 6 ? 2 : PARTS * NU == 4 ? 3 : 4, TOK = 32 * NU;
-    __shared__ uint8_t Y[R][PARTS][TOK * 128];
-    __shared__ uint8_t A[R][kBlockBytes / 2];
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), i = lane & 15, q = lane >> 4;
+    __shared__ uint8_t all_y[G][R][PARTS][TOK * 128];
+    __shared__ uint8_t all_a[G][R][kBlockBytes / 2];
+    const int group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kBlock), tid = G == 1 ? threadIdx.x : threadIdx.x % kBlock;
+    auto &Y = all_y[group];
+    auto &A = all_a[group];
+    const int lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
     const int wm = wave & 1, wn = wave >> 1;
     int major, vtile;
     tile_of_block(blockIdx.x, g.bcols, g.vtiles, &major, &vtile);
@@ -784,6 +813,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         if (blockIdx.y + 1 < gridDim.y) edge = 2 * end;
         dx += blockIdx.y * g.slice;
     }
+    const int rounds = half_of<G>(group, &first, &last);
     f32x4 acc[NU][4];
 #pragma unroll
     for (int u = 0; u < NU; u++)
@@ -918,6 +948,7 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
         if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
         ring<R>(first, last, step);
     }
+    for (int k = last - first; k < rounds; k++) stage_barrier<0>();      // as many as the other group
     stage_barrier<0>();                                      // no load to LDS outlives the workgroup, or meets the next
     for (int k = edge; k < 2 * end; k++) {
         look_up(k);
@@ -929,9 +960,10 @@ __global__ __launch_bounds__(kBlock, 2) void transposed_kernel(TransposedArgs g,
             __builtin_memcpy(&Y[0][0][(j * 32 + wave * 8) * 128 + lane * 16], one.v, 16);
         }
         stage_barrier<0>();
-        compute(ic<0>(), [] {});
+        if (group == 0) compute(ic<0>(), [] {});
         stage_barrier<0>();
     }
+    if (!joined<G, NU>(group, tid, (f32x4 *)&all_y[0][0][0][0], acc)) return;
 #pragma unroll
     for (int u = 0; u < NU; u++) {
         const int v = t0 + wn * 16 * NU + 16 * u + i;
@@ -960,12 +992,14 @@ struct GradientArgs {
 // lie on different banks.  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane:
 // widened there with the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane
 // i's columns are 4 i + s.
-template <int PARTS, int NB, typename OT>
-__global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT *__restrict__ dv)
+template <int PARTS, int NB, int G, typename OT>
+__global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, OT *__restrict__ dv)
 {
     constexpr int STEP = 32, NU = 4 * NB, R = NB == 2 ? (PARTS == 1 ? 3 : 2) : PARTS == 3 ? 3 : 4;
-    __shared__ uint8_t Y[R][PARTS][STEP * kB * 2];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
+    __shared__ uint8_t all_y[G][R][PARTS][STEP * kB * 2];
+    const int group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kBlock), tid = G == 1 ? threadIdx.x : threadIdx.x % kBlock;
+    auto &Y = all_y[group];
+    const int lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave), i = lane & 15, q = lane >> 4;
     const int wg = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
     const int which = NB == 2 ? wave >> 1 : 0;               // the wave's block, its columns and rows in it
     const int id0 = table(g.list, NB * wg), id = table(g.list, NB * wg + which);
@@ -1073,6 +1107,7 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
         if (blockIdx.y + 1 < gridDim.y) rest = g.n;
         dv += blockIdx.y * g.slice;
     }
+    const int rounds = half_of<G>(group, &first, &last);
     if (first < last) {
         issue(ic<0>(), first);
         if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
@@ -1083,12 +1118,15 @@ __global__ __launch_bounds__(kBlock, 2) void gradient_kernel(GradientArgs g, OT 
             compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
         });
     }
+    for (int k = last - first; k < rounds; k++) stage_barrier<0>();      // as many as the other group
     stage_barrier<0>();                                      // no load to LDS outlives the workgroup, or meets the next
     if (rest < g.n) {
         bring_rest(rest);
         stage_barrier<0>();
-        compute(ic<0>(), [] {});
+        if (group == 0) compute(ic<0>(), [] {});
+        if (G > 1) stage_barrier<0>();
     }
+    if (!joined<G, NU>(group, tid, (f32x4 *)&all_y[0][0][0][0], acc)) return;
     if (id < 0) return;
     // result r of tile (u, s) is row 16 u + 4 q + r, column 4 i + s: 16 lanes write 64 neighbours of a row.  (The other way
     // round a lane had 16 neighbours, and a store 64 pieces of 16 bytes: MEASURE.)
@@ -1248,20 +1286,20 @@ static int check_tiles(const char *what, int majors, int vtiles)
 struct BackwardPlan {
     int dx_parts, dv_parts;        // bf16 numbers an entry of dy is taken as
     bool pairs;                    // two blocks of a block row a workgroup
+    bool dx_halves, dv_halves;     // a workgroup is two groups of waves
     int tiles, dx_slices, dv_slices;
     int64_t dx_slice, dv_slice, parts_bytes, copy_bytes, work;
 };
 
 // Slices to cut sums of `steps` steps into, whose `tiles` workgroups leave CUs idle: as many as take the least time by
-// what was measured -- `step` us a step, 1.4 times that where two workgroups share a CU; the slices, `bytes` each, written and
-// read again at 4 TB/s, and 5 us for the launch that adds them.  (dx of 96 tiles x 80 steps of fp32: 106 us in one piece, 47
-// cut; of 132 tiles x 16 steps of fp16: 17 us in one, 22 in three.)
+// what was measured -- `step` us for two steps in a CU's two groups of waves; the slices, `bytes` each, written and
+// read again at 4 TB/s, and 5 us for the launch that adds them.
 static int slices(int64_t tiles, int64_t steps, int cus, float step, int64_t bytes)
 {
     int best = 1;
-    float least = steps * step;
-    for (int64_t k = 2; k * tiles <= 2 * cus && k <= steps; k += k / 2) {
-        const float us = (steps + k - 1) / k * step * (k * tiles > cus ? 1.4f : 1.0f) + 5.0f + k * bytes * 0.5e-6f;
+    float least = (steps + 1) / 2 * step;
+    for (int64_t k = 2; k * tiles <= cus && k <= steps; k += k / 2) {
+        const float us = (steps + 2 * k - 1) / (2 * k) * step + 5.0f + k * bytes * 0.5e-6f;
         if (us < least) { least = us; best = (int)k; }
     }
     return best;
@@ -1287,15 +1325,17 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
         // only with 1 1/2 workgroups a CU left (777 vectors: 30 us, 42 with 4; 3000: 66 us with 8, 77 with 2)
         p.tiles = p.dx_parts > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2);
         p.dx_slice = (int64_t)n * m->bcols * kB;
-        p.dx_slices = slices((int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), 2 * (int64_t)m->longest, m->cus,
-                             0.15f + 0.25f * p.dx_parts, p.dx_slice * 4);
+        const int64_t tiles = (int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), steps = 2 * (int64_t)m->longest;
+        p.dx_slices = slices(tiles, steps, m->cus, 0.2f + 0.3f * p.dx_parts, p.dx_slice * 4);
+        p.dx_halves = p.tiles == 2 && tiles * p.dx_slices <= m->cus && steps >= 4 * p.dx_slices;
     }
     if (with_dv && m->nblocks) {
         // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
         // registers; and not where many pairs lack their second block
         p.pairs = m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
         p.dv_slice = (int64_t)m->nblocks * kBlockBytes;
-        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, n / 32, m->cus, 0.1f + 0.2f * p.dv_parts, p.dv_slice * 4);
+        p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, n / 32, m->cus, 0.2f + 0.25f * p.dv_parts, p.dv_slice * 4);
+        p.dv_halves = !p.pairs && (int64_t)m->nblocks * p.dv_slices <= m->cus && n / 32 >= 4 * p.dv_slices;
     }
     p.work = p.parts_bytes + p.copy_bytes + 4 * std::max(p.dx_slices > 1 ? p.dx_slices * p.dx_slice : 0, p.dv_slices > 1 ? p.dv_slices * p.dv_slice : 0);
     return p;
@@ -1600,16 +1640,20 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
         auto into = [&](auto *to, int64_t ld) {
             typedef std::remove_pointer_t<decltype(to)> O;
             a.lddx = ld;
-            auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles, plan.dx_slices), dim3(kBlock), 0, st, a, to); };
+            auto go = [&](auto kernel, int groups) {
+                hipLaunchKernelGGL(kernel, dim3(m->bcols * a.vtiles, plan.dx_slices), dim3(groups * kBlock), 0, st, a, to);
+            };
             auto tiles = [&](auto e) {
                 typedef decltype(e) E;
-                if (nu == 8) go(transposed_kernel<E, 1, 8, O>);
-                else if (nu == 4) go(transposed_kernel<E, 1, 4, O>);
-                else go(transposed_kernel<E, 1, 2, O>);
+                if (nu == 8) go(transposed_kernel<E, 1, 8, 1, O>, 1);
+                else if (nu == 4) go(transposed_kernel<E, 1, 4, 1, O>, 1);
+                else if (plan.dx_halves) go(transposed_kernel<E, 1, 2, 2, O>, 2);
+                else go(transposed_kernel<E, 1, 2, 1, O>, 1);
             };
-            if (dy_dtype == SPMV_HIP_F32) go(transposed_kernel<__bf16, 3, 2, O>);
-            else if (dy_dtype == SPMV_HIP_F16) tiles(_Float16());
-            else tiles(__bf16());
+            if (dy_dtype == SPMV_HIP_F16) tiles(_Float16());
+            else if (dy_dtype == SPMV_HIP_BF16) tiles(__bf16());
+            else if (plan.dx_halves) go(transposed_kernel<__bf16, 3, 2, 2, O>, 2);
+            else go(transposed_kernel<__bf16, 3, 2, 1, O>, 1);
         };
         with_elem(dx_dtype, [&](auto o) {
             typedef decltype(o) O;
@@ -1629,9 +1673,12 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
             a.accumulate = add;
             with_parts([&](auto p) {
                 constexpr int P = decltype(p)::value;
-                auto go = [&](auto kernel, int wgs) { hipLaunchKernelGGL(kernel, dim3(wgs, plan.dv_slices), dim3(kBlock), 0, st, a, to); };
-                if (plan.pairs) { go(gradient_kernel<P, 2, O>, m->npairs); return; }
-                go(gradient_kernel<P, 1, O>, m->nblocks);
+                auto go = [&](auto kernel, int wgs, int groups) {
+                    hipLaunchKernelGGL(kernel, dim3(wgs, plan.dv_slices), dim3(groups * kBlock), 0, st, a, to);
+                };
+                if (plan.pairs) go(gradient_kernel<P, 2, 1, O>, m->npairs, 1);
+                else if (plan.dv_halves) go(gradient_kernel<P, 1, 2, O>, m->nblocks, 2);
+                else go(gradient_kernel<P, 1, 1, O>, m->nblocks, 1);
             });
         };
         with_elem(dv_dtype, [&](auto o) {
