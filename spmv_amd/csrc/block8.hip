@@ -347,12 +347,12 @@ __device__ __forceinline__ int table(const int *p, int k)
 
 // ---- few vectors ----------------------------------------------------------------------------------------------
 
-// One workgroup per S strips of 16 rows; its W waves take the strips' blocks in turn and add their results in LDS.
-// Bound by reading the matrix once (8192 x 8192, up to 16 vectors in 8 bits: 12.5 us, 5.4 TB/s), for small matrices by
-// latency -- a wave's next block is on its way while it works on one -- and with more vectors by widening x, which every
-// strip's workgroup does again: two strips share it.  NT tiles of 16 vectors.  XT: uint8_t (x in 8 bits) or a wide type, rounded to 8 bits
-// here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.  Operands are widened
-// to bf16 (exact), sums are 32 bits.
+// One workgroup per S strips of 16 rows and NT tiles of 16 vectors; its W waves take the strips' blocks in turn and add
+// their results in LDS.  Bound by reading the matrix once (8192 x 8192, up to 16 vectors in 8 bits: 12.5 us, 5.4 TB/s),
+// for small matrices by latency -- a wave's next block is on its way while it works on one -- and with more vectors by
+// widening x, which every strip's workgroup does again: two strips share it.  XT: uint8_t (x in 8 bits) or a wide type,
+// rounded to 8 bits here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.
+// Operands are widened to bf16 (exact), sums are 32 bits.
 template <typename XT, int NT, int W, int S>
 __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, int columns, const int *__restrict__ block_ptr,
                                                                const int *__restrict__ block_col, const uint8_t *__restrict__ val8,
@@ -369,10 +369,11 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
     for (int k = 0; k < S; k++)
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[k][t] = f32x4{0, 0, 0, 0};
+    const int v0 = blockIdx.y * 16 * NT;
     // vectors past the last read the last: a column of the result that is not stored
     int64_t vec[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) vec[t] = min(t * 16 + i, n - 1);
+    for (int t = 0; t < NT; t++) vec[t] = min(v0 + t * 16 + i, n - 1);
 
     constexpr bool AHEAD = NT * sizeof(XT) <= 4;             // x ahead too, in up to 32 registers
     struct Vector {
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         for (int t = 0; t < NT; t++) part[wave][t][lane] = acc[k][t];
         __syncthreads();
         for (int id = threadIdx.x; id < NT * kWave; id += W * kWave) {
-            const int t = id / kWave, l = id & (kWave - 1), v = t * 16 + (l & 15);
+            const int t = id / kWave, l = id & (kWave - 1), v = v0 + t * 16 + (l & 15);
             f32x4 s = part[0][t][l];
 #pragma unroll
             for (int w = 1; w < W; w++) s += part[w][t][l];
@@ -1200,7 +1201,7 @@ static int launch_few(const spmv_hip_matrix *m, int n, const void *x, int x_dtyp
     auto go = [&](auto t) {
         typedef decltype(t) XT;
         auto launch = [&](auto kernel, int waves, int strips) {
-            hipLaunchKernelGGL(kernel, dim3(m->brows * (8 / strips)), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
+            hipLaunchKernelGGL(kernel, dim3(m->brows * (8 / strips), (n + 63) / 64), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
                                m->d_block_col, m->d_val8, m->d_scale8, (const XT *)x, ldx, xscale, lds, y, y_dtype, ldy);
         };
         auto tiles = [&](auto w, auto two) {
@@ -1543,7 +1544,9 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     if (n == 0 || m->rows == 0) return 0;
     DeviceGuard on(m->device);
     if (!on.ok) return 1;
-    if (n <= SPMV_HIP_BLOCK8_MAX_WIDE)
+    // few vectors, or few tiles of many: there the strips, eight times as many, give the GPU more to do (fp32, 8192 x 1024, 128
+    // vectors: 11 us, 21 in tiles; 32 tiles of 64 vectors 12 and 21 us, 64 tiles 22 and 22)
+    if (n <= SPMV_HIP_BLOCK8_MAX_WIDE || (int64_t)m->brows * ((n + 63) / 64) * 8 <= m->cus)
         return launch_few(m, n, d_x, x_dtype, ldx, d_scale, lds, d_y, y_dtype, ldy, (hipStream_t)stream);
     ProductArgs a{};
     a.n = n; a.rows = m->rows; a.brows = m->brows;
