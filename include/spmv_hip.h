@@ -381,10 +381,13 @@ int spmv_hip_dist_free(spmv_hip_dist *d);
  * element's own; 16-byte aligned bases and strides are faster.
  *
  * All calls are asynchronous on `stream`, allocate nothing and may be captured
- * into a graph; they keep nothing in the handle, so that products on one handle
- * may overlap.  Vectors of dy are less than 2^23 entries apart.  n = 0 is allowed.  spmv_hip_mult, _mult_dev, _mult_mv, _mult_mv_dev
- * and _bench take such a handle too (dtype F32): x is rounded to 8 bits on its way
- * in.  "variant", "block_map" and "hot_columns" do not apply. */
+ * into a graph.  set_values and load write the handle's values on their stream:
+ * products on other streams have to be ordered behind them.  Products keep nothing
+ * in the handle and may overlap.  Vectors of dy are less than 2^23 entries apart.
+ * n = 0 is allowed.  Results have the same bits on every call.
+ * spmv_hip_mult, _mult_dev, _mult_mv, _mult_mv_dev and _bench take such a handle too
+ * (dtype F32): x is rounded to 8 bits on its way in.  "variant", "block_map" and
+ * "hot_columns" do not apply. */
 
 /* block_ptr[0 .. ceil(rows/128)], block_col[0 .. nblocks): host arrays, like row_ptr
  * and col of a CSR matrix.  All values are zero until one of the next two calls. */
@@ -409,7 +412,9 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
 /* y_v = A x_v (mult_mv_csr, spmv.h:54, for this format).  x_dtype E4M3: x in 8 bits
  * with its scales; otherwise x is F32, BF16 or F16, d_scale is NULL, x is rounded to
  * 8 bits inside the product, and n is at most SPMV_HIP_BLOCK8_MAX_WIDE (quantize
- * larger blocks of vectors first).  y in F32, BF16 or F16. */
+ * larger blocks of vectors first).  y in F32, BF16 or F16.  Products are exact and
+ * sums 32 bits wide, but for BF16 results of more than 64 vectors: those may be off
+ * by 7 * 2^-13 of the sum of the terms' magnitudes (the 8-bit matrix instruction). */
 enum { SPMV_HIP_BLOCK8_MAX_WIDE = 64 };
 int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, int x_dtype, int64_t ldx,
                              const uint8_t *d_scale, int64_t lds, void *d_y, int y_dtype, int64_t ldy, void *stream);
@@ -421,10 +426,10 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
  *     8-bit checkpoint (needed for this one only); zero beyond the matrix's edge.
  *     accumulate != 0 adds to what d_dvalues holds.
  * d_work: spmv_hip_block8_backward_work() bytes of device memory, 16-byte aligned,
- * scratch for this call, NULL if that is 0.  It holds dy in bf16 parts, where dy is
- * not bf16 or, for dx, its vectors are not 16-byte aligned, and the slices of sums
- * that are cut because there are too few of them to fill the device.  with_dx,
- * with_dvalues: which of the two the call will ask for. */
+ * scratch for this call, NULL if that is 0.  It holds dy in bf16 parts (F32; F16 for
+ * d_dvalues), a copy of 16-bit vectors that are not 16-byte aligned, and the slices
+ * of sums that are cut because there are too few of them to fill the device.
+ * with_dx, with_dvalues: which of the two the call will ask for. */
 int64_t spmv_hip_block8_backward_work(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy, int with_dx,
                                       int with_dvalues);
 int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_dy, int dy_dtype, int64_t lddy,

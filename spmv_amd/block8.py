@@ -174,7 +174,8 @@ class Block8(Matrix):
         return out
 
     def set_values(self, values: torch.Tensor) -> None:
-        """Rounds values [blocks, 128, 128] into the matrix.  linear() returns the gradient of this tensor."""
+        """Rounds values [blocks, 128, 128] into the matrix, on the current stream (products on others have to wait for
+        it).  linear() returns the gradient of this tensor."""
         self._blocks("values", values, _DTYPE)
         L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _raw_stream(self._index)))
         self.values = values

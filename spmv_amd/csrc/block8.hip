@@ -608,6 +608,10 @@ struct ProductArgs {
 // EXACT: operands widened to bf16 in registers (exact), 32-bit sums.  Otherwise the 8-bit matrix instruction, which applies
 // both scales and runs at twice the rate, but aligns 8 products at a time and drops what lies 13 bits below the largest:
 // good to about 16 bits, for bf16 results only.
+// 8192 vectors, full 8192 x 8192, bf16: 435 us, 2.5 PFLOP/s (a library product of plain 8-bit matrices of that size reaches
+// 3.2); the matrix pipes are busy 64 % of the cycles at the 1.9 GHz that the power allows.  Widened: 860 us.  LDS reads that
+// meet twice as many banks (vectors exchanged in pairs too) changed nothing.  Few workgroups are bound by the chain of a
+// step -- LDS, widening, products -- which two groups of waves overlap.
 template <bool EXACT, int NU, int G, typename OT>
 __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT *__restrict__ y)
 {
@@ -719,8 +723,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
     for (int k = last - first; k < rounds; k++) stage_barrier<0>();      // as many as the other group
     stage_barrier<0>();                                      // no load to LDS outlives the workgroup
     if (!joined<G, NU>(group, tid, (f32x4 *)&all_x[0][0][0], acc)) return;
-    // result k of tile (u, s) is vector NU (4 q + k) + u, row 4 i + s of the wave's 64: 16 lanes write 64 neighbours.  (The
-    // other way round a lane had 16 neighbours, and a store 64 pieces of 16 bytes: MEASURE.)
+    // result k of tile (u, s) is vector NU (4 q + k) + u, row 4 i + s of the wave's 64: 16 lanes write 64 neighbours.
     const int r = major * kB + wm * 64 + 4 * i, v1 = t0 + wn * 16 * NU + NU * 4 * q;
 #pragma unroll
     for (int k = 0; k < 4; k++)
@@ -742,7 +745,7 @@ static int parts(int dtype) { return dtype == SPMV_HIP_BF16 ? 1 : dtype == SPMV_
 
 // dy into its parts, `plane` entries apart, vectors `ld` apart (a multiple of 128), zero past `length`; 8 entries a
 // thread.  Before the products rather than in them: there the splitting stood between loads and matrix instructions of
-// every step (fp32, 333 vectors, 264 blocks: 41 us, now 6 + 26).
+// every step (fp32, 333 vectors, 264 blocks: 41 us, now 5 + 20).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void split_kernel(int n, int length, int ld, const T *__restrict__ dy, int64_t lddy,
                                                        __bf16 *__restrict__ out, int64_t plane)
@@ -790,7 +793,9 @@ struct TransposedArgs {
 // each of four strips of the block (block8_offset); in LDS the 4-row pieces of a 16 x 16 subtile are exchanged by XOR
 // with the strip, which puts the four on different banks.  The blocks of a last block row that is not whole come last in
 // every list: they are taken after the others, one by one, with the entries past the end masked (dy in parts is padded
-// and has no such rows).
+// and has no such rows).  fp16 dy multiplies blocks widened without their scale, which is put on the sums of half a block.
+// 8192 vectors, full 8192 x 8192, bf16: 825 us, 1.33 PFLOP/s (a library product of plain bf16 matrices 1.45); the matrix
+// pipes are busy 64 % of the cycles at 2 GHz.
 template <typename E, int PARTS, int NU, int G, typename OT>
 __global__ __launch_bounds__(G *kBlock, 2) void transposed_kernel(TransposedArgs g, OT *__restrict__ dx)
 {
@@ -998,6 +1003,8 @@ struct GradientArgs {
 // lie on different banks.  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane:
 // widened there with the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane
 // i's columns are 4 i + s.
+// 8192 vectors, full 8192 x 8192, bf16: 875-910 us, 1.2 PFLOP/s; the matrix pipes are busy 59 % of the cycles at 2 GHz.  x
+// through LDS as well, a third of the loads, left that as it is and made fp32's slower (fewer stages fit).
 template <int PARTS, int NB, int G, typename OT>
 __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, OT *__restrict__ dv)
 {
@@ -1134,8 +1141,8 @@ __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, 
     }
     if (!joined<G, NU>(group, tid, (f32x4 *)&all_y[0][0][0][0], acc)) return;
     if (id < 0) return;
-    // result r of tile (u, s) is row 16 u + 4 q + r, column 4 i + s: 16 lanes write 64 neighbours of a row.  (The other way
-    // round a lane had 16 neighbours, and a store 64 pieces of 16 bytes: MEASURE.)
+    // result r of tile (u, s) is row 16 u + 4 q + r, column 4 i + s: 16 lanes write 64 neighbours of a row.  (With the
+    // operands the other way round a lane had 16 neighbours, and a store 64 pieces of 16 bytes: 920 us for 8192 vectors, now 870.)
     const int c = c0 + 4 * i, left = g.columns - (col * kB + c);
     OT *o = dv + (int64_t)id * kBlockBytes + (n0 + 4 * q) * kB + c;
 #pragma unroll
@@ -1337,8 +1344,8 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
         p.dx_halves = p.tiles == 2 && tiles * p.dx_slices <= m->cus && steps >= 4 * p.dx_slices;
     }
     if (with_dv && m->nblocks) {
-        // two blocks a workgroup once they fill the GPU; not where dy is split: its parts and two blocks' sums do not fit the
-        // registers; and not where many pairs lack their second block
+        // two blocks a workgroup once they fill the GPU (512 blocks, 2000 vectors of bf16: 44 us, 56 with one), and not where
+        // many pairs lack their second block
         p.pairs = m->npairs >= m->cus && m->nblocks * (int64_t)4 >= m->npairs * (int64_t)7;
         p.dv_slice = (int64_t)m->nblocks * kBlockBytes;
         p.dv_slices = slices(p.pairs ? m->npairs : m->nblocks, n / 32, m->cus, 0.2f + 0.25f * p.dv_parts, p.dv_slice * 4);
