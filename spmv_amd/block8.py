@@ -26,6 +26,7 @@ from .matrix import Matrix
 
 BLOCK = 128
 MAX_WIDE = 64                         # vectors a product rounds to 8 bits by itself (SPMV_HIP_BLOCK8_MAX_WIDE)
+MAX_APART = 1 << 23                   # entries between vectors of dy, less than
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
 
@@ -249,6 +250,8 @@ class Block8(Matrix):
 
     def _dy(self, dy) -> torch.Tensor:
         d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
+        if _ld(d) >= MAX_APART:
+            d = d.contiguous()
         self._here("dy", d)
         return d
 

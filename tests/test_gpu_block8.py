@@ -405,6 +405,69 @@ def test_a_cut_gradient_replays_and_does_not_share_its_workspace():
             assert all(torch.equal(a, b) for a, b in zip(out, f())), k
 
 
+def test_dy_vectors_far_apart():
+    c = Case(200, 300, 1.0, 23)
+    wide = torch.zeros(3, (1 << 23) + 8, dtype=F16, device=DEV)
+    dy = wide[:, :200]
+    dy.copy_(_vectors(3, 200, F16, 1))
+    q = quantize(_vectors(3, 300, F16, 2))
+    assert torch.equal(c.A.product_t(dy), c.A.product_t(dy.contiguous()))
+    assert torch.equal(c.A.gradient(dy, q), c.A.gradient(dy.contiguous(), q))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_together_from_vectors_at_odd_addresses(dtype):
+    """dx and the blocks' gradient of one backward pass against the two by themselves, dy not 16-byte aligned"""
+    c = Case(389, 517, 0.8, 24)
+    w = c.values.to(DEV).requires_grad_()
+    c.A.set_values(w)
+    for n in (1, 70):
+        x = _vectors(n, 517, dtype, 1).requires_grad_()
+        dy = _vectors(n + 1, 389, dtype, 2).flatten()[1:1 + n * 389].view(n, 389)
+        dx, dw = torch.autograd.grad(c.A.linear(x), (x, w), dy)
+        assert torch.equal(dx, c.A.product_t(dy)) and torch.equal(dw, c.A.gradient(dy, quantize(x)))
+
+
+def test_offsets_past_32_bits():
+    """a matrix of 2.2 GB and blocks of vectors past 2 GB: the last block row, block column, block and vectors"""
+    k = 370
+    A = Block8.full(128 * k, 128 * k)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    v8 = torch.randint(0, 256, (A.nblocks, 128, 128), generator=g, device=DEV, dtype=torch.uint8)
+    v8[(v8 & 127) == 127] = 5                                # no NaN
+    scale = torch.randint(118, 124, (A.nblocks,), generator=g, device=DEV, dtype=torch.uint8)
+    A.load(v8, scale)
+    code = torch.from_numpy(O.decode(np.arange(256, dtype=np.uint8))).to(DEV)
+
+    def blocks(ids):                                         # in 64 bits
+        return code[v8[ids].long()] * torch.exp2(scale[ids].double() - 127)[:, None, None]
+
+    last_row = blocks(torch.arange(A.nblocks - k, A.nblocks, device=DEV)).permute(1, 0, 2).reshape(128, -1)
+    last_col = blocks(torch.arange(k - 1, A.nblocks, k, device=DEV)).reshape(-1, 128)
+    n = 46000
+    x = torch.randn(n, 128 * k, generator=g, device=DEV, dtype=BF16)
+    q = quantize(x)
+    tail = quantize(x[-200:])
+    assert torch.equal(tail.values, q.values[-200:]) and torch.equal(tail.scale, q.scale[:, -200:])
+    back = q.restore(F32)
+    assert torch.equal(back[-200:], tail.restore(F32))
+    xq = back[-200:].double()
+    del back
+    for m, p, dtype, extra in ((3, quantize(x[-3:]), F32, 0.0), (200, tail, F32, 0.0), (200, q, BF16, EIGHT)):
+        y = A.product(p, dtype)
+        a = xq[-m:]
+        _close_64(y[-m:, -128:], torch.mm(a, last_row.t().contiguous()), 128 * k, torch.mm(a.abs(), last_row.abs().t().contiguous()), extra)
+    dy = y                                                   # [46000, 47360] of bf16
+    d = dy[-200:].double()
+    for p, m in ((dy, 200), (dy[-3:], 3)):
+        dx = A.product_t(p, BF16)
+        _close_64(dx[-m:, -128:], torch.mm(d[-m:], last_col), 2 * 128 * k, torch.mm(d[-m:].abs(), last_col.abs()))
+    del dx
+    dv = A.gradient(dy[-200:], tail, BF16)
+    t = d[:, -128:].t().contiguous()
+    _close_64(dv[-1], torch.mm(t, xq[:, -128:].contiguous()), 200, torch.mm(t.abs(), xq[:, -128:].abs().contiguous()))
+
+
 @pytest.mark.parametrize("dtype,n", [(F32, 5500), (BF16, 9000)])
 def test_results_larger_than_the_last_cache(dtype, n):
     """restore past the caches against restore through them, of the same vectors in two halves"""
