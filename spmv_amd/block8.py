@@ -35,21 +35,13 @@ _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class _On:
-    """Makes `device` current for calls without a handle, which know no device of their own; free where it is already."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(device: torch.device, f, *args) -> None:
+    """A library call without a handle, which knows no device of its own, on `device`."""
+    if torch.cuda.current_device() == device.index:
+        L.check(f(*args))
+    else:
+        with torch.cuda.device(device):
+            L.check(f(*args))
 
 
 def _wide(name: str, x: torch.Tensor, length: int | None = None) -> torch.Tensor:
@@ -107,10 +99,9 @@ class Packed8:
         if dtype not in _DTYPE:
             raise TypeError("dtype must be float32, bfloat16 or float16")
         device, (n, ld8) = self.values.device, self.values.shape
-        x = torch.empty(self.shape, dtype=dtype, device=device)
-        with _On(device):
-            L.check(L.lib().spmv_hip_restore8_dev(n, self.columns, self.values.data_ptr(), ld8, self.scale.data_ptr(), n,
-                                                  x.data_ptr(), _DTYPE[dtype], self.columns, _raw_stream(device.index)))
+        x = self.values.new_empty(self.shape, dtype=dtype)
+        _call(device, L.lib().spmv_hip_restore8_dev, n, self.columns, self.values.data_ptr(), ld8, self.scale.data_ptr(), n,
+              x.data_ptr(), _DTYPE[dtype], self.columns, _raw_stream(device.index))
         return x
 
 
@@ -118,11 +109,10 @@ def _rounded(rows: torch.Tensor, shape) -> Packed8:
     n, columns = rows.shape
     groups = -(-columns // BLOCK)
     device = rows.device
-    values = torch.empty((n, groups * BLOCK), dtype=torch.uint8, device=device)
-    scale = torch.empty((groups, n), dtype=torch.uint8, device=device)
-    with _On(device):
-        L.check(L.lib().spmv_hip_quantize8_dev(n, columns, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows), values.data_ptr(),
-                                               groups * BLOCK, scale.data_ptr(), n, _raw_stream(device.index)))
+    values = rows.new_empty((n, groups * BLOCK), dtype=torch.uint8)
+    scale = rows.new_empty((groups, n), dtype=torch.uint8)
+    _call(device, L.lib().spmv_hip_quantize8_dev, n, columns, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows), values.data_ptr(),
+          groups * BLOCK, scale.data_ptr(), n, _raw_stream(device.index))
     return Packed8._made(values, scale, columns, rows.dtype, shape)
 
 
@@ -168,7 +158,7 @@ class Block8(Matrix):
         if dtype not in _DTYPE:
             raise TypeError("the result's type must be float32, bfloat16 or float16")
         if out is None:
-            return torch.empty(shape, dtype=dtype, device=like.device)
+            return like.new_empty(shape, dtype=dtype)
         if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {tuple(shape)} of {dtype}")
         self._here("out", out)
@@ -261,7 +251,7 @@ class Block8(Matrix):
         p, t, work = d.data_ptr(), _DTYPE[d.dtype], None
         size = lib.spmv_hip_block8_backward_work(self._h, n, p, t, ld, dx is not None, dv is not None)
         if size:
-            work = torch.empty(size, dtype=torch.uint8, device=self.device)
+            work = d.new_empty(size, dtype=torch.uint8)
         L.check(lib.spmv_hip_block8_backward_dev(
             self._h, n, p, t, ld,
             *((x.values.data_ptr(), x.values.shape[1], x.scale.data_ptr(), x.n) if dv is not None else (None, 0, None, 0)),
@@ -298,9 +288,9 @@ class _Linear(torch.autograd.Function):
         if matrix._version != ctx.version:
             raise RuntimeError("the values of the 8-bit matrix were set again between forward and backward")
         d = matrix._dy(dy)
-        dx = torch.empty(ctx.x_shape, dtype=ctx.x_dtype, device=d.device) if ctx.needs_input_grad[0] else None
+        dx = d.new_empty(ctx.x_shape, dtype=ctx.x_dtype) if ctx.needs_input_grad[0] else None
         dv = None
         if ctx.needs_input_grad[1]:
-            dv = torch.empty((matrix.nblocks, BLOCK, BLOCK), dtype=ctx.values_dtype, device=d.device)
+            dv = d.new_empty((matrix.nblocks, BLOCK, BLOCK), dtype=ctx.values_dtype)
         matrix._backward(d, Packed8._made(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), dx, dv, False)
         return dx, dv, None
