@@ -413,9 +413,9 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
  * with its scales; otherwise x is F32, BF16 or F16, d_scale is NULL, x is rounded to
  * 8 bits inside the product, and n is at most SPMV_HIP_BLOCK8_MAX_WIDE (quantize
  * larger blocks of vectors first).  y in F32, BF16 or F16.  Products are exact and
- * sums 32 bits wide, but for BF16 results of more than 64 vectors: those may be off
- * by 7 * 2^-13 of the sum of the terms' magnitudes (the 8-bit matrix instruction). */
-enum { SPMV_HIP_BLOCK8_MAX_WIDE = 64 };
+ * sums 32 bits wide, but for BF16 results of more than 64 vectors in 8 bits: those may
+ * be off by 7 * 2^-13 of the sum of the terms' magnitudes (the 8-bit matrix instruction). */
+enum { SPMV_HIP_BLOCK8_MAX_WIDE = 1024 };
 int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, int x_dtype, int64_t ldx,
                              const uint8_t *d_scale, int64_t lds, void *d_y, int y_dtype, int64_t ldy, void *stream);
 /* The two gradients of the product, from dy (F32, BF16 or F16, used as it is, not

@@ -25,7 +25,7 @@ from . import _lib as L
 from .matrix import Matrix
 
 BLOCK = 128
-MAX_WIDE = 64                         # vectors a product rounds to 8 bits by itself (SPMV_HIP_BLOCK8_MAX_WIDE)
+MAX_WIDE = 1024                       # vectors a product rounds to 8 bits by itself (SPMV_HIP_BLOCK8_MAX_WIDE)
 MAX_APART = 1 << 23                   # entries between vectors of dy, less than
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
@@ -198,8 +198,10 @@ class Block8(Matrix):
             shape = (*x.shape[:-1], self.rows)
             # Rounded inside the product, by every workgroup again, where that costs less than a call to quantize (bf16,
             # 1920 blocks: 16 vectors 11 us inside, 17 before; 32 vectors 26 and 17 us; 4096 blocks, 16 vectors 17 and 17 us)
+            # More than 64 vectors only where those in 8 bits go by the same kernel (32 tiles of 64): the same bits either way.
             n = rows.shape[0]
-            if n <= MAX_WIDE and self.nblocks * (-(-n // 16) * rows.element_size()) < (8500 if n <= 16 else 7500):
+            if (n <= 64 or n <= MAX_WIDE and -(-self.rows // BLOCK) * -(-n // 64) <= 32) and \
+                    self.nblocks * (-(-n // 16) * rows.element_size()) < (8500 if n <= 16 else 7500):
                 y = self._out(out, shape, dtype or rows.dtype, rows)
                 L.check(L.lib().spmv_hip_block8_mult_dev(self._h, n, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
                                                          None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _raw_stream(self._index)))

@@ -1554,7 +1554,7 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     if (!on.ok) return 1;
     // few vectors, or few tiles of many: there the strips, eight times as many, give the GPU more to do (fp32, 8192 x 1024, 128
     // vectors: 11 us, 21 in tiles; 32 tiles of 64 vectors 12 and 21 us, 64 tiles 22 and 22)
-    if (n <= SPMV_HIP_BLOCK8_MAX_WIDE || (int64_t)m->brows * ((n + 63) / 64) * 8 <= m->cus)
+    if (x_dtype != SPMV_HIP_E4M3 || n <= 64 || (int64_t)m->brows * ((n + 63) / 64) * 8 <= m->cus)
         return launch_few(m, n, d_x, x_dtype, ldx, d_scale, lds, d_y, y_dtype, ldy, (hipStream_t)stream);
     ProductArgs a{};
     a.n = n; a.rows = m->rows; a.brows = m->brows;

@@ -497,6 +497,18 @@ def test_few_vectors_and_many_blocks(dtype):
         _close_64(y, torch.mm(xq, a), 3900, torch.mm(xq.abs(), mag))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,columns,n", [(300, 700, 65), (300, 700, 515), (130, 200, 1024), (250, 130, 1025), (128, 1000, 777)])
+def test_many_wide_vectors_and_few_rows(rows, columns, n, dtype):
+    """rounded inside the product or before it: the same bits"""
+    c = Case(rows, columns, 0.9, rows + n)
+    x = _vectors(n, columns, dtype, n)
+    xq = _on_gpu(O.quantized(_np(x)))
+    y = c.A.product(x)
+    _close_64(y, torch.mm(xq, _on_gpu(c.dense.T)), columns, torch.mm(xq.abs(), _on_gpu(c.dense_abs.T)), EIGHT if dtype == BF16 else 0.0)
+    assert torch.equal(y, c.A.product(quantize(x)))
+
+
 def test_two_blocks_at_one_place_add_up_and_get_a_gradient_each():
     ptr, col = np.array([0, 3], np.int32), np.array([1, 0, 1], np.int32)
     A = Block8(100, 200, ptr, col)
@@ -860,7 +872,7 @@ def test_refusals():
         assert rc != 0 and text in L.spmv_hip_last_error().decode()
 
     p, h = x.data_ptr(), A._h
-    fails(L.spmv_hip_block8_mult_dev(h, 65, p, S.F32, 300, None, 0, p, S.F32, 200, None), "at most 64")
+    fails(L.spmv_hip_block8_mult_dev(h, 1025, p, S.F32, 300, None, 0, p, S.F32, 200, None), "at most 1024")
     fails(L.spmv_hip_block8_mult_dev(h, 1, p, S.F32, 300, p, 0, p, S.F32, 200, None), "scales belong")
     fails(L.spmv_hip_block8_mult_dev(h, 1, p, S.F64, 300, None, 0, p, S.F32, 200, None), "F32, BF16, F16 or E4M3")
     fails(L.spmv_hip_block8_mult_dev(h, 1, p, S.F32, 300, None, 0, p, S.E4M3, 200, None), "must be F32, BF16 or F16")
