@@ -45,17 +45,22 @@ def _call(device: torch.device, f, *args) -> None:
 
 
 def _wide(name: str, x: torch.Tensor, length: int | None = None) -> torch.Tensor:
-    """x as [n, length] rows that are contiguous inside (any distance apart); copies only what has no such view."""
+    """x, without its history, as [n, length] rows that are contiguous inside (any distance apart); copies only what has no
+    such view."""
     if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPE:
         raise TypeError(f"{name} must be a float32, bfloat16 or float16 tensor")
     if not x.is_cuda:
         raise ValueError(f"{name} must be on a GPU; there is no CPU path")
     if x.dim() < 1 or (length is not None and x.shape[-1] != length):
         raise ValueError(f"{name} has shape {tuple(x.shape)}, expected (..., {length})")
+    if x.requires_grad:
+        x = x.detach()
     if x.dim() != 2:
         x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()                       # transposed or broadcast rows
+    if not x.is_contiguous():
+        n, columns = x.shape
+        if columns > 1 and x.stride(1) != 1 or n > 1 and x.stride(0) < columns:
+            x = x.contiguous()                   # transposed or broadcast rows
     return x
 
 
@@ -118,7 +123,7 @@ def _rounded(rows: torch.Tensor, shape) -> Packed8:
 
 def quantize(x: torch.Tensor) -> Packed8:
     """x [..., columns] to 8 bits."""
-    return _rounded(_wide("x", x.detach() if isinstance(x, torch.Tensor) else x), x.shape)
+    return _rounded(_wide("x", x), x.shape)
 
 
 class Block8(Matrix):
@@ -193,7 +198,7 @@ class Block8(Matrix):
         """y[..., rows] = A x for the vectors of x: a tensor [..., columns] (rounded to 8 bits on the way in) or a
         Packed8.  `dtype` of y: that of x unless given."""
         if not isinstance(x, Packed8):
-            rows = _wide("x", x.detach() if isinstance(x, torch.Tensor) else x, self.columns)
+            rows = _wide("x", x, self.columns)
             self._here("x", rows)
             shape = (*x.shape[:-1], self.rows)
             # Rounded inside the product, by every workgroup again, where that costs less than a call to quantize (bf16,
@@ -241,7 +246,7 @@ class Block8(Matrix):
         return dv
 
     def _dy(self, dy) -> torch.Tensor:
-        d = _wide("dy", dy.detach() if isinstance(dy, torch.Tensor) else dy, self.rows)
+        d = _wide("dy", dy, self.rows)
         if _ld(d) >= MAX_APART:
             d = d.contiguous()
         self._here("dy", d)
