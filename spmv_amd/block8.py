@@ -70,11 +70,14 @@ def _ld(x: torch.Tensor) -> int:
 
 class Packed8:
     """n vectors in 8 bits: `values` uint8 [n, columns rounded up to 128] (zero past `columns`), `scale` uint8
-    [groups, n], `dtype` of the vectors it was made from."""
+    [groups, n], `dtype` of the vectors it was made from, `shape` (..., columns) of the tensor that held them: n vectors in
+    all.  The calls that take it trust these to fit each other, so none can be replaced."""
 
     __slots__ = ("values", "scale", "columns", "dtype", "shape")
 
     def __init__(self, values: torch.Tensor, scale: torch.Tensor, columns: int, dtype: torch.dtype, shape=None):
+        if columns < 0:
+            raise ValueError(f"columns is {columns}, must not be negative")
         groups = -(-columns // BLOCK)
         if dtype not in _DTYPE:
             raise TypeError("dtype must be float32, bfloat16 or float16")
@@ -82,17 +85,33 @@ class Packed8:
             raise ValueError(f"values must be a contiguous uint8 tensor [n, {groups * BLOCK}]")
         if scale.dtype != torch.uint8 or tuple(scale.shape) != (groups, values.shape[0]) or not scale.is_contiguous():
             raise ValueError(f"scale must be a contiguous uint8 tensor [{groups}, {values.shape[0]}]")
+        n = values.shape[0]
+        shape = tuple(shape) if shape is not None else (n, columns)
+        if not shape or shape[-1] != columns or min(shape) < 0 or math.prod(shape[:-1]) != n:
+            raise ValueError(f"shape {shape} does not hold {n} vectors of {columns}")
         if not values.is_cuda or scale.device != values.device:
             raise ValueError("values and scale must be on one GPU")
-        self.values, self.scale, self.columns, self.dtype = values, scale, columns, dtype
-        self.shape = tuple(shape) if shape is not None else (values.shape[0], columns)
+        self._fill(values, scale, columns, dtype, shape)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"Packed8.{name} cannot be replaced")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"Packed8.{name} cannot be removed")
+
+    def __reduce__(self):
+        return Packed8._made, (self.values, self.scale, self.columns, self.dtype, self.shape)
 
     @classmethod
     def _made(cls, values, scale, columns, dtype, shape):
         """Of tensors made here: nothing to check."""
         q = object.__new__(cls)
-        q.values, q.scale, q.columns, q.dtype, q.shape = values, scale, columns, dtype, shape
+        q._fill(values, scale, columns, dtype, shape)
         return q
+
+    def _fill(self, *fields) -> None:
+        for put, value in zip(_PUT, fields):
+            put(self, value)
 
     @property
     def n(self) -> int:
@@ -108,6 +127,9 @@ class Packed8:
         _call(device, L.lib().spmv_hip_restore8_dev, n, self.columns, self.values.data_ptr(), ld8, self.scale.data_ptr(), n,
               x.data_ptr(), _DTYPE[dtype], self.columns, _raw_stream(device.index))
         return x
+
+
+_PUT = tuple(getattr(Packed8, name).__set__ for name in Packed8.__slots__)
 
 
 def _rounded(rows: torch.Tensor, shape) -> Packed8:

@@ -1,6 +1,8 @@
 """8-bit block matrices without a GPU: the oracle against torch's own e4m3 conversion, and every refusal that the library
 or the Python layer makes before it needs a device."""
+import copy
 import ctypes as C
+import pickle
 
 import numpy as np
 import pytest
@@ -104,3 +106,25 @@ def test_python_layer_refuses_what_is_not_on_a_gpu():
     with pytest.raises(ValueError, match="block_ptr has shape"):
         block8.Block8(300, 300, [0, 1], [0])
     assert C.sizeof(S._lib.Info) > 0 and S.FORMAT_NAMES[S.BLOCK8] == "block8"
+
+
+@pytest.mark.parametrize("columns,shape", [(200, (1, 200)), (200, (3, 200)), (200, (2, 199)), (200, (2, 201)), (200, (400,)), (200, ()), (200, (200,)),
+                                           (200, (2, 2, 200)), (200, (-1, -2, 200)), (200, (0, 200)), (-5, None)])
+def test_packed_vectors_refuse_a_shape_of_other_vectors(columns, shape):
+    """restore() and product() size their results by the shape and write one vector for each of values' rows"""
+    groups = max(-(-columns // 128), 0)
+    values, scale = torch.zeros(2, groups * 128, dtype=torch.uint8), torch.zeros(groups, 2, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="does not hold 2 vectors|must not be negative"):
+        block8.Packed8(values, scale, columns, torch.float32, shape)
+
+
+def test_packed_vectors_keep_their_parts():
+    q = block8.Packed8._made(torch.zeros(2, 256, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 200, torch.float32, (2, 200))
+    for name in ("values", "scale", "columns", "dtype", "shape"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(q, name, (1, 200))
+        with pytest.raises(AttributeError, match=name):
+            delattr(q, name)
+    assert q.shape == (2, 200) and q.n == 2
+    for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert other.shape == q.shape and other.dtype == q.dtype and other.columns == 200 and torch.equal(other.values, q.values)
