@@ -1031,6 +1031,9 @@ __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, 
     // a thread's pieces of dy: 8 rows from `prow` on, of vectors 8 wave + q and 4 further
     const int prow = row0 + 8 * (i ^ (q << 1 | (wave & 1) << 3));
     const unsigned lddy = (unsigned)g.lddy, near = ((8 * wave + q) * lddy + prow) * 2;
+    // The bound of the loads: the last vector's rows up to a whole 16 bytes.  A piece that the bound cuts loses the word it cuts
+    // (odd `rows`); what lies past the rows is inside the piece's own 16 aligned bytes and reaches only rows that are not stored.
+    const unsigned records = ((STEP - 1) * lddy + (((unsigned)g.rows + 7) & ~7u)) * 2;
     auto issue = [&](auto slot, int k) {                     // 32 whole vectors
         constexpr int S = decltype(slot)::value;
         const int t0 = k * STEP;
@@ -1040,7 +1043,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, 
         __builtin_memcpy(&sx[S], g.xscale + (int64_t)col * g.lds + t0 + 8 * q, 8);
 #pragma unroll
         for (int p = 0; p < PARTS; p++) {
-            const u32x4 y = buffer(g.dy + p * g.plane + (int64_t)t0 * g.lddy, ((STEP - 1) * lddy + g.rows) * 2);
+            const u32x4 y = buffer(g.dy + p * g.plane + (int64_t)t0 * g.lddy, records);
 #pragma unroll
             for (int j = 0; j < 2; j++) load_to_lds<true>(y, near + j * 8 * lddy, &Y[S][p][(8 * wave + 4 * j) * 256]);
         }
