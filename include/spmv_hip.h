@@ -361,11 +361,12 @@ int spmv_hip_dist_free(spmv_hip_dist *d);
  *
  * Number format.  Values are e4m3 (OCP: 4 exponent bits, 3 mantissa bits, no
  * infinities, largest finite 448).  A group of values shares one scale 2^(b-127),
- * kept as the byte b, 1 <= b <= 254.  The scale of a group is the least power of
+ * kept as the byte b, 1 <= b <= 247.  The scale of a group is the least power of
  * two >= 2^-126 that brings its largest finite magnitude to at most 448 (1 for a
  * group of zeros), and a value is x / scale rounded to nearest even: dividing by
  * the scale is exact, so that rounding is the only one.  Infinities and NaN become
- * NaN and do not count for the scale.  Groups are the matrix's blocks, and 128
+ * NaN and do not count for the scale.  Finite numbers of 32 bits never need a byte
+ * above 247; the products do not take one (it is not looked for).  Groups are the matrix's blocks, and 128
  * consecutive entries of a vector.
  *
  * The matrix: block k covers rows 128 I .. 128 I + 127 (I = its block row) and
@@ -414,12 +415,15 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
  * 8 bits inside the product, and n is at most SPMV_HIP_BLOCK8_MAX_WIDE (quantize
  * larger blocks of vectors first).  y in F32, BF16 or F16.  Products are exact and
  * sums 32 bits wide, but for BF16 results of more than 64 vectors in 8 bits: those may
- * be off by 7 * 2^-13 of the sum of the terms' magnitudes (the 8-bit matrix instruction). */
+ * be off by 7 * 2^-13 of the sum of the terms' magnitudes (the 8-bit matrix instruction).
+ * Here and in the backward call, entries of groups whose scale byte is below 4 (largest
+ * magnitude below 2^-115) may count with an error of 2^-133. */
 enum { SPMV_HIP_BLOCK8_MAX_WIDE = 1024 };
 int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, int x_dtype, int64_t ldx,
                              const uint8_t *d_scale, int64_t lds, void *d_y, int y_dtype, int64_t ldy, void *stream);
 /* The two gradients of the product, from dy (F32, BF16 or F16, used as it is, not
- * rounded to 8 bits); either may be left out with NULL.
+ * rounded to 8 bits; F32 entries below 2^-110 lose what lies under 2^-133); either may
+ * be left out with NULL.
  *   dx_v = A^T dy_v: the gradient of x, in F32, BF16 or F16
  *   d_dvalues[k][r][c] = sum over v of dy_v[128 I_k + r] * x_v[128 J_k + c]: the
  *     gradient of the stored blocks (I_k, J_k = block k's row and column), x as its

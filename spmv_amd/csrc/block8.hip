@@ -35,6 +35,8 @@ __host__ __device__ __forceinline__ int block8_offset(int row, int col)
 }
 
 __device__ __forceinline__ float scale_value(int b) { return __int_as_float(b << 23); }      // 2^(b-127)
+// 2^(b-128), b >= 1, for the scaled conversions alone: they read the exponent's byte, and 0 there stands for 2^-127
+__device__ __forceinline__ float scale_half(int b) { return __int_as_float((b - 1) << 23); }
 
 // scale byte of a group whose largest finite magnitude is `amax`: the least e >= -126 with amax <= 448 * 2^e =
 // 1.75 * 2^(e+8), from the bits -- adding 0x1fffff to a float carries into its exponent where the mantissa is above 1.75
@@ -51,7 +53,9 @@ __device__ __forceinline__ void unpack4(unsigned w, float scale, _Float16 *out) 
     const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true);
     out[0] = lo[0]; out[1] = lo[1]; out[2] = hi[0]; out[3] = hi[1];
 }
-// four e4m3 bytes times a power of two -> four bf16, exact
+// Four e4m3 bytes times a power of two -> four bf16.  The products widen by half the scale (scale_half) and double their
+// sums: the largest fp32 numbers round to 256 * 2^120, which bf16 has no number for, but half of it.  Exact for scale
+// bytes 4 to 247; below, where half a value can lie under bf16's smallest step, off by at most 2^-134 (2^-133 of the value).
 __device__ __forceinline__ void unpack4(unsigned w, float scale, __bf16 *out)
 {
     const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
@@ -352,7 +356,7 @@ __device__ __forceinline__ int table(const int *p, int k)
 // for small matrices by latency -- a wave's next block is on its way while it works on one -- and with more vectors by
 // widening x, which every strip's workgroup does again: two strips share it.  XT: uint8_t (x in 8 bits) or a wide type,
 // rounded to 8 bits here: lane (i, q) holds the 32 entries of vector i that it multiplies, 4 lanes a group of 128.
-// Operands are widened to bf16 (exact), sums are 32 bits.
+// Operands are widened to bf16 (unpack4), sums are 32 bits.
 template <typename XT, int NT, int W, int S>
 __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, int columns, const int *__restrict__ block_ptr,
                                                                const int *__restrict__ block_col, const uint8_t *__restrict__ val8,
@@ -412,7 +416,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         return s;
     };
     auto use = [&](const Stage &s) {
-        const float sa = scale_value(s.scale);
+        const float sa = scale_half(s.scale);
         bf16x8 a[S][4];
 #pragma unroll
         for (int d = 0; d < 8 * S; d++) unpack4(s.a[d >> 3][d >> 2 & 1][d & 3], sa, (__bf16 *)&a[d >> 3][d >> 1 & 3] + 4 * (d & 1));
@@ -420,18 +424,19 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
         for (int t = 0; t < NT; t++) {
             const Vector v = AHEAD ? s.x[AHEAD ? t : 0] : load_x(t, s.group);
             unsigned w8[8];
-            float sx;
+            int bx;
             if constexpr (kEight) {
                 __builtin_memcpy(w8, v.h, 32);
-                sx = scale_value(v.scale);
+                bx = v.scale;
             } else {
                 float top = fmaxf(finite_top(v.h[0]), finite_top(v.h[1]));
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                sx = scale_value(scale_byte(top));
-                v.h[0].pack(sx, w8);
-                v.h[1].pack(sx, w8 + 4);
+                bx = scale_byte(top);
+                v.h[0].pack(scale_value(bx), w8);
+                v.h[1].pack(scale_value(bx), w8 + 4);
             }
+            const float sx = scale_half(bx);
 #pragma unroll
             for (int p = 0; p < 4; p++) {
                 bf16x8 b;
@@ -463,6 +468,7 @@ __global__ __launch_bounds__(W *kWave) void few_vectors_kernel(int n, int rows, 
             f32x4 s = part[0][t][l];
 #pragma unroll
             for (int w = 1; w < W; w++) s += part[w][t][l];
+            s *= 4.0f;                                       // both operands were halves
             const int r0 = brow * kB + (strip >> 2) * 64 + 16 * (l >> 4) + (strip & 3);
             if (v >= n) continue;
             for (int e = 0; e < 4; e++) {
@@ -605,7 +611,7 @@ struct ProductArgs {
 // XOR so that the 8 lanes of a read cycle meet 8 different pieces; the blocks, whose layout is the operand's, go straight
 // to the registers of the two waves that need each half.  Vector NU i + u belongs to lane i of tile u: a lane's scale
 // bytes are neighbours.
-// EXACT: operands widened to bf16 in registers (exact), 32-bit sums.  Otherwise the 8-bit matrix instruction, which applies
+// EXACT: operands widened to bf16 in registers (unpack4), 32-bit sums.  Otherwise the 8-bit matrix instruction, which applies
 // both scales and runs at twice the rate, but aligns 8 products at a time and drops what lies 13 bits below the largest:
 // good to about 16 bits, for bf16 results only.
 // 8192 vectors, full 8192 x 8192, bf16: 435 us, 2.5 PFLOP/s (a library product of plain 8-bit matrices of that size reaches
@@ -660,7 +666,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
         const uint8_t *half = g.val8 + (int64_t)b * kBlockBytes + wm * (kBlockBytes / 2);
 #pragma unroll
         for (int s = 0; s < 4; s++) a[S][s] = join(*(const u32x4 *)(half + (lane * 16u + s * 2048)), *(const u32x4 *)(half + (lane * 16u + s * 2048 + 1024)));
-        sa[S] = scale;
+        sa[S] = EXACT ? scale - 1 : scale;                   // of half the scale, for widening (unpack4)
         sx[S] = 0;
         __builtin_memcpy(&sx[S], g.xscale + (int64_t)c * g.lds + (v0 - back), NU);
         look_up(min(b + 1, last - 1));
@@ -682,7 +688,8 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) w[u] = operand(u);
         if constexpr (NU < 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
-        const uint64_t bytes = sx[S] >> (8 * min(back, 7));
+        // for widening those of half the scales; past the last vector, in the upper bytes, whatever it is
+        const uint64_t bytes = (sx[S] >> (8 * min(back, 7))) - (EXACT ? 0x0101010101010101u : 0);
         bf16x8 aw[4][EXACT ? 4 : 1];
         if constexpr (EXACT) {
             const float fa = scale_value(sa[S]);
@@ -729,14 +736,16 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
     for (int k = 0; k < 4; k++)
 #pragma unroll
         for (int u = 0; u < NU; u++) {
-            const f32x4 f = {acc[u][0][k], acc[u][1][k], acc[u][2][k], acc[u][3][k]};
+            f32x4 f = {acc[u][0][k], acc[u][1][k], acc[u][2][k], acc[u][3][k]};
+            if (EXACT) f *= 4.0f;                            // both operands were halves
             const int v = v1 + NU * k + u;
             if (v < g.n && r < g.rows) store_row<OT, 1>(y + (int64_t)v * g.ldy + r, g.rows - r, &f);
         }
 }
 
 // dy is used as it is: as PARTS bf16 numbers that add up to it exactly (1 for bf16, 2 for fp16, 3 for fp32: each holds 8
-// bits of the mantissa), one matrix instruction each
+// bits of the mantissa), one matrix instruction each.  Of fp32 entries below 2^-110 what lies under bf16's smallest step,
+// 2^-133, is lost.
 template <typename DT> struct parts_of { static constexpr int value = 1; };
 template <> struct parts_of<_Float16> { static constexpr int value = 2; };
 template <> struct parts_of<float> { static constexpr int value = 3; };
@@ -790,7 +799,7 @@ struct TransposedArgs {
 };
 
 // dx = A^T dy, half a block (64 rows) a step, blocks and vectors through LDS.  ds_read_b64_tr_b8 hands every lane one
-// column of 8 rows of the block, widened to bf16 (exact) on the way to the matrix instruction.  8 rows of dy are 2 rows in
+// column of 8 rows of the block, widened to bf16 (unpack4) on the way to the matrix instruction.  8 rows of dy are 2 rows in
 // each of four strips of the block (block8_offset); in LDS the 4-row pieces of a 16 x 16 subtile are exchanged by XOR
 // with the strip, which puts the four on different banks.  The blocks of a last block row that is not whole come last in
 // every list: they are taken after the others, one by one, with the entries past the end masked (dy in parts is padded
@@ -894,7 +903,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void transposed_kernel(TransposedArgs
 #pragma unroll
                     for (int u = 0; u < (ALL ? NU : 1); u++) b[h][part][u] = read_b(h, part, u);
         }
-        const float fa = scale_value(sa[S]);
+        const float fa = HALF ? scale_value(sa[S]) : scale_half(sa[S]);
         between();
         e8 a[2][4];
 #pragma unroll
@@ -983,6 +992,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void transposed_kernel(TransposedArgs
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             const int c = major * kB + wm * 64 + 16 * s + 4 * q;
+            if (!HALF) acc[u][s] *= 2.0f;                    // the blocks were halves
             if (c < g.columns) store_row<OT, 1>(dx + (int64_t)v * g.lddx + c, g.columns - c, &acc[u][s]);
         }
     }
@@ -1002,7 +1012,7 @@ struct GradientArgs {
 // and have to be turned.  dy, which all waves share, comes into LDS by direct loads and is turned by ds_read_b64_tr_b16 (a
 // lane gets one row of 4 vectors); a vector's 16-byte pieces are exchanged by XOR so that the 8 vectors of a read cycle
 // lie on different banks.  x goes straight into the registers of the wave that needs it, 4 columns of 8 vectors a lane:
-// widened there with the vectors' scales (exact; pairs of columns, which share a scale), then the pairs are turned.  Lane
+// widened there with the vectors' scales (unpack4; pairs of columns, which share a scale), then the pairs are turned.  Lane
 // i's columns are 4 i + s.
 // 8192 vectors, full 8192 x 8192, bf16: 875-910 us, 1.2 PFLOP/s; the matrix pipes are busy 59 % of the cycles at 2 GHz.  x
 // through LDS as well, a third of the loads, left that as it is and made fp32's slower (fewer stages fit).
@@ -1089,9 +1099,10 @@ __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, 
         bf16x8 a[4];
         {
             unsigned pair[8][2];                             // columns (0, 1) and (2, 3) of 8 vectors
+            const uint64_t halves = sx[S] - 0x0101010101010101u;
 #pragma unroll
             for (int w = 0; w < 8; w++) {
-                const float f = scale_value((int)((unsigned)(sx[S] >> (8 * w)) & 255));
+                const float f = scale_value((int)((unsigned)(halves >> (8 * w)) & 255));
                 __bf16 u[4];
                 unpack4(xr[S][w], f, u);
                 __builtin_memcpy(pair[w], u, 8);
@@ -1158,7 +1169,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, 
             const int here = row0 + n0 + 4 * q + row < g.edge ? left : 0;
             f32x4 v;
 #pragma unroll
-            for (int s = 0; s < 4; s++) v[s] = s < here ? acc[u][s][r] : 0.0f;
+            for (int s = 0; s < 4; s++) v[s] = s < here ? 2.0f * acc[u][s][r] : 0.0f;      // x was halved
             if (g.accumulate) {
                 Raw<OT, 4> old;
                 old.load(o + row * kB, 4);

@@ -72,3 +72,103 @@ def test_gradients_from_dy_in_place_that_ends_inside_16_bytes(rows, columns, kee
             d = _in_place(dy.to(dtype), gap)
             _equal(c.A.gradient(d, q), c.sampled(torch.mm(dy.t().contiguous(), x)), n, gap)
             _equal(c.A.product_t(d, F32), torch.mm(dy, c.dense), n, gap)
+
+
+# ---- the largest and the smallest numbers ---------------------------------------------------------------------------
+
+def _close(got, want, terms, magnitude, extra=0.0, floor=0.0):
+    """`terms` additions in 32 bits of terms whose magnitudes add up to `magnitude` (each off by at most 2^-23 of the partial
+    sum), `extra` more of `magnitude` and `floor` whatever it is, then one rounding to got's type"""
+    eps, least = torch.finfo(got.dtype).eps / 2, torch.finfo(got.dtype).smallest_normal
+    g = got.double()
+    want, magnitude = want.to(DEV), magnitude.to(DEV)
+    tol = (terms * 2.0 ** -23 + extra) * magnitude * (1 + eps) + eps * want.abs() + 2 * eps * least + floor
+    over = want.abs() > torch.finfo(got.dtype).max
+    off = torch.where(over, torch.zeros_like(want), (g - want).abs() - tol)
+    assert bool((off <= 0).all()), (float(off.max()), torch.nonzero(~(off <= 0))[0].tolist())
+    assert bool(torch.isinf(g[over]).all())
+
+
+EIGHT = 7 * 2.0 ** -13             # the 8-bit matrix instruction: what it drops of 8 products, each below 2^-13 of the largest
+
+
+def _blocks(c, values):
+    """the numbers the matrix's 8-bit blocks stand for, dense, and the same of their magnitudes"""
+    blocks, _ = O.quantized_blocks(values.double().cpu().numpy(), c.ptr, c.col, c.rows, c.columns)
+    dense = lambda b: torch.from_numpy(O.dense(b, c.ptr, c.col, c.rows, c.columns)).to(DEV)
+    return dense(blocks), dense(np.abs(blocks))
+
+
+@pytest.mark.parametrize("y_dtype", TYPES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [5, 64, 90, 700])
+def test_the_largest_numbers_in_x(n, dtype, y_dtype):
+    """their 8-bit form is 2^128; times small values, or zero, that is finite, in every path alike"""
+    c = Whole(700, 260, 1.0, 1)
+    values = _whole(2, len(c.col), 128, 128).float() * 2.0 ** -122
+    values[:, ::3, :] = 0
+    c.A.set_values(values)
+    a, mag = _blocks(c, values)
+    top = torch.finfo(dtype).max
+    x = _whole(3, n, 260).to(dtype)
+    x[0, 5], x[1, 200], x[n - 1, 259], x[n - 1, 0] = top, -top, top, top
+    xq = torch.from_numpy(O.quantized(x.double().cpu().numpy())).to(DEV)
+    assert float(xq.max()) == 2.0 ** 128
+    want, magnitude = torch.mm(xq, a.t().contiguous()), torch.mm(xq.abs(), mag.t().contiguous())
+    for given in (x, quantize(x)):
+        extra = EIGHT if y_dtype == BF16 and n > 64 else 0.0
+        _close(c.A.product(given, y_dtype), want, 260, magnitude, extra)
+    # the gradient of the blocks, from dy small enough for it
+    for dy_dtype in (F32, BF16):
+        dy = (_whole(4, n, 700) * 2.0 ** -30).to(dy_dtype)
+        dy[:, 10] = 0
+        d = dy.double()
+        want, magnitude = (c.sampled(torch.mm(t.t().contiguous(), u)) for t, u in ((d, xq), (d.abs(), xq.abs())))
+        _close(c.A.gradient(dy, quantize(x)), want, 3 * n, magnitude)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 64, 90, 700])
+def test_the_largest_numbers_in_the_matrix(n, dtype):
+    c = Whole(700, 260, 1.0, 1)
+    values = _whole(2, len(c.col), 128, 128).float()
+    values[:, 3, 5], values[:, 100, 100] = torch.finfo(F32).max, -torch.finfo(F32).max
+    c.A.set_values(values)
+    a, mag = _blocks(c, values)
+    assert float(a.max()) == 2.0 ** 128
+    x = (_whole(3, n, 260) * 2.0 ** (-10 if dtype == F16 else -60)).to(dtype)
+    x[:, 4] = 0
+    xq = torch.from_numpy(O.quantized(x.double().cpu().numpy())).to(DEV)
+    want, magnitude = torch.mm(xq, a.t().contiguous()), torch.mm(xq.abs(), mag.t().contiguous())
+    for y_dtype in TYPES:
+        extra = EIGHT if y_dtype == BF16 and n > 64 else 0.0
+        _close(c.A.product(x, y_dtype), want, 260, magnitude, extra)
+    dy = (_whole(4, n, 700) * 2.0 ** -20).to(dtype)
+    dy[:, 10] = 0
+    d = dy.double()
+    _close(c.A.product_t(dy, F32), torch.mm(d, a), 2100, torch.mm(d.abs(), mag))
+
+
+@pytest.mark.parametrize("n", [5, 90])
+@pytest.mark.parametrize("size", [-100, -114, -120, -130])
+def test_the_smallest_numbers_in_x_and_the_matrix(n, size):
+    """exact down to groups of 2^-115; below, an entry counts with an error of at most 2^-133"""
+    c = Whole(300, 260, 1.0, 1)
+    small, large = _whole(2, len(c.col), 128, 128).float() * 2.0 ** (size - 3), _whole(3, len(c.col), 128, 128).float() * 2.0 ** 90
+    tiny = lambda seed, *shape: _whole(seed, *shape).float() * 2.0 ** (size - 3)
+    off = 0.0 if size >= -114 else 2.0 ** -133
+    x = tiny(4, n, 260)
+    c.A.set_values(large)
+    a, _ = _blocks(c, large)
+    xq = torch.from_numpy(O.quantized(x.double().cpu().numpy())).to(DEV)
+    # sums of whole numbers times one power of two: exact but for what the entries lose
+    want, lost = torch.mm(xq, a.t().contiguous()), off * a.abs().sum(1)
+    for given in (x, quantize(x)):
+        got = c.A.product(given).double()
+        assert bool(((got - want).abs() <= lost + 2.0 ** -23 * lost).all())
+    dy = _whole(5, n, 300).float() * 2.0 ** 90
+    want = c.sampled(torch.mm(dy.double().t().contiguous(), xq))
+    assert bool(((c.A.gradient(dy, quantize(x)).double() - want).abs() <= off * 1.001 * n * 2.0 ** 93).all())
+    c.A.set_values(small)
+    a, _ = _blocks(c, small)
+    assert bool(((c.A.product_t(dy).double() - torch.mm(dy.double(), a)).abs() <= off * 1.001 * 300 * 2.0 ** 93).all())
