@@ -27,6 +27,7 @@ from .matrix import Matrix
 BLOCK = 128
 MAX_WIDE = 1024                       # vectors a product rounds to 8 bits by itself (SPMV_HIP_BLOCK8_MAX_WIDE)
 MAX_APART = 1 << 23                   # entries between vectors of dy, less than
+MAX_INT = (1 << 31) - 1               # of the library's sizes; ctypes would cut a larger one off without a word
 _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
 
@@ -57,6 +58,8 @@ def _wide(name: str, x: torch.Tensor, length: int | None = None) -> torch.Tensor
         x = x.detach()
     if x.dim() != 2:
         x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    if x.shape[0] > MAX_INT or x.shape[1] > MAX_INT:
+        raise ValueError(f"{name} holds {x.shape[0]} vectors of {x.shape[1]}, more than 2^31 - 1")
     if not x.is_contiguous():
         n, columns = x.shape
         if columns > 1 and x.stride(1) != 1 or n > 1 and x.stride(0) < columns:
@@ -86,6 +89,8 @@ class Packed8:
         if scale.dtype != torch.uint8 or tuple(scale.shape) != (groups, values.shape[0]) or not scale.is_contiguous():
             raise ValueError(f"scale must be a contiguous uint8 tensor [{groups}, {values.shape[0]}]")
         n = values.shape[0]
+        if n > MAX_INT or columns > MAX_INT:
+            raise ValueError(f"{n} vectors of {columns} are more than 2^31 - 1")
         shape = tuple(shape) if shape is not None else (n, columns)
         if not shape or shape[-1] != columns or min(shape) < 0 or math.prod(shape[:-1]) != n:
             raise ValueError(f"shape {shape} does not hold {n} vectors of {columns}")
@@ -148,13 +153,24 @@ def quantize(x: torch.Tensor) -> Packed8:
     return _rounded(_wide("x", x), x.shape)
 
 
+def _whole(name: str, a) -> np.ndarray:
+    """a as the library's 32-bit integers, refused where that would change a number."""
+    a = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        whole = np.ascontiguousarray(a, np.int32)
+    if not np.array_equal(a, whole):
+        raise ValueError(f"{name} must hold whole numbers of 32 bits")
+    return whole
+
+
 class Block8(Matrix):
     """A handle of 8-bit blocks on the current device.  block_ptr [ceil(rows / 128) + 1] and block_col are host integers
     like the row_ptr and col of a CSR matrix, in units of blocks."""
 
     def __init__(self, rows: int, columns: int, block_ptr, block_col):
-        ptr = np.ascontiguousarray(block_ptr, np.int32)
-        col = np.ascontiguousarray(block_col, np.int32)
+        if max(rows, columns) > MAX_INT:
+            raise ValueError(f"{rows} x {columns} is more than 2^31 - 1 a side")
+        ptr, col = _whole("block_ptr", block_ptr), _whole("block_col", block_col)
         if ptr.shape != (-(-max(rows, 0) // BLOCK) + 1,) or col.ndim != 1:
             raise ValueError(f"block_ptr has shape {ptr.shape} for {rows} rows, block_col {col.shape}")
         super().__init__(L.lib().spmv_hip_create_block8(rows, columns, len(col), ptr.ctypes.data, col.ctypes.data))

@@ -128,3 +128,22 @@ def test_packed_vectors_keep_their_parts():
     assert q.shape == (2, 200) and q.n == 2
     for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
         assert other.shape == q.shape and other.dtype == q.dtype and other.columns == 200 and torch.equal(other.values, q.values)
+
+
+@pytest.mark.parametrize("rows,columns,ptr,col,text", [
+    (130, 2 ** 32 + 128, [0, 1, 1], [0], "more than 2\\^31"),     # would be a matrix of 128 columns
+    (2 ** 31, 128, [0, 1], [0], "more than 2\\^31"),
+    (130, 130, [0, 1, 1], [2 ** 32], "block_col must hold"),      # would be block column 0
+    (130, 130, [0, 1, 2 ** 32 + 1], [0], "block_ptr must hold"),
+    (130, 130, [0, 1, 1], [0.5], "block_col must hold"),
+    (130, 130, [0, 1, float("nan")], [0], "block_ptr must hold"),
+])
+def test_sizes_that_32_bits_would_change_are_refused(rows, columns, ptr, col, text):
+    with pytest.raises(ValueError, match=text):
+        block8.Block8(rows, columns, ptr, col)
+
+
+def test_whole_numbers_of_any_type_make_a_pattern():
+    for a in ([0, 1, 2], np.arange(3), np.arange(3, dtype=np.uint64), torch.arange(3), np.array([0.0, 1.0, 2.0])):
+        assert np.array_equal(block8._whole("a", a), np.arange(3)) and block8._whole("a", a).dtype == np.int32
+    assert block8._whole("a", []).shape == (0,)

@@ -172,3 +172,15 @@ def test_the_smallest_numbers_in_x_and_the_matrix(n, size):
     c.A.set_values(small)
     a, _ = _blocks(c, small)
     assert bool(((c.A.product_t(dy).double() - torch.mm(dy.double(), a)).abs() <= off * 1.001 * 300 * 2.0 ** 93).all())
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------------
+
+def test_more_vectors_than_32_bits_count_are_refused():
+    """without memory for them: one entry, broadcast"""
+    A = Block8.full(1, 1)
+    for n in (2 ** 31, 2 ** 32 + 5):
+        many = torch.ones(1, 1, device=DEV, dtype=BF16).expand(n, 1)
+        for f in (quantize, A.product, A.linear, A.product_t, lambda x: A.gradient(x, quantize(x[:1]))):
+            with pytest.raises(ValueError, match="more than 2"):
+                f(many)
