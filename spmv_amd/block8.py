@@ -19,6 +19,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -306,9 +307,12 @@ class Block8(Matrix):
 
     def linear(self, x: torch.Tensor) -> torch.Tensor:
         """y = A x, differentiable in x and in the tensor that set_values took.  Between the passes x is kept in 8 bits;
-        the backward pass refuses a matrix whose values were set again meanwhile."""
+        the backward pass refuses a matrix whose values were set again meanwhile.  Forward-mode differentiation is refused."""
         if not isinstance(x, torch.Tensor):
             raise TypeError("x must be a tensor")
+        for t in (x, self.values):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("linear has no forward-mode derivative")
         if torch.is_grad_enabled() and (x.requires_grad or self.values is not None and self.values.requires_grad):
             return _Linear.apply(x, self.values, self)
         return self.product(x)

@@ -7,6 +7,7 @@ import pickle
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import spmv_amd as S
 from spmv_amd import block8
@@ -147,3 +148,17 @@ def test_whole_numbers_of_any_type_make_a_pattern():
     for a in ([0, 1, 2], np.arange(3), np.arange(3, dtype=np.uint64), torch.arange(3), np.array([0.0, 1.0, 2.0])):
         assert np.array_equal(block8._whole("a", a), np.arange(3)) and block8._whole("a", a).dtype == np.int32
     assert block8._whole("a", []).shape == (0,)
+
+
+def test_linear_refuses_forward_mode():
+    """a dual tensor does not require grad: without this its tangent would be dropped"""
+    A = object.__new__(block8.Block8)
+    A._h, A.columns = None, 128
+    t = torch.ones(2, 128)
+    with forward_ad.dual_level():
+        for x, A.values in ((forward_ad.make_dual(t, t), None), (t, forward_ad.make_dual(torch.ones(1, 128, 128), torch.ones(1, 128, 128)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.linear(x)
+    A.values = None
+    with pytest.raises(ValueError, match="no CPU path"):
+        A.linear(t)
