@@ -37,6 +37,13 @@ _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _stream(index: int) -> int:
+    """The stream of a call.  torch.jit.trace would record the tensors made for the results, and not the calls that fill them."""
+    if torch.jit.is_tracing():
+        raise RuntimeError("products with 8-bit blocks cannot be traced by torch.jit")
+    return _raw_stream(index)
+
+
 def _call(device: torch.device, f, *args) -> None:
     """A library call without a handle, which knows no device of its own, on `device`."""
     if torch.cuda.current_device() == device.index:
@@ -131,7 +138,7 @@ class Packed8:
         device, (n, ld8) = self.values.device, self.values.shape
         x = self.values.new_empty(self.shape, dtype=dtype)
         _call(device, L.lib().spmv_hip_restore8_dev, n, self.columns, self.values.data_ptr(), ld8, self.scale.data_ptr(), n,
-              x.data_ptr(), _DTYPE[dtype], self.columns, _raw_stream(device.index))
+              x.data_ptr(), _DTYPE[dtype], self.columns, _stream(device.index))
         return x
 
 
@@ -145,7 +152,7 @@ def _rounded(rows: torch.Tensor, shape) -> Packed8:
     values = rows.new_empty((n, groups * BLOCK), dtype=torch.uint8)
     scale = rows.new_empty((groups, n), dtype=torch.uint8)
     _call(device, L.lib().spmv_hip_quantize8_dev, n, columns, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows), values.data_ptr(),
-          groups * BLOCK, scale.data_ptr(), n, _raw_stream(device.index))
+          groups * BLOCK, scale.data_ptr(), n, _stream(device.index))
     return Packed8._made(values, scale, columns, rows.dtype, shape)
 
 
@@ -212,7 +219,7 @@ class Block8(Matrix):
         """Rounds values [blocks, 128, 128] into the matrix, on the current stream (products on others have to wait for
         it).  linear() returns the gradient of this tensor."""
         self._blocks("values", values, _DTYPE)
-        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _raw_stream(self._index)))
+        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _stream(self._index)))
         self.values = values
         self._version += 1
 
@@ -222,7 +229,7 @@ class Block8(Matrix):
         if scale.dtype != torch.uint8 or tuple(scale.shape) != (self.nblocks,) or not scale.is_contiguous():
             raise ValueError(f"scale must be a contiguous uint8 tensor [{self.nblocks}]")
         self._here("scale", scale)
-        L.check(L.lib().spmv_hip_block8_load_dev(self._h, values8.data_ptr(), scale.data_ptr(), _raw_stream(self._index)))
+        L.check(L.lib().spmv_hip_block8_load_dev(self._h, values8.data_ptr(), scale.data_ptr(), _stream(self._index)))
         self.values = None
         self._version += 1
 
@@ -230,7 +237,7 @@ class Block8(Matrix):
         """(values8 uint8 [blocks, 128, 128], scale uint8 [blocks]): what load takes."""
         values8 = torch.empty((self.nblocks, BLOCK, BLOCK), dtype=torch.uint8, device=self.device)
         scale = torch.empty(self.nblocks, dtype=torch.uint8, device=self.device)
-        L.check(L.lib().spmv_hip_block8_store_dev(self._h, values8.data_ptr(), scale.data_ptr(), _raw_stream(self._index)))
+        L.check(L.lib().spmv_hip_block8_store_dev(self._h, values8.data_ptr(), scale.data_ptr(), _stream(self._index)))
         return values8, scale
 
     def product(self, x, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -248,7 +255,7 @@ class Block8(Matrix):
                     self.nblocks * (-(-n // 16) * rows.element_size()) < (8500 if n <= 16 else 7500):
                 y = self._out(out, shape, dtype or rows.dtype, rows)
                 L.check(L.lib().spmv_hip_block8_mult_dev(self._h, n, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
-                                                         None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _raw_stream(self._index)))
+                                                         None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self._index)))
                 return y
             dtype = dtype or rows.dtype
             x = _rounded(rows, rows.shape)
@@ -259,7 +266,7 @@ class Block8(Matrix):
             shape = (*x.shape[:-1], self.rows)
         y = self._out(out, shape, dtype or x.dtype, x.values)
         L.check(L.lib().spmv_hip_block8_mult_dev(self._h, x.n, x.values.data_ptr(), L.E4M3, x.values.shape[1], x.scale.data_ptr(),
-                                                 x.n, y.data_ptr(), _DTYPE[y.dtype], self.rows, _raw_stream(self._index)))
+                                                 x.n, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self._index)))
         return y
 
     def product_t(self, dy: torch.Tensor, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -303,7 +310,7 @@ class Block8(Matrix):
             *((x.values.data_ptr(), x.values.shape[1], x.scale.data_ptr(), x.n) if dv is not None else (None, 0, None, 0)),
             *((dx.data_ptr(), _DTYPE[dx.dtype], self.columns) if dx is not None else (None, 0, 0)),
             *((dv.data_ptr(), _DTYPE[dv.dtype]) if dv is not None else (None, 0)), accumulate,
-            work.data_ptr() if work is not None else None, _raw_stream(self._index)))
+            work.data_ptr() if work is not None else None, _stream(self._index)))
 
     def linear(self, x: torch.Tensor) -> torch.Tensor:
         """y = A x, differentiable in x and in the tensor that set_values took.  Between the passes x is kept in 8 bits;

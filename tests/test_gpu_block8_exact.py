@@ -184,3 +184,26 @@ def test_more_vectors_than_32_bits_count_are_refused():
         for f in (quantize, A.product, A.linear, A.product_t, lambda x: A.gradient(x, quantize(x[:1]))):
             with pytest.raises(ValueError, match="more than 2"):
                 f(many)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+def test_calls_are_not_traced():
+    """a trace would hold the results' allocations alone"""
+    c = Whole(200, 300, 1.0, 1)
+    x, dy, w = _whole(2, 3, 300).float(), _whole(3, 3, 200).float(), c.values.float()
+    q = quantize(x)
+
+    def load(scale):
+        c.A.load(torch.zeros(c.A.nblocks, 128, 128, dtype=torch.uint8, device=DEV), scale)
+        return scale
+
+    def set_values(v):
+        c.A.set_values(v)
+        return v
+
+    for f, a in ((lambda t: quantize(t).values, x), (lambda t: q.restore() + t, x), (c.A.product, x), (c.A.linear, x), (lambda t: c.A.product(q) + t, dy),
+                 (c.A.product_t, dy), (lambda t: c.A.gradient(t, q), dy), (set_values, w),
+                 (load, torch.full((c.A.nblocks,), 127, dtype=torch.uint8, device=DEV)), (lambda t: c.A.store()[0] + t, torch.zeros(1, device=DEV))):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (a,), check_trace=False)
+    _equal(c.A.product(x), torch.mm(_whole(2, 3, 300), c.dense.t().contiguous()))
