@@ -64,6 +64,8 @@ def _wide(name: str, x: torch.Tensor, length: int | None = None) -> torch.Tensor
         raise ValueError(f"{name} has shape {tuple(x.shape)}, expected (..., {length})")
     if x.requires_grad:
         x = x.detach()
+    if x.is_neg():                               # the memory holds the negated numbers
+        x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     if x.shape[0] > MAX_INT or x.shape[1] > MAX_INT:
@@ -210,7 +212,7 @@ class Block8(Matrix):
             raise TypeError("the result's type must be float32, bfloat16 or float16")
         if out is None:
             return like.new_empty(shape, dtype=dtype)
-        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous():
+        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous() or out.is_neg():
             raise ValueError(f"out must be contiguous {tuple(shape)} of {dtype}")
         self._here("out", out)
         return out
@@ -219,7 +221,8 @@ class Block8(Matrix):
         """Rounds values [blocks, 128, 128] into the matrix, on the current stream (products on others have to wait for
         it).  linear() returns the gradient of this tensor."""
         self._blocks("values", values, _DTYPE)
-        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, values.data_ptr(), _DTYPE[values.dtype], _stream(self._index)))
+        data = values.detach().resolve_neg() if values.is_neg() else values
+        L.check(L.lib().spmv_hip_block8_set_values_dev(self._h, data.data_ptr(), _DTYPE[values.dtype], _stream(self._index)))
         self.values = values
         self._version += 1
 

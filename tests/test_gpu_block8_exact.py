@@ -207,3 +207,27 @@ def test_calls_are_not_traced():
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, (a,), check_trace=False)
     _equal(c.A.product(x), torch.mm(_whole(2, 3, 300), c.dense.t().contiguous()))
+
+
+# ---- views ----------------------------------------------------------------------------------------------------------
+
+def test_negated_views():
+    """z.conj().imag and its like: the memory holds the numbers with the other sign"""
+    c = Whole(200, 300, 1.0, 1)
+    x, dy = _whole(2, 3, 300), _whole(3, 3, 200)
+    neg = lambda a: torch.complex(torch.zeros_like(a), -a).conj().imag
+    flat = lambda a: torch._neg_view(-a)
+    for view in (neg, flat):
+        xv, dv = view(x.float()), view(dy.float())
+        assert xv.is_neg() and dv.is_neg()
+        q = quantize(xv)
+        _equal(q.restore(), x)
+        _equal(c.A.product(xv), torch.mm(x, c.dense.t().contiguous()))
+        _equal(c.A.product_t(dv), torch.mm(dy, c.dense))
+        _equal(c.A.gradient(dv, q), c.sampled(torch.mm(dy.t().contiguous(), x)))
+    w = flat(-c.values.float())
+    c.A.set_values(w)
+    assert c.A.values is w
+    _equal(c.A.product(x.float()), -torch.mm(x, c.dense.t().contiguous()))
+    with pytest.raises(ValueError, match="out must be"):
+        c.A.product(x.float(), out=torch._neg_view(torch.zeros(3, 200, device=DEV)))
