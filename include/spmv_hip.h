@@ -385,7 +385,8 @@ int spmv_hip_dist_free(spmv_hip_dist *d);
  * into a graph.  set_values and load write the handle's values on their stream:
  * products on other streams have to be ordered behind them.  Products keep nothing
  * in the handle and may overlap.  Vectors of dy are less than 2^23 entries apart.
- * n = 0 is allowed.  The same call gives the same bits every time.
+ * n = 0 is allowed.  The same call gives the same bits every time.  A call's results
+ * and workspace lie apart from its operands.
  * spmv_hip_mult, _mult_dev, _mult_mv, _mult_mv_dev and _bench take such a handle too
  * (dtype F32): x is rounded to 8 bits on its way in.  "variant", "block_map" and
  * "hot_columns" do not apply. */

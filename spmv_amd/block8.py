@@ -81,6 +81,17 @@ def _ld(x: torch.Tensor) -> int:
     return max(x.stride(0), x.shape[1])
 
 
+def _meets(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Does the contiguous `out` share memory with the rows of t (contiguous inside, any distance apart)?"""
+    if out.numel() == 0 or t.numel() == 0:
+        return False
+    o, p, size = out.data_ptr(), t.data_ptr(), t.element_size()
+    n, row = (t.shape[0], t.shape[1] * size) if t.dim() == 2 else (1, t.numel() * size)
+    apart = max(t.stride(0) * size, row) if n > 1 else row
+    i = max((o - p - row) // apart + 1, 0)       # the first row that ends behind out's beginning
+    return i < n and p + i * apart < o + out.numel() * out.element_size()
+
+
 class Packed8:
     """n vectors in 8 bits: `values` uint8 [n, columns rounded up to 128] (zero past `columns`), `scale` uint8
     [groups, n], `dtype` of the vectors it was made from, `shape` (..., columns) of the tensor that held them: n vectors in
@@ -207,14 +218,16 @@ class Block8(Matrix):
             raise ValueError(f"{name} must be contiguous [{self.nblocks}, 128, 128], has shape {tuple(t.shape)}")
         self._here(name, t)
 
-    def _out(self, out, shape, dtype, like: torch.Tensor):
+    def _out(self, out, shape, dtype, *operands: torch.Tensor):
         if dtype not in _DTYPE:
             raise TypeError("the result's type must be float32, bfloat16 or float16")
         if out is None:
-            return like.new_empty(shape, dtype=dtype)
+            return operands[0].new_empty(shape, dtype=dtype)
         if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous() or out.is_neg():
             raise ValueError(f"out must be contiguous {tuple(shape)} of {dtype}")
         self._here("out", out)
+        if any(_meets(out, t) for t in operands):
+            raise ValueError("out shares memory with an operand, which is still read while it is written")
         return out
 
     def set_values(self, values: torch.Tensor) -> None:
@@ -267,7 +280,7 @@ class Block8(Matrix):
                 raise ValueError(f"x has {x.columns} columns, the matrix {self.columns}")
             self._here("x", x.values)
             shape = (*x.shape[:-1], self.rows)
-        y = self._out(out, shape, dtype or x.dtype, x.values)
+        y = self._out(out, shape, dtype or x.dtype, x.values, x.scale)
         L.check(L.lib().spmv_hip_block8_mult_dev(self._h, x.n, x.values.data_ptr(), L.E4M3, x.values.shape[1], x.scale.data_ptr(),
                                                  x.n, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self._index)))
         return y
@@ -290,7 +303,7 @@ class Block8(Matrix):
         self._here("x", x.values)
         if accumulate and out is None:
             raise ValueError("accumulate adds to out, which is missing")
-        dv = self._out(out, (self.nblocks, BLOCK, BLOCK), out.dtype if out is not None else dtype, d)
+        dv = self._out(out, (self.nblocks, BLOCK, BLOCK), out.dtype if out is not None else dtype, d, x.values, x.scale)
         self._backward(d, x, None, dv, accumulate)
         return dv
 

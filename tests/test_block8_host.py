@@ -162,3 +162,31 @@ def test_linear_refuses_forward_mode():
     A.values = None
     with pytest.raises(ValueError, match="no CPU path"):
         A.linear(t)
+
+
+def test_a_result_on_top_of_an_operand_is_refused():
+    """where the operand's rows lie, its gaps left out"""
+    rng = np.random.default_rng(1)
+    buf = torch.zeros(4000, dtype=torch.uint8)
+    for k in range(3000):
+        dtype = [torch.float32, torch.float16][k % 2]
+        size = torch.finfo(dtype).bits // 8
+        n, length, gap, at = rng.integers(1, 6), rng.integers(1, 20), rng.integers(0, 30), 4 * rng.integers(0, 200)
+        t = buf[at:at + n * (length + gap) * size].view(dtype).view(n, length + gap)[:, :length]
+        first, count = 4 * rng.integers(0, 300), rng.integers(1, 60)
+        out = buf[first:first + 4 * count].view(torch.float32)
+        held = {int(t.data_ptr()) + int(v) * (length + gap) * size + b for v in range(n) for b in range(length * size)}
+        want = any(b in held for b in range(out.data_ptr(), out.data_ptr() + 4 * count))
+        assert block8._meets(out, t) == want
+    A = object.__new__(block8.Block8)
+    A._h, A.device = None, torch.device("cpu")
+    x = torch.zeros(6, 64)
+    assert A._out(None, (3, 64), torch.float32, x).shape == (3, 64)
+    assert A._out(x[3:], (3, 64), torch.float32, x[:3]) is not None
+    for out in (x[:3], x[2:5]):
+        with pytest.raises(ValueError, match="shares memory"):
+            A._out(out, (3, 64), torch.float32, x[:3])
+    scale = torch.zeros(2, 3, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="shares memory"):
+        A._out(x[3:], (3, 64), torch.float32, x[:3], x.view(torch.uint8)[5:6, 8:11])
+    assert not block8._meets(x[3:], scale) and not block8._meets(x[:0], x) and not block8._meets(x, x[:0])
