@@ -228,6 +228,10 @@ class Block8(Matrix):
         self._here("out", out)
         if any(_meets(out, t) for t in operands):
             raise ValueError("out shares memory with an operand, which is still read while it is written")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out requires grad, and results written into it have no history")
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)      # for passes that saved it
         return out
 
     def set_values(self, values: torch.Tensor) -> None:

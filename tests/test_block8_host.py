@@ -190,3 +190,21 @@ def test_a_result_on_top_of_an_operand_is_refused():
     with pytest.raises(ValueError, match="shares memory"):
         A._out(x[3:], (3, 64), torch.float32, x[:3], x.view(torch.uint8)[5:6, 8:11])
     assert not block8._meets(x[3:], scale) and not block8._meets(x[:0], x) and not block8._meets(x, x[:0])
+
+
+def test_out_counts_as_changed_in_place():
+    """a backward pass that saved the tensor has to notice"""
+    A = object.__new__(block8.Block8)
+    A._h, A.device = None, torch.device("cpu")
+    x, out, w = torch.zeros(3, 64), torch.ones(3, 64), torch.ones(3, 64, requires_grad=True)
+    loss = (out * w).sum()
+    assert A._out(out, (3, 64), torch.float32, x) is out
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(ValueError, match="requires grad"):
+        A._out(w, (3, 64), torch.float32, x)
+    with torch.no_grad():
+        assert A._out(w, (3, 64), torch.float32, x) is w
+    with torch.inference_mode():
+        out = torch.ones(3, 64)
+        assert A._out(out, (3, 64), torch.float32, x) is out
