@@ -184,6 +184,16 @@ def _whole(name: str, a) -> np.ndarray:
     return whole
 
 
+def _inside(n: int, size: int, rows: int, nblocks: int, cus: int) -> bool:
+    """Are n vectors rounded inside the product, by every workgroup again, or by a call to quantize before?  Inside where that
+    costs less (bf16, 1920 blocks: 16 vectors 11 us inside, 17 before; 32 vectors 26 and 17 us; 4096 blocks, 16 vectors 17
+    and 17 us), and more than 64 vectors only where the library takes those in 8 bits by the same kernel (tiles of 64 for an
+    eighth of the CUs): the same bits either way."""
+    if n > 64 and (n > MAX_WIDE or -(-rows // BLOCK) * -(-n // 64) * 8 > cus):
+        return False
+    return nblocks * (-(-n // 16) * size) < (8500 if n <= 16 else 7500)
+
+
 class Block8(Matrix):
     """A handle of 8-bit blocks on the current device.  block_ptr [ceil(rows / 128) + 1] and block_col are host integers
     like the row_ptr and col of a CSR matrix, in units of blocks."""
@@ -198,6 +208,7 @@ class Block8(Matrix):
         self.rows, self.columns, self.nblocks = rows, columns, len(col)
         self._index = torch.cuda.current_device()
         self.device = torch.device("cuda", self._index)
+        self._cus = torch.cuda.get_device_properties(self._index).multi_processor_count
         self.values = None               # the tensor set_values last took: the leaf that linear() differentiates
         self._version = 0                # set_values / load calls so far
 
@@ -267,12 +278,8 @@ class Block8(Matrix):
             rows = _wide("x", x, self.columns)
             self._here("x", rows)
             shape = (*x.shape[:-1], self.rows)
-            # Rounded inside the product, by every workgroup again, where that costs less than a call to quantize (bf16,
-            # 1920 blocks: 16 vectors 11 us inside, 17 before; 32 vectors 26 and 17 us; 4096 blocks, 16 vectors 17 and 17 us)
-            # More than 64 vectors only where those in 8 bits go by the same kernel (32 tiles of 64): the same bits either way.
             n = rows.shape[0]
-            if (n <= 64 or n <= MAX_WIDE and -(-self.rows // BLOCK) * -(-n // 64) <= 32) and \
-                    self.nblocks * (-(-n // 16) * rows.element_size()) < (8500 if n <= 16 else 7500):
+            if _inside(n, rows.element_size(), self.rows, self.nblocks, self._cus):
                 y = self._out(out, shape, dtype or rows.dtype, rows)
                 L.check(L.lib().spmv_hip_block8_mult_dev(self._h, n, rows.data_ptr(), _DTYPE[rows.dtype], _ld(rows),
                                                          None, 0, y.data_ptr(), _DTYPE[y.dtype], self.rows, _stream(self._index)))

@@ -208,3 +208,16 @@ def test_out_counts_as_changed_in_place():
     with torch.inference_mode():
         out = torch.ones(3, 64)
         assert A._out(out, (3, 64), torch.float32, x) is out
+
+
+def test_rounding_inside_the_product_follows_the_devices_cus():
+    """more than 64 vectors inside only where the library takes their 8-bit form by the same kernel: block rows times tiles of
+    64 vectors at most an eighth of the CUs (spmv_hip_block8_mult_dev)"""
+    for cus in (256, 128, 64, 32):
+        for rows in (1, 128, 300, 2000, 4096):
+            for n in (1, 16, 64, 65, 128, 300, 1024, 1025):
+                same = n <= 64 or -(-rows // 128) * -(-n // 64) * 8 <= cus
+                assert block8._inside(n, 2, rows, 1, cus) == (same and n <= 1024)
+    assert not block8._inside(65, 2, 128, 1, 15) and block8._inside(64, 2, 128, 1, 15)
+    assert block8._inside(16, 2, 128, 4249, 256) and not block8._inside(16, 2, 128, 4250, 256)
+    assert block8._inside(32, 4, 128, 937, 256) and not block8._inside(32, 4, 128, 938, 256)

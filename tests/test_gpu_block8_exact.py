@@ -231,3 +231,17 @@ def test_negated_views():
     _equal(c.A.product(x.float()), -torch.mm(x, c.dense.t().contiguous()))
     with pytest.raises(ValueError, match="out must be"):
         c.A.product(x.float(), out=torch._neg_view(torch.zeros(3, 200, device=DEV)))
+
+
+# ---- which kernel ---------------------------------------------------------------------------------------------------
+
+def test_wide_and_packed_vectors_change_kernels_together():
+    """bf16 results on both sides of the border between the kernels, an eighth of the CUs in tiles of 64 vectors"""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    for brows in (1, 2, 5):
+        c = Whole(128 * brows - 3, 300, 1.0, brows)
+        c.A.set_values(torch.randn(c.values.shape, device=DEV))
+        tiles = cus // 8 // brows
+        for n in (64, 65, 64 * tiles, 64 * tiles + 1):
+            x = torch.randn(n, 300, device=DEV).to(BF16)
+            assert torch.equal(c.A.product(x), c.A.product(quantize(x))), (brows, n)
