@@ -273,7 +273,11 @@ class Block8(Matrix):
 
     def product(self, x, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """y[..., rows] = A x for the vectors of x: a tensor [..., columns] (rounded to 8 bits on the way in) or a
-        Packed8.  `dtype` of y: that of x unless given."""
+        Packed8.  `dtype` of y: that of x unless given.  y has no history (linear has).
+
+        Sums are 32 bits wide, with one exception: bfloat16 results of more than 64 vectors come from the 8-bit matrix
+        instruction, at twice the rate, and may be off by 7 * 2^-13 of the sum of the terms' magnitudes before they are
+        rounded, so that a vector's last bits depend on how many others come with it.  dtype=torch.float32 avoids that."""
         if not isinstance(x, Packed8):
             rows = _wide("x", x, self.columns)
             self._here("x", rows)
@@ -339,29 +343,30 @@ class Block8(Matrix):
             *((dv.data_ptr(), _DTYPE[dv.dtype]) if dv is not None else (None, 0)), accumulate,
             work.data_ptr() if work is not None else None, _stream(self._index)))
 
-    def linear(self, x: torch.Tensor) -> torch.Tensor:
-        """y = A x, differentiable in x and in the tensor that set_values took.  Between the passes x is kept in 8 bits;
-        the backward pass refuses a matrix whose values were set again meanwhile.  Forward-mode differentiation is refused."""
+    def linear(self, x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """y = A x, differentiable in x and in the tensor that set_values took.  `dtype` of y as in product: float32 for sums of
+        32 bits whatever the number of vectors.  Between the passes x is kept in 8 bits; the backward pass refuses a matrix
+        whose values were set again meanwhile.  Forward-mode differentiation is refused."""
         if not isinstance(x, torch.Tensor):
             raise TypeError("x must be a tensor")
         for t in (x, self.values):
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError("linear has no forward-mode derivative")
         if torch.is_grad_enabled() and (x.requires_grad or self.values is not None and self.values.requires_grad):
-            return _Linear.apply(x, self.values, self)
-        return self.product(x)
+            return _Linear.apply(x, self.values, self, dtype)
+        return self.product(x, dtype)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, values, matrix):
+    def forward(ctx, x, values, matrix, dtype):
         rows = _wide("x", x, matrix.columns)
         matrix._here("x", rows)
         q = _rounded(rows, x.shape)
         ctx.save_for_backward(q.values, q.scale)
         ctx.matrix, ctx.version, ctx.x_shape, ctx.x_dtype = matrix, matrix._version, x.shape, x.dtype
         ctx.values_dtype = values.dtype if values is not None else None
-        return matrix.product(q)
+        return matrix.product(q, dtype)
 
     @staticmethod
     @once_differentiable
@@ -376,4 +381,4 @@ class _Linear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             dv = d.new_empty((matrix.nblocks, BLOCK, BLOCK), dtype=ctx.values_dtype)
         matrix._backward(d, Packed8._made(values8, scale, matrix.columns, ctx.x_dtype, ctx.x_shape), dx, dv, False)
-        return dx, dv, None
+        return dx, dv, None, None

@@ -245,3 +245,23 @@ def test_wide_and_packed_vectors_change_kernels_together():
         for n in (64, 65, 64 * tiles, 64 * tiles + 1):
             x = torch.randn(n, 300, device=DEV).to(BF16)
             assert torch.equal(c.A.product(x), c.A.product(quantize(x))), (brows, n)
+
+
+@pytest.mark.parametrize("n", [5, 90, 700])
+def test_linear_in_32_bits(n):
+    """bf16 vectors into fp32 results: 32-bit sums for any number of them, where the 8-bit instruction would lose the 2^-13 beside 1 - 1"""
+    A = Block8.full(128, 128)
+    w = torch.ones(1, 128, 128, device=DEV, requires_grad=True)
+    A.set_values(w)
+    x = torch.zeros(n, 128, dtype=BF16, device=DEV)
+    x[:, 0::8], x[:, 1::8], x[:, 2::8] = 1.0, -1.0, 2.0 ** -16
+    x.requires_grad_(True)
+    y = A.linear(x, F32)
+    assert y.dtype == F32 and bool((y == 16 * 2.0 ** -16).all())
+    with torch.no_grad():
+        assert torch.equal(A.linear(x, F32), y)
+    dy = _whole(1, n, 128).float()
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert dx.dtype == BF16 and dw.dtype == F32
+    assert torch.equal(dx, A.product_t(dy, BF16)) and torch.equal(dw, A.gradient(dy, quantize(x)))
+    assert A.linear(x).dtype == BF16
