@@ -265,3 +265,120 @@ def test_linear_in_32_bits(n):
     assert dx.dtype == BF16 and dw.dtype == F32
     assert torch.equal(dx, A.product_t(dy, BF16)) and torch.equal(dw, A.gradient(dy, quantize(x)))
     assert A.linear(x).dtype == BF16
+
+
+# ---- no term lost ---------------------------------------------------------------------------------------------------
+
+# rows, columns, share of blocks, vectors: a block and less, ragged edges, 16 waves a row, more block rows than CUs / 8 in every tile size,
+# pairs of blocks, cut sums
+SHAPES = [(1, 1, 1.0, [1, 33, 70]), (129, 127, 1.0, [1, 17, 64, 65, 128, 515]), (700, 2300, 1.0, [1, 13, 31, 64, 200]), (2000, 1500, 0.5, [3, 33, 130, 777]),
+          (4200, 500, 0.7, [40, 1000, 2050]), (500, 4200, 0.7, [16, 700, 2900]), (4100, 4100, 0.6, [5, 64, 333, 1500]), (5200, 200, 0.8, [5, 130, 4000])]
+
+
+@pytest.mark.parametrize("rows,columns,keep,counts", SHAPES)
+def test_whole_numbers_through_every_product(rows, columns, keep, counts):
+    """at most 4: sums stay below fp16's largest number too; rounding the exact sum is all that is left"""
+    c = Whole(rows, columns, keep, rows + columns)
+    c.values = c.values.sign() * (c.values.abs() % 4 + 1)
+    c.A.set_values(c.values.float())
+    c.dense = torch.from_numpy(O.dense(c.values.cpu().numpy(), c.ptr, c.col, rows, columns)).to(DEV)
+    for n in counts:
+        x, dy = _whole(n, n, columns, top=4), _whole(n + 1, n, rows, top=4)
+        want_y, want_dx, want_dv = torch.mm(x, c.dense.t().contiguous()), torch.mm(dy, c.dense), c.sampled(torch.mm(dy.t().contiguous(), x))
+        for dtype in TYPES:
+            xt, dt = x.to(dtype), dy.to(dtype)
+            q = quantize(xt)
+            _equal(q.restore(), x)
+            for y_dtype in TYPES:
+                want = want_y.to(y_dtype).double()
+                _equal(c.A.product(xt, y_dtype), want, n, dtype, y_dtype)
+                _equal(c.A.product(q, y_dtype), want, n, dtype, y_dtype)
+            for to in (F32, dtype):
+                _equal(c.A.product_t(dt, to), want_dx.to(to).double(), n, dtype, to)
+                _equal(c.A.gradient(dt, q, to), want_dv.to(to).double(), n, dtype, to)
+
+
+def _full_mantissas(dtype, seed, *shape):
+    """numbers whose last mantissa bit is set, so that every bf16 part of them is needed"""
+    bits = {F32: 23, F16: 10, BF16: 7}[dtype]
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    m = torch.randint(0, 1 << (bits - 1), shape, generator=g, device=DEV).double() * 2 + 1 + 2.0 ** bits
+    e = torch.randint(-4, 5, shape, generator=g, device=DEV).double()
+    sign = torch.randint(0, 2, shape, generator=g, device=DEV).double() * 2 - 1
+    a = (sign * m * torch.exp2(e - bits)).to(dtype)
+    assert bool((a.double() == sign * m * torch.exp2(e - bits)).all())
+    return a
+
+
+def _powers(seed, *shape):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    e = torch.randint(-3, 4, shape, generator=g, device=DEV).double()
+    return torch.exp2(e) * (torch.randint(0, 2, shape, generator=g, device=DEV).double() * 2 - 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,columns,keep,counts", [(129, 127, 1.0, [1, 31, 32, 33, 128, 2000]), (300, 260, 0.9, [32, 64, 95, 128, 2000]), (2001, 1500, 0.6, [33, 256, 2000]),
+                                                      (4200, 4200, 0.7, [32, 70, 1000]), (5200, 200, 0.8, [5, 40, 130]), (500, 4200, 0.7, [64, 1500])])
+def test_every_bit_of_dy_reaches_both_gradients(rows, columns, keep, counts, dtype):
+    """one entry of dy to a sum, times a power of two: the product is the sum, and needs all of dy's bits.  (The tolerance of K
+    additions hides the last part of an fp32 entry, 2^-16 of it, from K = 33 on.)"""
+    c = Whole(rows, columns, keep, rows)
+    values = _powers(1, len(c.col), 128, 128)
+    c.A.set_values(values.float())
+    dense = torch.from_numpy(O.dense(values.cpu().numpy(), c.ptr, c.col, rows, columns)).to(DEV)
+    for n in counts:
+        for seed in (1, 2):
+            g = torch.Generator(device=DEV).manual_seed(seed + n)
+            # the gradient: every row of A has its one vector
+            dy, at = torch.zeros(n, rows, dtype=dtype, device=DEV), torch.randint(0, n, (rows,), generator=g, device=DEV)
+            dy[at, torch.arange(rows, device=DEV)] = _full_mantissas(dtype, seed, rows)
+            x = _powers(seed + 1, n, columns)
+            want = c.sampled(torch.mm(dy.double().t().contiguous(), x))
+            _equal(c.A.gradient(dy, quantize(x.float())), want, n, seed)
+            # dx: every vector has its one row
+            dy, at = torch.zeros(n, rows, dtype=dtype, device=DEV), torch.randint(0, rows, (n,), generator=g, device=DEV)
+            dy[torch.arange(n, device=DEV), at] = _full_mantissas(dtype, seed, n)
+            _equal(c.A.product_t(dy, F32), torch.mm(dy.double(), dense), n, seed)
+
+
+def test_no_term_is_lost_past_32_bit_offsets():
+    """a matrix of 2.2 GB and blocks of vectors past 2 GB, in whole numbers: sums of 47360 products of at most 64"""
+    k = 370
+    g = torch.Generator(device=DEV).manual_seed(1)
+
+    def whole(*shape):
+        a = torch.randint(-8, 9, shape, generator=g, device=DEV, dtype=torch.int8)
+        return a
+
+    A = Block8.full(128 * k, 128 * k)
+    v = whole(A.nblocks, 128, 128)
+    codes = torch.arange(-8, 9, device=DEV).float().to(torch.float8_e4m3fn).view(torch.uint8)
+    v8 = torch.empty(v.shape, dtype=torch.uint8, device=DEV)
+    for at in range(0, A.nblocks, 10000):
+        v8[at:at + 10000] = codes[v[at:at + 10000].int() + 8]
+    A.load(v8, torch.full((A.nblocks,), 127, dtype=torch.uint8, device=DEV))
+    del v8
+    rows = lambda i: v[i * k:(i + 1) * k].double().permute(1, 0, 2).reshape(128, -1)
+    cols = lambda j: v[j::k].double().reshape(-1, 128)
+    n = 46000
+    x, dy = whole(n, 128 * k).to(BF16), whole(n, 128 * k).to(BF16)
+    x[:, ::128] = 8                                          # the scale of every group: all its whole numbers are exact
+    q = quantize(x)
+    part = {200: quantize(x[-200:]), 3: quantize(x[-3:])}
+    y = A.product(q)
+    for i in (0, k // 2, k - 1):
+        at = slice(128 * i, 128 * (i + 1))
+        r, c = rows(i).t().contiguous(), cols(i)
+        for m, p in part.items():
+            _equal(A.product(p, F32)[:, at], torch.mm(x[-m:].double(), r), "product", i, m)
+        dx = A.product_t(dy)
+        for t in (slice(0, 300), slice(n - 300, n)):
+            _equal(y[t, at], torch.mm(x[t].double(), r).to(BF16).double(), "product", i, t)
+            _equal(dx[t, at], torch.mm(dy[t].double(), c).to(BF16).double(), "product_t", i, t)
+        _equal(A.product_t(dy[-3:], F32)[:, at], torch.mm(dy[-3:].double(), c), "product_t", i)
+        del dx
+    del y
+    dv = A.gradient(dy, q, BF16)
+    for i, j in ((0, 0), (0, k - 1), (k // 2, 7), (k - 1, 0), (k - 1, k - 1)):
+        a, b = dy[:, 128 * i:128 * (i + 1)].double().t().contiguous(), x[:, 128 * j:128 * (j + 1)].double().contiguous()
+        _equal(dv[i * k + j], torch.mm(a, b).to(BF16).double(), "gradient", i, j)
