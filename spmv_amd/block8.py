@@ -218,6 +218,15 @@ class Block8(Matrix):
         brows, bcols = -(-rows // BLOCK), -(-columns // BLOCK)
         return cls(rows, columns, np.arange(brows + 1) * bcols, np.tile(np.arange(bcols), brows))
 
+    def download(self, which: int) -> np.ndarray:
+        """The pattern (ARR_ROW_PTR: block_ptr, ARR_COL: block_col); store has the values."""
+        size = {L.ARR_ROW_PTR: -(-self.rows // BLOCK) + 1, L.ARR_COL: self.nblocks}.get(which)
+        if size is None:
+            return super().download(which)       # refused there
+        out = np.empty(size, np.int32)
+        L.check(L.lib().spmv_hip_download(self._h, which, out.ctypes.data, out.nbytes))
+        return out
+
     def _here(self, name: str, t: torch.Tensor) -> None:
         if t.device != self.device:
             raise ValueError(f"{name} is on {t.device}, the matrix on {self.device}")

@@ -382,3 +382,13 @@ def test_no_term_is_lost_past_32_bit_offsets():
     for i, j in ((0, 0), (0, k - 1), (k // 2, 7), (k - 1, 0), (k - 1, k - 1)):
         a, b = dy[:, 128 * i:128 * (i + 1)].double().t().contiguous(), x[:, 128 * j:128 * (j + 1)].double().contiguous()
         _equal(dv[i * k + j], torch.mm(a, b).to(BF16).double(), "gradient", i, j)
+
+
+def test_download_gives_the_pattern():
+    c = Whole(700, 520, 0.6, 3)
+    assert np.array_equal(c.A.download(S.ARR_ROW_PTR), c.ptr) and np.array_equal(c.A.download(S.ARR_COL), c.col)
+    for which in (S.ARR_VAL, S.ARR_SLICE_PTR, S.ARR_ROW_ORDER, S.ARR_TILE_COORD):
+        with pytest.raises(S.SpmvHipError, match="not part of format"):
+            c.A.download(which)
+    empty = Block8(300, 200, [0, 0, 0, 0], [])
+    assert np.array_equal(empty.download(S.ARR_ROW_PTR), np.zeros(4)) and empty.download(S.ARR_COL).shape == (0,)
