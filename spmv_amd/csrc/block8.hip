@@ -532,21 +532,27 @@ template <bool ASM> __device__ __forceinline__ void load_to_lds(u32x4 r, unsigne
             (__attribute__((address_space(3))) void *)to, 16, (int)offset, 0, 0, 0);
 }
 
-// step(slot, k) for k = first .. last - 1, slot = (k - first) % R as a constant: whole rounds, then what is left (exits
-// from inside a round would cost the accumulators copies)
+// step(slot, k, behind) for k = first .. last - 1, slot = (k - first) % R as a constant: whole rounds, then what is left (exits
+// from inside a round would cost the accumulators copies).  `behind`: how many stages have been issued behind stage k when
+// the step begins, so that its wait may leave their loads outstanding.  A step of a whole round issues stage k + R - 1;
+// the last ones, `behind` = TAIL + that number, issue nothing: all stages are under way, and loads that nothing uses any more
+// would be dropped by the compiler while the wait went on counting them.
+constexpr int TAIL = 100;
 template <int R, typename F> __device__ __forceinline__ void ring(int first, int last, F step)
 {
     int k = first;
     for (; k + R <= last; k += R) {
-        step(ic<0>(), k);
-        step(ic<1>(), k + 1);
-        if constexpr (R > 2) step(ic<2>(), k + 2);
-        if constexpr (R > 3) step(ic<3>(), k + 3);
+        step(ic<0>(), k, ic<R - 2>());
+        step(ic<1>(), k + 1, ic<R - 2>());
+        if constexpr (R > 2) step(ic<2>(), k + 2, ic<R - 2>());
+        if constexpr (R > 3) step(ic<3>(), k + 3, ic<R - 2>());
     }
-    if (k < last) step(ic<0>(), k);
-    if constexpr (R > 2) if (k + 1 < last) step(ic<1>(), k + 1);
-    if constexpr (R > 3) if (k + 2 < last) step(ic<2>(), k + 2);
+    if (k < last) step(ic<0>(), k, ic<TAIL + R - 2>());
+    if constexpr (R > 2) if (k + 1 < last) step(ic<1>(), k + 1, ic<TAIL + R - 3>());
+    if constexpr (R > 3) if (k + 2 < last) step(ic<2>(), k + 2, ic<TAIL + R - 4>());
 }
+// Keeps the memory accesses before it before those behind it: a wait counts the loads of whole stages, in their order
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 // G = 2 groups of four waves share a tile whose workgroup has a CU to itself, each with half of the sum and its own stages: one
 // group's loads and LDS reads run beside the other's matrix instructions.  Every barrier is the whole workgroup's, so
@@ -671,11 +677,12 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
         __builtin_memcpy(&sx[S], g.xscale + (int64_t)c * g.lds + (v0 - back), NU);
         look_up(min(b + 1, last - 1));
     };
-    auto step = [&](auto slot, int b) {
-        constexpr int S = decltype(slot)::value;
+    auto step = [&](auto slot, int b, auto behind) {
+        constexpr int S = decltype(slot)::value, BEHIND = decltype(behind)::value;
+        constexpr bool MORE = BEHIND < TAIL;
         here(c);
         here(scale);
-        stage_barrier<(R - 2) * (NU + 8)>();
+        stage_barrier<BEHIND % TAIL * (NU + 8)>();
         auto operand = [&](int u) {
             const uint8_t *row = &X[S][(wn * 16 * NU + NU * i + u) * kB];
             return join(*(const u32x4 *)(row + ((q ^ (i & 7)) << 4)), *(const u32x4 *)(row + (((q + 4) ^ (i & 7)) << 4)));
@@ -684,10 +691,10 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
         // one tile ahead and no more: left alone, the compiler reads all of them first and runs out of registers.
         constexpr int AHEAD = NU == 8 || EXACT ? 1 : NU;
         i32x8 w[NU];
-        if constexpr (NU == 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
+        if constexpr (MORE && NU == 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) w[u] = operand(u);
-        if constexpr (NU < 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
+        if constexpr (MORE && NU < 8) issue(ic<(S + R - 1) % R>(), min(b + R - 1, last - 1));
         // for widening those of half the scales; past the last vector, in the upper bytes, whatever it is
         const uint64_t bytes = (sx[S] >> (8 * min(back, 7))) - (EXACT ? 0x0101010101010101u : 0);
         bf16x8 aw[4][EXACT ? 4 : 1];
@@ -723,7 +730,9 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
     if (first < last) {
         look_up(first);
         issue(ic<0>(), first);
+        in_order();
         if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
+        in_order();
         if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
         ring<R>(first, last, step);
     }
@@ -954,13 +963,13 @@ __global__ __launch_bounds__(G *kBlock, 2) void transposed_kernel(TransposedArgs
             }
         }
     };
-    auto step = [&](auto slot, int k) {
-        constexpr int S = decltype(slot)::value;
+    auto step = [&](auto slot, int k, auto behind) {
+        constexpr int S = decltype(slot)::value, BEHIND = decltype(behind)::value;
         here(id);
         here(row);
         here(scale);
-        stage_barrier<(R - 2) * (2 + PARTS * NU)>();
-        compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
+        stage_barrier<BEHIND % TAIL * (2 + PARTS * NU)>();
+        compute(slot, [&] { if constexpr (BEHIND < TAIL) issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
     };
     if (first < last) {
         look_up(first);
@@ -1140,10 +1149,10 @@ __global__ __launch_bounds__(G *kBlock, 2) void gradient_kernel(GradientArgs g, 
         issue(ic<0>(), first);
         if constexpr (R > 2) issue(ic<1>(), min(first + 1, last - 1));
         if constexpr (R > 3) issue(ic<2>(), min(first + 2, last - 1));
-        ring<R>(first, last, [&](auto slot, int k) {
-            constexpr int S = decltype(slot)::value;
-            stage_barrier<(R - 2) * (9 + 2 * PARTS)>();
-            compute(slot, [&] { issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
+        ring<R>(first, last, [&](auto slot, int k, auto behind) {
+            constexpr int S = decltype(slot)::value, BEHIND = decltype(behind)::value;
+            stage_barrier<BEHIND % TAIL * (9 + 2 * PARTS)>();
+            compute(slot, [&] { if constexpr (BEHIND < TAIL) issue(ic<(S + R - 1) % R>(), min(k + R - 1, last - 1)); });
         });
     }
     for (int k = last - first; k < rounds; k++) stage_barrier<0>();      // as many as the other group

@@ -392,3 +392,52 @@ def test_download_gives_the_pattern():
             c.A.download(which)
     empty = Block8(300, 200, [0, 0, 0, 0], [])
     assert np.array_equal(empty.download(S.ARR_ROW_PTR), np.zeros(4)) and empty.download(S.ARR_COL).shape == (0,)
+
+
+# ---- the pipelines' ends --------------------------------------------------------------------------------------------
+
+def _rows_of(lengths, bcols, seed):
+    """a pattern whose block rows hold `lengths` blocks"""
+    rng = np.random.default_rng(seed)
+    col = [sorted(rng.permutation(bcols)[:k]) for k in lengths]
+    return np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32), np.concatenate(col).astype(np.int32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [130, 1000, 2100, 4103])
+def test_block_rows_and_columns_of_every_length_give_the_same_bits(n, dtype):
+    """1 to 13 blocks: whole rounds of 2, 3 or 4 stages and every number of steps after them, in tiles of 64, 128 and 256 vectors;
+    a stage read before its loads have arrived is wrong now and then, so every product is repeated"""
+    lengths = [5, 1, 2, 3, 4, 5, 0, 6, 7, 8, 9, 10, 11, 12, 13, 5, 8]
+    for turned in (False, True):
+        ptr, col = _rows_of(lengths, 16, n)
+        rows, columns = 128 * len(lengths) - 70, 16 * 128 - 30
+        if turned:                                           # the lengths are those of block columns
+            place = sorted((c, r) for r in range(len(lengths)) for c in col[ptr[r]:ptr[r + 1]])
+            rows, columns = columns, rows
+            ptr = np.array([sum(1 for p in place if p[0] < r) for r in range(17)], np.int32)
+            col = np.array([p[1] for p in place], np.int32)
+        values = _whole(n, len(col), 128, 128, top=4)
+        A = Block8(rows, columns, ptr, col)
+        A.set_values(values.float())
+        a = torch.from_numpy(O.dense(values.cpu().numpy(), ptr, col, rows, columns)).to(DEV)
+        x, dy = _whole(n, n, columns, top=4), _whole(n + 1, n, rows, top=4)
+        q, d = quantize(x.to(dtype)), dy.to(dtype)
+        y, dx = torch.mm(x, a.t().contiguous()), torch.mm(dy, a)
+        for k in range(20):
+            for to in TYPES:
+                _equal(A.product(q, to), y.to(to).double(), to, k)
+            _equal(A.product_t(d, dtype), dx.to(dtype).double(), k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,columns", [(128, 128), (1300, 1300), (2600, 2600), (4200, 4200)])
+def test_gradients_of_every_number_of_vectors_give_the_same_bits(rows, columns, dtype):
+    """1 to 9 steps of 32 vectors and what is left, single blocks and pairs"""
+    c = Whole(rows, columns, 0.7 if rows > 2600 else 1.0, rows)
+    for n in [32 * k + r for k in range(1, 10) for r in (0, 5)]:
+        x, dy = _whole(n, n, columns), _whole(n + 1, n, rows)
+        q, d = quantize(x.to(dtype)), dy.to(dtype)
+        want = c.sampled(torch.mm(dy.t().contiguous(), x))
+        for k in range(4):
+            _equal(c.A.gradient(d, q), want, n, k)
