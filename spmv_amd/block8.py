@@ -37,9 +37,17 @@ _DTYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
+def _dual_level() -> int:
+    """negative outside of forward-mode differentiation"""
+    return getattr(forward_ad, "_current_level", 0)
+
+
 def _stream(index: int) -> int:
     """The stream of a call.  torch.jit.trace would record the tensors made for the results, and not the calls that fill them."""
-    if torch.jit.is_tracing():
+    if _tracing():
         raise RuntimeError("products with 8-bit blocks cannot be traced by torch.jit")
     return _raw_stream(index)
 
@@ -135,9 +143,12 @@ class Packed8:
         q._fill(values, scale, columns, dtype, shape)
         return q
 
-    def _fill(self, *fields) -> None:
-        for put, value in zip(_PUT, fields):
-            put(self, value)
+    def _fill(self, values, scale, columns, dtype, shape) -> None:
+        _put_values(self, values)
+        _put_scale(self, scale)
+        _put_columns(self, columns)
+        _put_dtype(self, dtype)
+        _put_shape(self, shape)
 
     @property
     def n(self) -> int:
@@ -155,7 +166,7 @@ class Packed8:
         return x
 
 
-_PUT = tuple(getattr(Packed8, name).__set__ for name in Packed8.__slots__)
+_put_values, _put_scale, _put_columns, _put_dtype, _put_shape = (getattr(Packed8, name).__set__ for name in Packed8.__slots__)
 
 
 def _rounded(rows: torch.Tensor, shape) -> Packed8:
@@ -358,9 +369,10 @@ class Block8(Matrix):
         whose values were set again meanwhile.  Forward-mode differentiation is refused."""
         if not isinstance(x, torch.Tensor):
             raise TypeError("x must be a tensor")
-        for t in (x, self.values):
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("linear has no forward-mode derivative")
+        if _dual_level() >= 0:
+            for t in (x, self.values):
+                if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                    raise NotImplementedError("linear has no forward-mode derivative")
         if torch.is_grad_enabled() and (x.requires_grad or self.values is not None and self.values.requires_grad):
             return _Linear.apply(x, self.values, self, dtype)
         return self.product(x, dtype)
