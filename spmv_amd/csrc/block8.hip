@@ -652,7 +652,7 @@ __global__ __launch_bounds__(G *kBlock, 2) void product_kernel(ProductArgs g, OT
     const uint8_t *xbase = g.x8 + (int64_t)t0 * g.ldx8;
     const unsigned ldx8 = (unsigned)g.ldx8, records = (unsigned)min(g.n - t0, TOK) * ldx8;
     const u32x4 xs = buffer(xbase, records);
-    const int back = max(v0 + NU - g.n, 0);                  // n > NU, so the load of scale bytes can move back from the end
+    const int back = max(v0 - g.n + NU, 0);                  // n > NU, so the load of scale bytes can move back from the end
 
     i32x8 a[R][4];
     uint64_t sx[R];
@@ -1224,7 +1224,17 @@ static int launched(const char *what)
     return 1;
 }
 
+// groups of `per` vectors; n may be the largest int
+static int tiles_of(int n, int per) { return (int)(((int64_t)n + per - 1) / per); }
 static int groups_of(int length) { return length / kB + (length % kB != 0); }
+
+// a launch has fewer than 2^32 threads along x
+static int check_launch(const char *what, int64_t workgroups, int threads)
+{
+    if (workgroups <= 0xffffffffll / threads) return 0;
+    set_error("%s: %lld workgroups of %d threads are more than one launch takes", what, (long long)workgroups, threads);
+    return 1;
+}
 
 static int launch_few(const spmv_hip_matrix *m, int n, const void *x, int x_dtype, int64_t ldx, const uint8_t *xscale,
                       int64_t lds, void *y, int y_dtype, int64_t ldy, hipStream_t st)
@@ -1232,10 +1242,11 @@ static int launch_few(const spmv_hip_matrix *m, int n, const void *x, int x_dtyp
     // 16 waves a workgroup where every one of them gets a block, else 4; two strips a workgroup where that leaves workgroups
     // for two CUs in three (8 bits, 64 vectors: 8192 x 8192 37.7 us with one, 22.3 with two; 4096 x 4096 11.1 and 12.4)
     const bool many_waves = m->nblocks >= 16 * (int64_t)m->brows, pairs = m->brows * (int64_t)6 >= m->cus;
+    if (check_launch("block8_mult", m->brows * (int64_t)(pairs ? 4 : 8), (many_waves ? 16 : 4) * kWave)) return 1;
     auto go = [&](auto t) {
         typedef decltype(t) XT;
         auto launch = [&](auto kernel, int waves, int strips) {
-            hipLaunchKernelGGL(kernel, dim3(m->brows * (8 / strips), (n + 63) / 64), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
+            hipLaunchKernelGGL(kernel, dim3(m->brows * (8 / strips), tiles_of(n, 64)), dim3(waves * kWave), 0, st, n, m->rows, m->columns, m->d_block_ptr,
                                m->d_block_col, m->d_val8, m->d_scale8, (const XT *)x, ldx, xscale, lds, y, y_dtype, ldy);
         };
         auto tiles = [&](auto w, auto two) {
@@ -1258,8 +1269,8 @@ int launch_block8_f32(const spmv_hip_matrix *m, int n, const float *d_x, int64_t
                       hipStream_t stream)
 {
     if (m->rows == 0) return 0;
-    for (int v = 0; v < n; v += SPMV_HIP_BLOCK8_MAX_WIDE) {
-        const int k = n - v < SPMV_HIP_BLOCK8_MAX_WIDE ? n - v : (int)SPMV_HIP_BLOCK8_MAX_WIDE;
+    for (int64_t v = 0; v < n; v += SPMV_HIP_BLOCK8_MAX_WIDE) {
+        const int k = (int)std::min(n - v, (int64_t)SPMV_HIP_BLOCK8_MAX_WIDE);
         if (launch_few(m, k, d_x + v * ldx, SPMV_HIP_F32, ldx, nullptr, 0, d_y + v * ldy, SPMV_HIP_F32, ldy, stream)) return 1;
     }
     return 0;
@@ -1300,12 +1311,11 @@ static int check_block8(const char *what, const spmv_hip_matrix *m)
     if (m->format != SPMV_HIP_BLOCK8) { set_error("%s needs a handle of 8-bit blocks (format %d)", what, m->format); return 1; }
     return 0;
 }
-// launch shape of quantize8 / restore8; R vectors a wave
+// workgroups of quantize8 / restore8; R vectors a wave
 static bool many_groups(int n, int groups) { return (int64_t)(n / 16) * ((groups + kQuantGroups - 1) / kQuantGroups) >= 512; }
-static dim3 group_grid(int n, int groups, int r)
+static int64_t group_grid(int n, int groups, int r)
 {
-    const int64_t per = (int64_t)kQuantWaves * r;
-    return dim3((unsigned)((n + per - 1) / per * ((groups + kQuantGroups - 1) / kQuantGroups)));
+    return (int64_t)tiles_of(n, kQuantWaves * r) * ((groups + kQuantGroups - 1) / kQuantGroups);
 }
 
 // Tiles of 16 vectors a wave takes: `most` where that still makes `least` workgroups, else half, down to 2; 4 are enough with
@@ -1313,14 +1323,8 @@ static dim3 group_grid(int n, int groups, int r)
 static int vector_tiles(int majors, int n, int most, int least, int four)
 {
     int nu = most;
-    while (nu > 2 && (int64_t)majors * ((n + 32 * nu - 1) / (32 * nu)) < (nu == 4 ? four : least)) nu /= 2;
+    while (nu > 2 && (int64_t)majors * tiles_of(n, 32 * nu) < (nu == 4 ? four : least)) nu /= 2;
     return nu;
-}
-static int check_tiles(const char *what, int majors, int vtiles)
-{
-    if ((int64_t)majors * vtiles <= 0x7fffffff) return 0;
-    set_error("%s: %d x %d tiles are more than one launch takes", what, majors, vtiles);
-    return 1;
 }
 
 // How a backward call runs; `work` in bytes: the parts of dy, its copy for dx, then the slices of a cut sum
@@ -1366,7 +1370,7 @@ static BackwardPlan backward_plan(const spmv_hip_matrix *m, int n, const void *d
         // only with 1 1/2 workgroups a CU left (777 vectors: 30 us, 42 with 4; 3000: 66 us with 8, 77 with 2)
         p.tiles = p.dx_parts > 1 ? 2 : vector_tiles(m->bcols, n, 8, m->cus * 3 / 2, m->cus * 3 / 2);
         p.dx_slice = (int64_t)n * m->bcols * kB;
-        const int64_t tiles = (int64_t)m->bcols * ((n + 32 * p.tiles - 1) / (32 * p.tiles)), steps = 2 * (int64_t)m->longest;
+        const int64_t tiles = (int64_t)m->bcols * tiles_of(n, 32 * p.tiles), steps = 2 * (int64_t)m->longest;
         p.dx_slices = slices(tiles, steps, m->cus, 0.2f + 0.3f * p.dx_parts, p.dx_slice * 4);
         p.dx_halves = p.tiles == 2 && tiles * p.dx_slices <= m->cus && steps >= 4 * p.dx_slices;
     }
@@ -1525,13 +1529,16 @@ int spmv_hip_quantize8_dev(int n, int columns, const void *d_x, int dtype, int64
     if (check_vectors("quantize8", n, d_x, ldx, columns) || check_eight("quantize8", n, columns, d_x8, ldx8, d_scale, lds)) return 1;
     const int groups = groups_of(columns);
     if (n == 0 || groups == 0) return 0;
+    const bool many = many_groups(n, groups);
+    const int64_t grid = group_grid(n, groups, many ? 4 : 1);
+    if (check_launch("quantize8", grid, kBlock)) return 1;
     with_elem(dtype, [&](auto t) {
         typedef decltype(t) T;
-        auto go = [&](auto kernel, int r) {
-            hipLaunchKernelGGL(kernel, group_grid(n, groups, r), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, (const T *)d_x, ldx, d_x8, ldx8, d_scale, lds);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, (const T *)d_x, ldx, d_x8, ldx8, d_scale, lds);
         };
-        if (many_groups(n, groups)) go(quantize8_kernel<T, 4>, 4);
-        else go(quantize8_kernel<T, 1>, 1);
+        if (many) go(quantize8_kernel<T, 4>);
+        else go(quantize8_kernel<T, 1>);
     });
     return launched("quantize8");
 }
@@ -1544,15 +1551,17 @@ int spmv_hip_restore8_dev(int n, int columns, const uint8_t *d_x8, int64_t ldx8,
     if (check_vectors("restore8", n, d_x, ldx, columns) || check_eight("restore8", n, columns, d_x8, ldx8, d_scale, lds)) return 1;
     const int groups = groups_of(columns);
     if (n == 0 || groups == 0) return 0;
+    const int64_t grid = group_grid(n, groups, 2);
+    if (check_launch("restore8", grid, kBlock)) return 1;
     with_elem(dtype, [&](auto t) {
         typedef decltype(t) T;
-        auto go = [&](auto kernel, int r) {
-            hipLaunchKernelGGL(kernel, group_grid(n, groups, r), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, d_x8, ldx8, d_scale, lds, (T *)d_x, ldx);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kBlock), 0, (hipStream_t)stream, n, groups, columns, d_x8, ldx8, d_scale, lds, (T *)d_x, ldx);
         };
         // Past the caches where the 256 MB of the last one would not hold both sides (16384 x 8192 of bf16: 57 us, 67 through
         // them), but not below (30000 x 1000 of fp32: 36 us, 24 through them)
-        if ((int64_t)n * columns * (int64_t)(sizeof(T) + 1) > (int64_t)192 << 20) go(restore8_kernel<T, 2, true>, 2);
-        else go(restore8_kernel<T, 2, false>, 2);
+        if ((int64_t)n * columns * (int64_t)(sizeof(T) + 1) > (int64_t)192 << 20) go(restore8_kernel<T, 2, true>);
+        else go(restore8_kernel<T, 2, false>);
     });
     return launched("restore8");
 }
@@ -1580,7 +1589,7 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     if (!on.ok) return 1;
     // few vectors, or few tiles of many: there the strips, eight times as many, give the GPU more to do (fp32, 8192 x 1024, 128
     // vectors: 11 us, 21 in tiles; 32 tiles of 64 vectors 12 and 21 us, 64 tiles 22 and 22)
-    if (x_dtype != SPMV_HIP_E4M3 || n <= 64 || (int64_t)m->brows * ((n + 63) / 64) * 8 <= m->cus)
+    if (x_dtype != SPMV_HIP_E4M3 || n <= 64 || (int64_t)m->brows * tiles_of(n, 64) * 8 <= m->cus)
         return launch_few(m, n, d_x, x_dtype, ldx, d_scale, lds, d_y, y_dtype, ldy, (hipStream_t)stream);
     ProductArgs a{};
     a.n = n; a.rows = m->rows; a.brows = m->brows;
@@ -1588,9 +1597,9 @@ int spmv_hip_block8_mult_dev(const spmv_hip_matrix *m, int n, const void *d_x, i
     a.x8 = (const uint8_t *)d_x; a.xscale = d_scale; a.ldx8 = ldx; a.lds = lds; a.ldy = ldy;
     // With 4 tiles of vectors a wave, workgroups for every second CU are enough: they are two groups of waves then.
     const int nu = vector_tiles(m->brows, n, y_dtype == SPMV_HIP_BF16 ? 8 : 4, m->cus, m->cus / 2);
-    a.vtiles = (n + 32 * nu - 1) / (32 * nu);
-    if (check_tiles(what, m->brows, a.vtiles)) return 1;
+    a.vtiles = tiles_of(n, 32 * nu);
     const bool halves = nu < 8 && (int64_t)m->brows * a.vtiles <= m->cus && m->nblocks >= (int64_t)4 * m->brows;
+    if (check_launch(what, (int64_t)m->brows * a.vtiles, (halves ? 2 : 1) * kBlock)) return 1;
     with_elem(y_dtype, [&](auto t) {
         typedef decltype(t) T;
         constexpr bool exact = !std::is_same<T, __bf16>::value;
@@ -1648,9 +1657,10 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
     int64_t dx_ld = lddy, dv_ld = lddy, plane = 0;
     int dx_rows = m->rows, dv_rows = m->rows;
     if (plan.parts_bytes || plan.copy_bytes) {
-        const int padded = m->brows * kB;
-        plane = (int64_t)n * padded;
-        if (plane / 8 > (int64_t)0x7fffffff * kBlock || padded >= 1 << 23) { set_error("%s: %d vectors of %d are more than one launch takes", what, n, m->rows); return 1; }
+        const int64_t wide = m->brows * (int64_t)kB;
+        const int padded = (int)wide;
+        plane = n * wide;
+        if (wide >= 1 << 23 || (plane / 8 + kBlock - 1) / kBlock > 0xffffffffll / kBlock) { set_error("%s: %d vectors of %d are more than one launch takes", what, n, m->rows); return 1; }
         auto go = [&](auto kernel, auto *from, void *to) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)((plane / 8 + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, n, m->rows, padded, from, lddy, (__bf16 *)to, plane);
         };
@@ -1685,8 +1695,8 @@ int spmv_hip_block8_backward_dev(const spmv_hip_matrix *m, int n, const void *d_
         a.ptr = m->d_bt_ptr; a.row = m->d_bt_row; a.id = m->d_bt_id; a.val8 = m->d_val8; a.scale = m->d_bt_scale8;
         a.dy = dx_dy; a.lddy = dx_ld; a.plane = plane; a.slice = plan.dx_slice;
         const int nu = plan.tiles;
-        a.vtiles = (n + 32 * nu - 1) / (32 * nu);
-        if (check_tiles(what, m->bcols, a.vtiles)) return 1;
+        a.vtiles = tiles_of(n, 32 * nu);
+        if (check_launch(what, (int64_t)m->bcols * a.vtiles, (plan.dx_halves ? 2 : 1) * kBlock)) return 1;
         auto into = [&](auto *to, int64_t ld) {
             typedef std::remove_pointer_t<decltype(to)> O;
             a.lddx = ld;

@@ -221,3 +221,10 @@ def test_rounding_inside_the_product_follows_the_devices_cus():
     assert not block8._inside(65, 2, 128, 1, 15) and block8._inside(64, 2, 128, 1, 15)
     assert block8._inside(16, 2, 128, 4249, 256) and not block8._inside(16, 2, 128, 4250, 256)
     assert block8._inside(32, 4, 128, 937, 256) and not block8._inside(32, 4, 128, 938, 256)
+
+
+def test_more_than_one_launch_takes_is_refused():
+    """2^31 - 1 vectors of one entry: 2^27 workgroups of 256 threads"""
+    L, p, n = S.lib(), 4096, 2 ** 31 - 1
+    _fails(L.spmv_hip_quantize8_dev(n, 1, p, S.BF16, 1, p, 128, p, n, None), "more than one launch takes")
+    _fails(L.spmv_hip_restore8_dev(n, 1, p, 128, p, n, p, S.BF16, 1, None), "more than one launch takes")

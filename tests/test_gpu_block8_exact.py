@@ -441,3 +441,20 @@ def test_gradients_of_every_number_of_vectors_give_the_same_bits(rows, columns, 
         want = c.sampled(torch.mm(dy.t().contiguous(), x))
         for k in range(4):
             _equal(c.A.gradient(d, q), want, n, k)
+
+
+def test_the_largest_number_of_vectors():
+    """2^31 - 1: rounding their number up to whole tiles passes 32 bits"""
+    n = 2 ** 31 - 1
+    A = Block8(1, 0, [0, 0], [])                            # neither product here reads or writes past 2^31 - 1 vectors
+    q = Packed8(torch.empty(n, 0, dtype=torch.uint8, device=DEV), torch.empty(0, n, dtype=torch.uint8, device=DEV), 0, BF16)
+    y = torch.full((n, 1), float("nan"), dtype=BF16, device=DEV)
+    A.product(q, out=y)
+    assert int(torch.count_nonzero(y)) == 0
+    del y
+    A = Block8.full(8, 1)
+    A.set_values(torch.ones(1, 128, 128, device=DEV))
+    dy = torch.zeros(n, 8, dtype=BF16, device=DEV)
+    dy[0, 3], dy[n - 1, 7], dy[n - 1, 0], dy[2 ** 30, 5] = 1, 2, 3, 4
+    dx = A.product_t(dy)
+    assert int(torch.count_nonzero(dx)) == 3 and [float(dx[k, 0]) for k in (0, n - 1, 2 ** 30)] == [1, 5, 4]
