@@ -10,7 +10,7 @@ there, and is checked here before the library sees an address.
     y = A.product(x)                                  # the product alone
 
 Number format (include/spmv_hip.h has the definition): e4m3 values, one power-of-two scale per block of the matrix and per
-128 consecutive entries of a vector, kept as the byte b of 2^(b-127).  Gradients are those of the product with the
+128 consecutive entries of a vector, kept as the byte b of 2^(b-127), 1 to 247.  Gradients are those of the product with the
 rounded operands (the rounding itself counts as the identity).
 """
 from __future__ import annotations
@@ -366,7 +366,8 @@ class Block8(Matrix):
     def linear(self, x: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
         """y = A x, differentiable in x and in the tensor that set_values took.  `dtype` of y as in product: float32 for sums of
         32 bits whatever the number of vectors.  Between the passes x is kept in 8 bits; the backward pass refuses a matrix
-        whose values were set again meanwhile.  Forward-mode differentiation is refused."""
+        whose values were set again meanwhile (not by the replay of a graph, which is not seen here).  Forward-mode
+        differentiation is refused."""
         if not isinstance(x, torch.Tensor):
             raise TypeError("x must be a tensor")
         if _dual_level() >= 0:
