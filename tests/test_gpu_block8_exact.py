@@ -458,3 +458,53 @@ def test_the_largest_number_of_vectors():
     dy[0, 3], dy[n - 1, 7], dy[n - 1, 0], dy[2 ** 30, 5] = 1, 2, 3, 4
     dx = A.product_t(dy)
     assert int(torch.count_nonzero(dx)) == 3 and [float(dx[k, 0]) for k in (0, n - 1, 2 ** 30)] == [1, 5, 4]
+
+
+# ---- every number ---------------------------------------------------------------------------------------------------
+
+def _same_numbers(got, want):
+    """equal, NaN where NaN"""
+    got = got.double().cpu().numpy()
+    assert got.shape == want.shape and np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    assert np.array_equal(got[ok], want[ok]), (int((got[ok] != want[ok]).sum()), got[ok][got[ok] != want[ok]][:3], want[ok][got[ok] != want[ok]][:3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_number_to_8_bits(dtype):
+    """all 16-bit numbers (of fp32 a million bit patterns), alone and beside larger ones that set the scale"""
+    if dtype == F32:
+        g = torch.Generator().manual_seed(1)
+        bits = torch.randint(-2 ** 31, 2 ** 31, (1 << 20,), generator=g).to(torch.int32)
+        bits[:1 << 19] &= ~0xfffff                           # near the borders of 8 bits
+        x = bits.view(F32)
+    else:
+        x = torch.arange(-2 ** 15, 2 ** 15).to(torch.int16).view(dtype)
+    for up in (0, 1, 4, 9, 18):
+        big = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).double()
+        beside = torch.minimum(big * 1.5 * 2.0 ** up, torch.full_like(big, torch.finfo(dtype).max)).to(dtype) if up else torch.zeros_like(x)
+        v = torch.stack((x, beside), 1)
+        q = quantize(v.to(DEV))
+        want, b = O.quantize(v.double().numpy())
+        assert np.array_equal(q.scale.cpu().numpy(), b)
+        _same_numbers(q.values.view(torch.float8_e4m3fn), want)
+        A = Block8.full(1, 2)                                # rounded inside the product: the same
+        w = torch.zeros(1, 128, 128)
+        w[0, 0, 0] = 1
+        A.set_values(w.to(DEV))
+        ok = torch.isfinite(v).all(1) & torch.from_numpy(b[0] >= 4)
+        y = torch.cat([A.product(p, F32) for p in v[ok].to(DEV).split(1024)])
+        exact = O.quantized(v[ok].double().numpy())[:, :1]
+        _same_numbers(y, np.where(np.abs(exact) > torch.finfo(F32).max, np.copysign(np.inf, exact), exact))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_code_back(dtype):
+    """256 codes times 247 scales; past the type's largest number that number"""
+    code, byte = torch.arange(256, dtype=torch.uint8), torch.arange(1, 248, dtype=torch.uint8)
+    q = Packed8(code.repeat(247, 1).to(DEV), byte.repeat(2, 1).contiguous().to(DEV), 256, dtype)
+    want = O.decode(code.numpy())[None] * np.exp2(byte.numpy().astype(np.float64) - 127)[:, None]
+    top = torch.finfo(dtype).max
+    with np.errstate(invalid="ignore"):
+        want = torch.from_numpy(np.clip(want, -top, top)).to(dtype).double().numpy()
+    _same_numbers(q.restore(), want)
