@@ -1,11 +1,12 @@
 #!/bin/bash
 # Kernel times of every case of perf/operators.py, and counters of the three products of the training batch: rocprofv3 passes around
-# tools/block8_profile.py.  Output: gpurun_out/block8_kernel_times.txt and gpurun_out/block8_counters.txt.
+# tools/block8_profile.py.
+#   tools/profile_block8.sh DIR    -> DIR/block8_kernel_times.txt, DIR/block8_counters.txt
 # Each pass holds at most 8 SQ, 4 TCC, 4 TCP and 2 GRBM counters and runs under its own time limit; the script stops at the first failure.
 set -e
 root=$(cd "$(dirname "$0")/.." && pwd)
-out=$root/gpurun_out
-mkdir -p "$out"
+mkdir -p "$1"
+out=$(cd "$1" && pwd)
 cd /tmp && export TMPDIR=/tmp
 tool=$root/tools/block8_profile.py
 timeout -s KILL 150 rocprofv3 --kernel-trace --stats -M -f csv -d "$out/block8_trace" -o p -- python3 "$tool" run > "$out/block8_trace.log" 2>&1
